@@ -44,7 +44,9 @@ enum {
   MIT2CFM_E_INTERNAL = 4  /* anything else                                   */
 };
 
-enum { MIT2CFM_DTYPE_F32 = 0, MIT2CFM_DTYPE_F16 = 1 };
+/* Weight tensors are f32 or f16; bf16 is a type of the cache operators and of
+ * the beam selection's logits (kv_*, beam_* below). */
+enum { MIT2CFM_DTYPE_F32 = 0, MIT2CFM_DTYPE_F16 = 1, MIT2CFM_DTYPE_BF16 = 2 };
 
 /* One named host tensor (element count, f32 or f16 payload). */
 typedef struct {
@@ -523,6 +525,164 @@ mit2cfm_status mit2cfm_gpt_get_counts(mit2cfm_ctx* ctx, mit2cfm_gpt_counts* coun
  * counterpart. */
 mit2cfm_status mit2cfm_gpt_profile_launch(mit2cfm_ctx* ctx, int32_t kernel, uint32_t count,
                                           double* bytes_per_launch, const char** name);
+
+/* ---- a paged key/value cache and its operators ------------------------------
+ * For decoding several sequences, hypotheses or drafted continuations over
+ * shared pages, beside the one-sequence GPT calls above.  All pointers are
+ * DEVICE pointers; work is enqueued on the context's stream (flags as for
+ * mit2cfm_decode_device) and nothing is allocated, so the calls may be captured
+ * into a graph.  Sizes that change from step to step (start, length, parent
+ * ..) are read on the device.  A call needs no tensors of its own in the
+ * context.  No reference counterpart (its decoder holds one sequence,
+ * runtime/impl/gpt.cpp:1914). */
+
+/* One layer's cache: pages of page_rows rows each, k and v
+ * [pages][kv_heads][page_rows][head_dim], 16-byte aligned.  table
+ * [seqs][table_stride] names the page of rows page_rows * j .. of a sequence.
+ * An entry outside 0 .. pages - 1 is no page: rows that fall there are not
+ * written, and nobody sees them. */
+typedef struct mit2cfm_kv_cache {
+  void* k;
+  void* v;
+  const int32_t* table;
+  uint32_t pages;
+  uint32_t page_rows;    /* a power of two, 1 .. 1024 */
+  uint32_t kv_heads;     /* 1 .. 1024 */
+  uint32_t head_dim;     /* 32, 64, 96, 128, 192 or 256 */
+  uint32_t table_stride; /* entries of a table row; page_rows * table_stride < 2^31 */
+  int32_t dtype;         /* MIT2CFM_DTYPE_F32, _F16 or _BF16: of the cache and of every row given with it */
+} mit2cfm_kv_cache;
+
+/* The new rows of a batch of sequences: rows start[s] .. start[s + 1] - 1 are
+ * sequence s's, in order (start does not decrease; a sequence may have none);
+ * rows of the buffers outside start[0] .. start[seqs] - 1 are left alone.
+ * length[s] counts the rows of the sequence's cache with its new ones, which
+ * are its last. */
+typedef struct mit2cfm_kv_rows {
+  const int32_t* start;  /* [seqs + 1] */
+  const int32_t* length; /* [seqs] */
+  uint32_t seqs;         /* 0 .. 65535 */
+  uint32_t rows;         /* rows the buffers hold, below 2^24; start[seqs] <= rows */
+  uint32_t max_length;   /* about the largest length: the work is split by it (any value is right) */
+} mit2cfm_kv_rows;
+
+/* Appends the new rows' keys and values to the cache, the keys rotated to their
+ * positions, and rotates the queries that go with them: for pair i of the first
+ * rotary_dim elements of a head, a = position * theta^(-2 i / rotary_dim),
+ *   (x, y) -> (x cos a - y sin a, y cos a + x sin a),
+ * pairs (2 i, 2 i + 1) when interleaved (the estimator's form,
+ * dit_cfm_bigvgan.cpp:469), else (i, i + rotary_dim / 2).  Angles are formed in
+ * 64 bits.  Strides are in elements; each head's elements are contiguous. */
+typedef struct mit2cfm_kv_append {
+  const void* k; /* [rows][kv_heads][head_dim] by k_row, k_head */
+  const void* v;
+  uint64_t k_row, k_head, v_row, v_head;
+  const void* q; /* [rows][q_heads][head_dim] by q_row, q_head; NULL: none */
+  void* q_out;   /* may be q itself, with its strides; no other overlap */
+  uint64_t q_row, q_head, q_out_row, q_out_head;
+  uint32_t q_heads;        /* 0 .. 4096 */
+  const int32_t* position; /* [rows]; NULL: a row's place in its sequence */
+  uint32_t rotary_dim;     /* even, <= head_dim; 0: no rotation (the GPT decoder's) */
+  int32_t interleaved;
+  double theta; /* > 0 */
+} mit2cfm_kv_append;
+mit2cfm_status mit2cfm_kv_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                        const mit2cfm_kv_rows* rows, const mit2cfm_kv_append* append,
+                                        uint32_t flags);
+
+/* Attention of the new rows (appended before) over their sequences' caches:
+ *   out = sum_j p_j v_j, p = softmax over the visible keys j of scale * q . k_j,
+ * query head h on key head h / (q_heads / kv_heads).  Every row sees the keys
+ * before its sequence's new rows.  Of the new rows, row i sees row j when bit
+ * j % 32 of mask[row][j / 32] is set (a tree of drafted tokens: the row's path
+ * from the root); without a mask, when j <= i (one token, or a chain).  A row
+ * that sees nothing, or only scores of -inf, gives 0.  What lies in places a
+ * row does not see, NaN and infinities too, does not change it.  Sums and the
+ * softmax are fp32; with 16-bit types the products run on the matrix cores,
+ * with the probabilities rounded to the type. */
+typedef struct mit2cfm_kv_attention {
+  const void* q; /* [rows][q_heads][head_dim] by q_row, q_head */
+  void* out;     /* the same by out_row, out_head; no overlap with q */
+  uint64_t q_row, q_head, out_row, out_head;
+  uint32_t q_heads; /* a multiple of kv_heads, <= 4096 */
+  float scale;      /* finite */
+  const uint32_t* mask;
+  uint32_t mask_words; /* words of a mask row: new rows from 32 * mask_words on are seen by none */
+  void* workspace;     /* 16-byte aligned, of mit2cfm_kv_attention_workspace bytes; calls that may
+                        * run at the same time need one each */
+  uint64_t workspace_bytes;
+} mit2cfm_kv_attention;
+/* 0 where no workspace is needed or an argument is out of its range. */
+uint64_t mit2cfm_kv_attention_workspace(const mit2cfm_kv_cache* cache, const mit2cfm_kv_rows* rows,
+                                        uint32_t q_heads);
+mit2cfm_status mit2cfm_kv_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                           const mit2cfm_kv_rows* rows, const mit2cfm_kv_attention* attention,
+                                           uint32_t flags);
+
+/* ---- beam search --------------------------------------------------------------
+ * (See the paged cache above for what holds of every call.)  groups searches
+ * of `beams` hypotheses each. */
+
+/* A step's best continuations: of every group's beams x vocab candidates, with
+ *   scores[b] + logits[b][t] - log(sum_u exp(logits[b][u])),
+ * the `count` largest, in order; of equal ones the lowest (b, t) first.  A NaN
+ * logit counts as -inf, +inf as the largest finite value.  A finished
+ * beam offers stop_token alone, at its unchanged score (its other candidates
+ * count as -inf).  Candidates of -inf fill the list when others run out.
+ * count = beams keeps a search going; 2 * beams leaves as many after stop
+ * tokens are taken out.  Sums are fp64 of fp32 terms, candidates compared in
+ * fp64. */
+typedef struct mit2cfm_beam_select {
+  const void* logits; /* [groups * beams][vocab], rows logits_row elements apart */
+  uint64_t logits_row;
+  int32_t dtype; /* MIT2CFM_DTYPE_* */
+  uint32_t groups;
+  uint32_t beams;           /* 1 .. 64 */
+  uint32_t vocab;           /* 1 .. 2^24 */
+  uint32_t count;           /* 1 .. 64, <= beams * vocab */
+  const float* scores;      /* [groups][beams]; -inf: a beam that does not exist yet */
+  const int32_t* finished;  /* [groups][beams], nonzero: finished; NULL: none */
+  int32_t stop_token;       /* 0 .. vocab - 1, or -1 for none (finished is NULL then) */
+  float* scores_out;        /* [groups][count] */
+  int32_t* parent_out;      /* the beam it continues, 0 .. beams - 1 */
+  int32_t* token_out;
+  int32_t* finished_out;    /* the parent was finished, or the token is the stop token; may be NULL */
+  void* workspace;          /* 16-byte aligned, of mit2cfm_beam_select_workspace bytes; calls that may
+                             * run at the same time need one each */
+  uint64_t workspace_bytes;
+} mit2cfm_beam_select;
+uint64_t mit2cfm_beam_select_workspace(const mit2cfm_beam_select* select); /* 0: an argument out of range */
+mit2cfm_status mit2cfm_beam_select_device(mit2cfm_ctx* ctx, const mit2cfm_beam_select* select, uint32_t flags);
+
+/* The states of new beams r from those of their parents.  The cache's table
+ * [groups * beams][table_stride] goes to table_out: rows of full pages
+ * (j < length / page_rows) follow the parent, whose pages its children then
+ * share; the pages from there on are private.  A parent's first child keeps
+ * them, each further child in turn takes those of the next beam without
+ * children, and the rows of the part page, length % page_rows, are copied there
+ * in every layer.  No page is lost or shared that will be written, as long
+ * as each group's private pages differ at the start.  A parent
+ * outside 0 .. beams - 1 counts as the beam itself.  A length that is negative
+ * or past the table counts as its end.  Rows of states (token histories or
+ * others, of 32-bit words) follow their parents; with token and place, the
+ * word at place[g] becomes token (a place outside the row writes none). */
+typedef struct mit2cfm_beam_reorder {
+  uint32_t groups;
+  uint32_t beams;         /* 1 .. 64 */
+  uint32_t layers;        /* >= 1; the cache's k and v are the first's */
+  uint64_t layer_stride;  /* elements from a layer's k (v) to the next's: a multiple of 8 */
+  const int32_t* parent;  /* [groups][beams], rows parent_stride apart */
+  uint32_t parent_stride; /* >= beams */
+  const int32_t* length;  /* [groups]: rows every beam of the group has cached */
+  int32_t* table_out;     /* no overlap with the cache's table */
+  const uint32_t* state;  /* [groups * beams][state_words]; NULL: none */
+  uint32_t* state_out;    /* no overlap with state */
+  uint32_t state_words;
+  const uint32_t* token; /* [groups][beams], rows parent_stride apart; NULL: none */
+  const int32_t* place;  /* [groups] */
+} mit2cfm_beam_reorder;
+mit2cfm_status mit2cfm_beam_reorder_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                           const mit2cfm_beam_reorder* reorder, uint32_t flags);
 
 #ifdef __cplusplus
 }

@@ -10,8 +10,10 @@
 
 #include "../runtime/bundle.h"
 #include "../runtime/synth.h"
+#include "beam_ops.h"
 #include "engine.h"
 #include "gpt.h"
+#include "kv_ops.h"
 #include "vocoder.h"
 
 struct mit2cfm_ctx {
@@ -121,6 +123,28 @@ void host_decode(mit2cfm_ctx* c, uint32_t nreq, uint32_t T, const uint32_t* vali
   hip_check(hipMemcpyAsync(x_out, d_out, nx * 4, hipMemcpyDeviceToHost, s), "copy x_out");
   if (v_trace) hip_check(hipMemcpyAsync(v_trace, d_v, nv * 4, hipMemcpyDeviceToHost, s), "copy v");
   c->eng->sync();
+}
+
+// An operator on the context's stream and device; the caller's current device
+// stays as it was.
+template <typename F>
+mit2cfm_status on_stream(mit2cfm_ctx* ctx, uint32_t flags, bool given, const char* missing, F&& f) {
+  if (!ctx) return fail(nullptr, MIT2CFM_E_ARG, "ctx must not be NULL");
+  return guarded(ctx, [&] {
+    require(given, missing);
+    int before = 0;
+    hip_check(hipGetDevice(&before), "hipGetDevice");
+    const int device = ctx->eng->device();
+    struct Back {
+      int to;
+      ~Back() {
+        if (to >= 0) (void)hipSetDevice(to);
+      }
+    } back{before != device ? before : -1};
+    if (before != device) hip_check(hipSetDevice(device), "hipSetDevice");
+    f(ctx->eng->stream());
+    if (flags & MIT2CFM_FLAG_SYNC) hip_check(hipStreamSynchronize(ctx->eng->stream()), "hipStreamSynchronize");
+  });
 }
 
 // Packs a single request's [P][80] prompt into [T][80].
@@ -633,6 +657,41 @@ mit2cfm_status mit2cfm_write_synthetic_bundle(const char* dir, uint64_t base_see
                     mit2::synth_tensor_bytes(i, base_seed, stddev)});
     mit2::write_bundle(dir, ts);
   });
+}
+
+// ---- paged key/value cache and beam search
+uint64_t mit2cfm_kv_attention_workspace(const mit2cfm_kv_cache* cache, const mit2cfm_kv_rows* rows,
+                                        uint32_t q_heads) {
+  return cache && rows ? mit2hip::kv_attention_workspace(*cache, *rows, q_heads) : 0;
+}
+
+mit2cfm_status mit2cfm_kv_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                        const mit2cfm_kv_rows* rows, const mit2cfm_kv_append* append,
+                                        uint32_t flags) {
+  return on_stream(ctx, flags, cache && rows && append, "cache, rows and append must not be NULL",
+                   [&](hipStream_t s) { mit2hip::kv_append(*cache, *rows, *append, s); });
+}
+
+mit2cfm_status mit2cfm_kv_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                           const mit2cfm_kv_rows* rows, const mit2cfm_kv_attention* attention,
+                                           uint32_t flags) {
+  return on_stream(ctx, flags, cache && rows && attention, "cache, rows and attention must not be NULL",
+                   [&](hipStream_t s) { mit2hip::kv_attention(*cache, *rows, *attention, s); });
+}
+
+uint64_t mit2cfm_beam_select_workspace(const mit2cfm_beam_select* select) {
+  return select ? mit2hip::beam_select_workspace(*select) : 0;
+}
+
+mit2cfm_status mit2cfm_beam_select_device(mit2cfm_ctx* ctx, const mit2cfm_beam_select* select, uint32_t flags) {
+  return on_stream(ctx, flags, select != nullptr, "select must not be NULL",
+                   [&](hipStream_t s) { mit2hip::beam_select(*select, s); });
+}
+
+mit2cfm_status mit2cfm_beam_reorder_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                           const mit2cfm_beam_reorder* reorder, uint32_t flags) {
+  return on_stream(ctx, flags, cache && reorder, "cache and reorder must not be NULL",
+                   [&](hipStream_t s) { mit2hip::beam_reorder(*cache, *reorder, s); });
 }
 
 }  // extern "C"

@@ -1,0 +1,437 @@
+// kv_ops.hip -- operators over a paged key/value cache (see kv_ops.h and
+// mit2cfm.h for what they compute).
+#include "kv_ops.h"
+
+#include <cmath>
+#include <stdexcept>
+#include <string>
+
+#include "device_common.h"
+#include "engine.h"
+
+namespace mit2hip {
+
+namespace {
+
+typedef __bf16 bf16_t;
+
+void need(bool ok, const char* what) {
+  if (!ok) throw std::invalid_argument(what);
+}
+void launched(hipError_t e) {
+  if (e != hipSuccess) throw HipError(std::string("kv operator launch: ") + hipGetErrorString(e));
+}
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// What the kernels take of a cache and of its new rows.
+struct CacheView {
+  char* k;
+  char* v;
+  const int32_t* table;
+  int pages, page_shift, kv_heads, table_stride;
+
+  // Page that holds a sequence's cached row j (0 <= j < capacity()), or -1.
+  __device__ int page_of(int seq, int j) const {
+    const int p = table[(size_t)seq * table_stride + (j >> page_shift)];
+    return (unsigned)p < (unsigned)pages ? p : -1;
+  }
+  __device__ int capacity() const { return table_stride << page_shift; }
+  // Element index of head 0's row j in a page.
+  __device__ int64_t row_in(int page, int j, int D) const {
+    return ((((int64_t)page * kv_heads) << page_shift) + (j & ((1 << page_shift) - 1))) * D;
+  }
+  __device__ int64_t head_stride(int D) const { return (int64_t)D << page_shift; }
+};
+struct RowView {
+  const int32_t* start;
+  const int32_t* length;
+  int seqs, rows;
+};
+
+CacheView view(const mit2cfm_kv_cache& c) {
+  return {static_cast<char*>(c.k), static_cast<char*>(c.v), c.table, (int)c.pages,
+          __builtin_ctz(c.page_rows), (int)c.kv_heads, (int)c.table_stride};
+}
+RowView view(const mit2cfm_kv_rows& r) { return {r.start, r.length, (int)r.seqs, (int)r.rows}; }
+
+// The sequence that new row `row` belongs to, or -1 (a wave's lanes look at 64
+// bounds at a time; all return the same).
+__device__ __forceinline__ int seq_of_row(const RowView& r, int row) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int base = 0; base < r.seqs; base += 64) {
+    const bool before = base + lane < r.seqs && r.start[base + lane + 1] <= row;
+    const int c = __popcll(__ballot(before));
+    n += c;
+    if (c < 64) break;
+  }
+  return n < r.seqs && row >= r.start[n] ? n : -1;
+}
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+// ------------------------------------------------------------------ append
+constexpr int kAppendThreads = 256;
+constexpr int kMaxPairs = 128;  // rotated pairs of a head
+
+struct AppendArgs {
+  CacheView c;
+  RowView r;
+  const char *k, *v, *q;
+  char* q_out;
+  int64_t k_row, k_head, v_row, v_head, q_row, q_head, qo_row, qo_head;
+  const int32_t* position;
+  int q_heads, rot, interleaved;
+  double log2_theta;
+};
+
+// A block takes R rows' items (blockIdx.y: its share of them).  An item is two
+// vectors of VEC elements of a head, chosen so that a rotated pair's two
+// elements are both in it: (i, i + rot/2), or neighbours when interleaved and
+// past the rotated part.  The rows' angles go through LDS once for all heads:
+// the angle in turns, fp64, brought to [-1/2, 1/2] there, and its cosine and
+// sine in fp32, as everything that follows.
+template <typename T, int VEC, int R>
+__global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, int D) {
+  __shared__ float2 turn[R][kMaxPairs];
+  __shared__ int64_t s_at[R];  // element index of the row in its page, head 0; -1: not written
+  __shared__ int s_place[R];   // the row's position; INT_MIN: no sequence's row
+  const int tid = threadIdx.x, row0 = blockIdx.x * R;
+  const int wave = tid >> 6;
+  for (int i = wave; i < R; i += kAppendThreads / 64) {
+    const int row = row0 + i;
+    const int seq = row < a.r.rows ? seq_of_row(a.r, row) : -1;
+    if ((tid & 63) == 0) {
+      int64_t at = -1;
+      int pos = INT_MIN;
+      if (seq >= 0) {
+        const int place = a.r.length[seq] - (a.r.start[seq + 1] - row);
+        if (place >= 0 && place < a.c.capacity()) {
+          const int page = a.c.page_of(seq, place);
+          if (page >= 0) at = a.c.row_in(page, place, D);
+        }
+        pos = a.position ? a.position[row] : place;
+        if (pos == INT_MIN) pos = INT_MIN + 1;
+      }
+      s_at[i] = at;
+      s_place[i] = pos;
+    }
+  }
+  __syncthreads();
+  const int half = a.rot >> 1;
+  for (int i = tid; i < R * half; i += kAppendThreads) {
+    const int rr = i / half, p = i - rr * half;
+    const double inv = exp2(-2.0 * p / a.rot * a.log2_theta) * 0.15915494309189533577;  // 1 / (2 pi)
+    double t = (double)s_place[rr] * inv;
+    t -= rint(t);
+    float sn, cs;
+    sincospif((float)(2.0 * t), &sn, &cs);
+    turn[rr][p] = make_float2(cs, sn);
+  }
+  __syncthreads();
+  const int per_head = D / (2 * VEC);
+  const int heads = a.q_heads + 2 * a.c.kv_heads;
+  const int items = R * heads * per_head;
+  for (int it = blockIdx.y * kAppendThreads + tid; it < items; it += gridDim.y * kAppendThreads) {
+    const int u = it % per_head, rh = it / per_head;
+    const int h = rh % heads, rr = rh / heads;
+    if (s_place[rr] == INT_MIN) continue;
+    const int row = row0 + rr;
+    // the item's two vectors, and the pair index of its first element
+    int e0, e1, pair0;
+    const bool rotates = h < a.q_heads + a.c.kv_heads;
+    bool turned = false;
+    if (a.interleaved || !rotates) {
+      e0 = 2 * VEC * u;
+      e1 = e0 + VEC;
+      pair0 = VEC * u;
+      turned = rotates && e0 < a.rot;
+    } else if (u * VEC < half) {
+      e0 = pair0 = VEC * u;
+      e1 = e0 + half;
+      turned = true;
+    } else {
+      e0 = a.rot + 2 * (VEC * u - half);
+      e1 = e0 + VEC;
+      pair0 = 0;
+    }
+    const T* src;
+    T* dst;
+    if (h < a.q_heads) {
+      src = reinterpret_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
+      dst = reinterpret_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head;
+    } else {
+      if (s_at[rr] < 0) continue;
+      const int kh = h - a.q_heads;
+      const bool is_k = kh < a.c.kv_heads;
+      const int hh = is_k ? kh : kh - a.c.kv_heads;
+      src = is_k ? reinterpret_cast<const T*>(a.k) + row * a.k_row + hh * a.k_head
+                 : reinterpret_cast<const T*>(a.v) + row * a.v_row + hh * a.v_head;
+      dst = reinterpret_cast<T*>(is_k ? a.c.k : a.c.v) + s_at[rr] + hh * a.c.head_stride(D);
+    }
+    Vec<T, VEC> x = *reinterpret_cast<const Vec<T, VEC>*>(src + e0);
+    Vec<T, VEC> y = *reinterpret_cast<const Vec<T, VEC>*>(src + e1);
+    if (turned) {
+      if (a.interleaved) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          // pair j of the item: elements 2 j, 2 j + 1 of (x, y)
+          T& p = 2 * j < VEC ? x.v[(2 * j) % VEC] : y.v[(2 * j) % VEC];
+          T& q = 2 * j + 1 < VEC ? x.v[(2 * j + 1) % VEC] : y.v[(2 * j + 1) % VEC];
+          if (pair0 + j < half) {
+            const float2 cs = turn[rr][pair0 + j];
+            const float fp = (float)p, fq = (float)q;
+            p = (T)(fp * cs.x - fq * cs.y);
+            q = (T)(fq * cs.x + fp * cs.y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float2 cs = turn[rr][pair0 + j];
+          const float fp = (float)x.v[j], fq = (float)y.v[j];
+          x.v[j] = (T)(fp * cs.x - fq * cs.y);
+          y.v[j] = (T)(fq * cs.x + fp * cs.y);
+        }
+      }
+    }
+    *reinterpret_cast<Vec<T, VEC>*>(dst + e0) = x;
+    *reinterpret_cast<Vec<T, VEC>*>(dst + e1) = y;
+  }
+}
+
+template <typename T, int VEC, int R>
+void launch_append_rows(const AppendArgs& a, int D, hipStream_t s) {
+  const int bx = (a.r.rows + R - 1) / R;
+  const int items = R * (a.q_heads + 2 * a.c.kv_heads) * (D / (2 * VEC));
+  // few rows: their heads over more blocks, down to one item a thread
+  const int by = std::max(1, std::min((items + kAppendThreads - 1) / kAppendThreads, 2048 / bx));
+  hipLaunchKernelGGL((append_kernel<T, VEC, R>), dim3(bx, by), dim3(kAppendThreads), 0, s, a, D);
+  launched(hipGetLastError());
+}
+
+template <typename T>
+void launch_append(const AppendArgs& a, int D, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  auto fits = [&](const void* p, int64_t row, int64_t head) { return aligned(p, 16) && row % V == 0 && head % V == 0; };
+  const bool wide = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head) &&
+                    (!a.q_heads || (fits(a.q, a.q_row, a.q_head) && fits(a.q_out, a.qo_row, a.qo_head))) &&
+                    (a.interleaved || a.rot % (2 * V) == 0);
+  // Rows that fill the chip by themselves share a block's angles four at a time.
+  if (!wide)
+    launch_append_rows<T, 1, 1>(a, D, s);
+  else if (a.r.rows >= 2048)
+    launch_append_rows<T, V, 4>(a, D, s);
+  else
+    launch_append_rows<T, V, 1>(a, D, s);
+}
+
+// ------------------------------------------------------------------ attention
+struct AttendArgs {
+  CacheView c;
+  RowView r;
+  const char* q;
+  char* out;
+  int64_t q_row, q_head, o_row, o_head;
+  const uint32_t* mask;
+  int mask_words, q_heads, group;
+  float scale;
+};
+
+// Whether a sequence's new row i sees cached row j; first: its cached rows
+// before the new ones.
+__device__ __forceinline__ bool sees(const AttendArgs& a, int row, int i, int j, int first) {
+  const int n = j - first;
+  if (n < 0) return true;
+  if (!a.mask) return n <= i;
+  return (n >> 5) < a.mask_words && (a.mask[(size_t)row * a.mask_words + (n >> 5)] >> (n & 31) & 1u);
+}
+
+// One wave a row and query head, fp32: its lanes take a key each.
+template <typename T, int D>
+__global__ __launch_bounds__(64) void attend_simple_kernel(AttendArgs a) {
+  __shared__ float sq[D], so[D], sp[64];
+  __shared__ int64_t sat[64];
+  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+  const int seq = seq_of_row(a.r, row);
+  if (seq < 0) return;
+  const int i = row - a.r.start[seq], n_new = a.r.start[seq + 1] - a.r.start[seq];
+  const int first = a.r.length[seq] - n_new, len = min(a.r.length[seq], a.c.capacity());
+  const T* q = reinterpret_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
+  for (int d = lane; d < D; d += 64) {
+    sq[d] = (float)q[d] * a.scale;
+    so[d] = 0.f;
+  }
+  __syncthreads();
+  const int64_t head = (h / a.group) * a.c.head_stride(D);
+  const T* K = reinterpret_cast<const T*>(a.c.k) + head;
+  const T* V = reinterpret_cast<const T*>(a.c.v) + head;
+  float m = -INFINITY, l = 0.f;
+  for (int j0 = 0; j0 < len; j0 += 64) {
+    const int j = j0 + lane;
+    float sc = -INFINITY;
+    int64_t at = -1;
+    if (j < len && sees(a, row, i, j, first)) {
+      const int page = a.c.page_of(seq, j);
+      if (page >= 0) {
+        at = a.c.row_in(page, j, D);
+        sc = 0.f;
+        for (int d = 0; d < D; ++d) sc += sq[d] * (float)K[at + d];
+      }
+    }
+    float t = sc;
+#pragma unroll
+    for (int off = 32; off; off >>= 1) t = fmaxf(t, __shfl_xor(t, off, kWave));
+    const float mn = fmaxf(m, t), ms = mn == -INFINITY ? 0.f : mn;
+    const float alpha = expf(m - ms), p = at >= 0 ? expf(sc - ms) : 0.f;
+    l = l * alpha + warp_sum(p);
+    m = mn;
+    sp[lane] = p;
+    sat[lane] = at;
+    __syncthreads();
+    for (int d = lane; d < D; d += 64) {
+      float o = so[d] * alpha;
+      for (int e = 0; e < 64; ++e)
+        if (sat[e] >= 0) o += sp[e] * (float)V[sat[e] + d];
+      so[d] = o;
+    }
+    __syncthreads();
+  }
+  T* o = reinterpret_cast<T*>(a.out) + row * a.o_row + h * a.o_head;
+  for (int d = lane; d < D; d += 64) o[d] = (T)(l == 0.f ? 0.f : so[d] / l);
+}
+
+template <typename T, int D>
+void launch_attend(const AttendArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((attend_simple_kernel<T, D>), dim3(a.r.rows, a.q_heads), dim3(64), 0, s, a);
+  launched(hipGetLastError());
+}
+
+template <typename T>
+void launch_attend_dim(const AttendArgs& a, int D, hipStream_t s) {
+  switch (D) {
+    case 32: return launch_attend<T, 32>(a, s);
+    case 64: return launch_attend<T, 64>(a, s);
+    case 96: return launch_attend<T, 96>(a, s);
+    case 128: return launch_attend<T, 128>(a, s);
+    case 192: return launch_attend<T, 192>(a, s);
+    case 256: return launch_attend<T, 256>(a, s);
+  }
+}
+
+void check_rows(const mit2cfm_kv_rows& r) {
+  need(r.seqs <= 65535, "seqs must be <= 65535");
+  need(r.rows < (1u << 24), "rows must be below 2^24");
+  need(r.seqs == 0 || r.rows == 0 || (r.start && r.length), "start and length must not be NULL");
+}
+
+// An output's rows and heads must not lie on one another.
+void check_out(uint64_t row, uint64_t head, uint32_t rows, uint32_t heads, uint32_t D, const char* what) {
+  need((heads <= 1 || head >= D) && (rows <= 1 || row >= D), what);
+}
+
+}  // namespace
+
+int kv_elem_bytes(int32_t dtype) { return dtype == MIT2CFM_DTYPE_F32 ? 4 : 2; }
+
+void check_kv_cache(const mit2cfm_kv_cache& c) {
+  need(c.dtype >= MIT2CFM_DTYPE_F32 && c.dtype <= MIT2CFM_DTYPE_BF16, "the cache's dtype must be f32, f16 or bf16");
+  need(c.page_rows >= 1 && c.page_rows <= 1024 && (c.page_rows & (c.page_rows - 1)) == 0,
+       "page_rows must be a power of two in [1, 1024]");
+  need(c.kv_heads >= 1 && c.kv_heads <= 1024, "kv_heads must be in [1, 1024]");
+  need(c.head_dim == 32 || c.head_dim == 64 || c.head_dim == 96 || c.head_dim == 128 || c.head_dim == 192 ||
+           c.head_dim == 256,
+       "head_dim must be 32, 64, 96, 128, 192 or 256");
+  need(c.pages >= 1 && c.pages < (1u << 31), "pages must be in [1, 2^31)");
+  need(c.table_stride >= 1 && (uint64_t)c.table_stride * c.page_rows < (1ull << 31),
+       "table_stride must be >= 1, page_rows * table_stride below 2^31");
+  need(c.k && c.v && c.table, "the cache's k, v and table must not be NULL");
+  need(aligned(c.k, 16) && aligned(c.v, 16), "the cache's k and v must be 16-byte aligned");
+}
+
+void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_append& p, hipStream_t s) {
+  check_kv_cache(c);
+  check_rows(r);
+  need(p.q_heads <= 4096, "q_heads must be <= 4096");
+  need(p.rotary_dim <= c.head_dim && p.rotary_dim % 2 == 0, "rotary_dim must be even and <= head_dim");
+  need(p.rotary_dim == 0 || (p.theta > 0.0 && std::isfinite(p.theta)), "theta must be positive and finite");
+  if (r.seqs == 0 || r.rows == 0) return;
+  const bool with_q = p.q != nullptr;
+  need(p.k && p.v, "k and v must not be NULL");
+  need(!with_q || (p.q_out && p.q_heads > 0), "q needs q_out and q_heads");
+  const size_t e = (size_t)kv_elem_bytes(c.dtype);
+  need(aligned(p.k, e) && aligned(p.v, e) && aligned(p.q, e) && aligned(p.q_out, e),
+       "k, v, q and q_out must be aligned to their type");
+  if (with_q) {
+    check_out(p.q_out_row, p.q_out_head, r.rows, p.q_heads, c.head_dim, "q_out's rows and heads overlap");
+    need(p.q != p.q_out || (p.q_row == p.q_out_row && p.q_head == p.q_out_head),
+         "q_out may be q only with its strides");
+  }
+  AppendArgs a;
+  a.c = view(c);
+  a.r = view(r);
+  a.k = static_cast<const char*>(p.k);
+  a.v = static_cast<const char*>(p.v);
+  a.q = static_cast<const char*>(p.q);
+  a.q_out = static_cast<char*>(p.q_out);
+  a.k_row = (int64_t)p.k_row; a.k_head = (int64_t)p.k_head;
+  a.v_row = (int64_t)p.v_row; a.v_head = (int64_t)p.v_head;
+  a.q_row = (int64_t)p.q_row; a.q_head = (int64_t)p.q_head;
+  a.qo_row = (int64_t)p.q_out_row; a.qo_head = (int64_t)p.q_out_head;
+  a.position = p.position;
+  a.q_heads = with_q ? (int)p.q_heads : 0;
+  a.rot = (int)p.rotary_dim;
+  a.interleaved = p.interleaved != 0;
+  a.log2_theta = p.rotary_dim ? std::log2(p.theta) : 0.0;
+  const int D = (int)c.head_dim;
+  if (c.dtype == MIT2CFM_DTYPE_F32)
+    launch_append<float>(a, D, s);
+  else if (c.dtype == MIT2CFM_DTYPE_F16)
+    launch_append<half_t>(a, D, s);
+  else
+    launch_append<bf16_t>(a, D, s);
+}
+
+uint64_t kv_attention_workspace(const mit2cfm_kv_cache&, const mit2cfm_kv_rows&, uint32_t) { return 0; }
+
+void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, hipStream_t s) {
+  check_kv_cache(c);
+  check_rows(r);
+  need(p.q_heads >= 1 && p.q_heads <= 4096 && p.q_heads % c.kv_heads == 0,
+       "q_heads must be a multiple of kv_heads, <= 4096");
+  need(std::isfinite(p.scale), "scale must be finite");
+  need(p.mask == nullptr || p.mask_words >= 1, "mask_words must be >= 1 with a mask");
+  need(p.mask_words < (1u << 24), "mask_words must be below 2^24");
+  if (r.seqs == 0 || r.rows == 0) return;
+  need(p.q && p.out, "q and out must not be NULL");
+  const size_t e = (size_t)kv_elem_bytes(c.dtype);
+  need(aligned(p.q, e) && aligned(p.out, e), "q and out must be aligned to their type");
+  check_out(p.out_row, p.out_head, r.rows, p.q_heads, c.head_dim, "out's rows and heads overlap");
+  const uint64_t bytes = kv_attention_workspace(c, r, p.q_heads);
+  need(bytes == 0 || (p.workspace && p.workspace_bytes >= bytes), "workspace is NULL or too small");
+  need(aligned(p.workspace, 16), "workspace must be 16-byte aligned");
+  AttendArgs a;
+  a.c = view(c);
+  a.r = view(r);
+  a.q = static_cast<const char*>(p.q);
+  a.out = static_cast<char*>(p.out);
+  a.q_row = (int64_t)p.q_row; a.q_head = (int64_t)p.q_head;
+  a.o_row = (int64_t)p.out_row; a.o_head = (int64_t)p.out_head;
+  a.mask = p.mask;
+  a.mask_words = p.mask ? (int)p.mask_words : 0;
+  a.q_heads = (int)p.q_heads;
+  a.group = (int)(p.q_heads / c.kv_heads);
+  a.scale = p.scale;
+  const int D = (int)c.head_dim;
+  if (c.dtype == MIT2CFM_DTYPE_F32)
+    launch_attend_dim<float>(a, D, s);
+  else if (c.dtype == MIT2CFM_DTYPE_F16)
+    launch_attend_dim<half_t>(a, D, s);
+  else
+    launch_attend_dim<bf16_t>(a, D, s);
+}
+
+}  // namespace mit2hip

@@ -22,7 +22,8 @@ HEADER_PATH = PKG_DIR.parent / "include" / "mit2cfm.h"
 PREFIX = "s2mel.net.cfm.estimator."
 
 OK, E_ARG, E_MODEL, E_HIP, E_INTERNAL = 0, 1, 2, 3, 4
-DTYPE_F32, DTYPE_F16 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+DTYPES = {"f32": DTYPE_F32, "f16": DTYPE_F16, "bf16": DTYPE_BF16}  # MIT2CFM_DTYPE_*
 FLAG_SYNC = 1
 STAGES = {"length_regulator": 1, "vocoder": 2}  # MIT2CFM_STAGE_*
 PRECISIONS = {"f16": 0, "f32": 1}  # MIT2CFM_PREC_*
@@ -132,6 +133,14 @@ def lib() -> ctypes.CDLL:
                                        ctypes.POINTER(ctypes.c_double)]),
         "mit2cfm_gpt_profile_launch": (st, [vp, i32, u32, ctypes.POINTER(ctypes.c_double),
                                             ctypes.POINTER(ctypes.c_char_p)]),
+        "mit2cfm_kv_attention_workspace": (u64, [ctypes.POINTER(KvCache), ctypes.POINTER(KvRows), u32]),
+        "mit2cfm_kv_append_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
+                                          ctypes.POINTER(KvAppend), u32]),
+        "mit2cfm_kv_attention_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
+                                             ctypes.POINTER(KvAttention), u32]),
+        "mit2cfm_beam_select_workspace": (u64, [ctypes.POINTER(BeamSelect)]),
+        "mit2cfm_beam_select_device": (st, [vp, ctypes.POINTER(BeamSelect), u32]),
+        "mit2cfm_beam_reorder_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(BeamReorder), u32]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -149,6 +158,68 @@ class _GptCounts(ctypes.Structure):
 class _GptSampling(ctypes.Structure):
     _fields_ = [("seed", ctypes.c_uint64), ("temperature", ctypes.c_float), ("top_k", ctypes.c_uint32),
                 ("top_p", ctypes.c_float), ("repetition_penalty", ctypes.c_float)]
+
+
+# Arguments of the cache and beam operators (mit2cfm.h describes them); pointers
+# are raw device addresses (None: NULL).
+class KvCache(ctypes.Structure):
+    """One layer's paged key/value cache (mit2cfm_kv_cache)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p), ("pages", ctypes.c_uint32),
+                ("page_rows", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("table_stride", ctypes.c_uint32), ("dtype", ctypes.c_int32)]
+
+
+class KvRows(ctypes.Structure):
+    """The new rows of a batch of sequences (mit2cfm_kv_rows)."""
+    _fields_ = [("start", ctypes.c_void_p), ("length", ctypes.c_void_p), ("seqs", ctypes.c_uint32),
+                ("rows", ctypes.c_uint32), ("max_length", ctypes.c_uint32)]
+
+
+class KvAppend(ctypes.Structure):
+    """mit2cfm_kv_append."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_row", ctypes.c_uint64), ("k_head", ctypes.c_uint64),
+                ("v_row", ctypes.c_uint64), ("v_head", ctypes.c_uint64), ("q", ctypes.c_void_p),
+                ("q_out", ctypes.c_void_p), ("q_row", ctypes.c_uint64), ("q_head", ctypes.c_uint64),
+                ("q_out_row", ctypes.c_uint64), ("q_out_head", ctypes.c_uint64), ("q_heads", ctypes.c_uint32),
+                ("position", ctypes.c_void_p), ("rotary_dim", ctypes.c_uint32), ("interleaved", ctypes.c_int32),
+                ("theta", ctypes.c_double)]
+
+
+class KvAttention(ctypes.Structure):
+    """mit2cfm_kv_attention."""
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_row", ctypes.c_uint64), ("q_head", ctypes.c_uint64),
+                ("out_row", ctypes.c_uint64), ("out_head", ctypes.c_uint64), ("q_heads", ctypes.c_uint32),
+                ("scale", ctypes.c_float), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_uint32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class BeamSelect(ctypes.Structure):
+    """mit2cfm_beam_select."""
+    _fields_ = [("logits", ctypes.c_void_p), ("logits_row", ctypes.c_uint64), ("dtype", ctypes.c_int32),
+                ("groups", ctypes.c_uint32), ("beams", ctypes.c_uint32), ("vocab", ctypes.c_uint32),
+                ("count", ctypes.c_uint32), ("scores", ctypes.c_void_p), ("finished", ctypes.c_void_p),
+                ("stop_token", ctypes.c_int32), ("scores_out", ctypes.c_void_p), ("parent_out", ctypes.c_void_p),
+                ("token_out", ctypes.c_void_p), ("finished_out", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class BeamReorder(ctypes.Structure):
+    """mit2cfm_beam_reorder."""
+    _fields_ = [("groups", ctypes.c_uint32), ("beams", ctypes.c_uint32), ("layers", ctypes.c_uint32),
+                ("layer_stride", ctypes.c_uint64), ("parent", ctypes.c_void_p), ("parent_stride", ctypes.c_uint32),
+                ("length", ctypes.c_void_p), ("table_out", ctypes.c_void_p), ("state", ctypes.c_void_p),
+                ("state_out", ctypes.c_void_p), ("state_words", ctypes.c_uint32), ("token", ctypes.c_void_p),
+                ("place", ctypes.c_void_p)]
+
+
+def kv_attention_workspace(cache: KvCache, rows: KvRows, q_heads: int) -> int:
+    """Bytes of workspace that Context.kv_attention_device needs for these sizes."""
+    return int(lib().mit2cfm_kv_attention_workspace(ctypes.byref(cache), ctypes.byref(rows), q_heads))
+
+
+def beam_select_workspace(select: BeamSelect) -> int:
+    """Bytes of workspace that Context.beam_select_device needs for these sizes."""
+    return int(lib().mit2cfm_beam_select_workspace(ctypes.byref(select)))
 
 
 def declared_symbols() -> list[str]:
@@ -731,6 +802,23 @@ class Context:
         nm = ctypes.c_char_p()
         self._c(lib().mit2cfm_gpt_profile_launch(self._h, kernel, count, ctypes.byref(b), ctypes.byref(nm)))
         return nm.value.decode(), float(b.value)
+
+    # -- paged key/value cache and beam search (device buffers, on the context's stream)
+    def kv_append_device(self, cache: KvCache, rows: KvRows, append: KvAppend, sync: bool = False) -> None:
+        """Appends new rows' keys (rotated) and values to a paged cache and rotates their queries."""
+        self._c(lib().mit2cfm_kv_append_device(self._h, cache, rows, append, FLAG_SYNC if sync else 0))
+
+    def kv_attention_device(self, cache: KvCache, rows: KvRows, attention: KvAttention, sync: bool = False) -> None:
+        """Attention of new rows (tokens, chains, trees) over their sequences' paged caches."""
+        self._c(lib().mit2cfm_kv_attention_device(self._h, cache, rows, attention, FLAG_SYNC if sync else 0))
+
+    def beam_select_device(self, select: BeamSelect, sync: bool = False) -> None:
+        """The best continuations of every group's beams."""
+        self._c(lib().mit2cfm_beam_select_device(self._h, select, FLAG_SYNC if sync else 0))
+
+    def beam_reorder_device(self, cache: KvCache, reorder: BeamReorder, sync: bool = False) -> None:
+        """Page tables, part pages and states of new beams from those of their parents."""
+        self._c(lib().mit2cfm_beam_reorder_device(self._h, cache, reorder, FLAG_SYNC if sync else 0))
 
     BIGVGAN_STAGES = {"conv_pre": 0, "upsample": 1, "activation": 2, "resblock": 3, "group": 4, "post": 5,
                       "body": 6}
