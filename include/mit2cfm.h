@@ -636,14 +636,14 @@ typedef struct mit2cfm_beam_select {
   const void* logits; /* [groups * beams][vocab], rows logits_row elements apart */
   uint64_t logits_row;
   int32_t dtype; /* MIT2CFM_DTYPE_* */
-  uint32_t groups;
+  uint32_t groups;          /* groups * beams <= 65535 */
   uint32_t beams;           /* 1 .. 64 */
   uint32_t vocab;           /* 1 .. 2^24 */
   uint32_t count;           /* 1 .. 64, <= beams * vocab */
-  const float* scores;      /* [groups][beams]; -inf: a beam that does not exist yet */
+  const float* scores;      /* [groups][beams], finite, or -inf: a beam that does not exist yet */
   const int32_t* finished;  /* [groups][beams], nonzero: finished; NULL: none */
   int32_t stop_token;       /* 0 .. vocab - 1, or -1 for none (finished is NULL then) */
-  float* scores_out;        /* [groups][count] */
+  float* scores_out;        /* [groups][count]; no overlap with scores */
   int32_t* parent_out;      /* the beam it continues, 0 .. beams - 1 */
   int32_t* token_out;
   int32_t* finished_out;    /* the parent was finished, or the token is the stop token; may be NULL */
@@ -667,7 +667,7 @@ mit2cfm_status mit2cfm_beam_select_device(mit2cfm_ctx* ctx, const mit2cfm_beam_s
  * others, of 32-bit words) follow their parents; with token and place, the
  * word at place[g] becomes token (a place outside the row writes none). */
 typedef struct mit2cfm_beam_reorder {
-  uint32_t groups;
+  uint32_t groups;        /* groups * beams <= 2^20 */
   uint32_t beams;         /* 1 .. 64 */
   uint32_t layers;        /* >= 1; the cache's k and v are the first's */
   uint64_t layer_stride;  /* elements from a layer's k (v) to the next's: a multiple of 8 */

@@ -2,6 +2,7 @@
 // the operators compute).
 #include "beam_ops.h"
 
+#include <algorithm>
 #include <cfloat>
 #include <stdexcept>
 #include <string>
@@ -30,18 +31,20 @@ constexpr int kMaxBeams = 64, kMaxCount = 64;
 struct SelectArgs {
   const void* logits;
   int64_t row;
-  int groups, beams, vocab, count, stop;
+  int beams, vocab, count, stop;
+  int splits, chunk;  // of a row's logits: chunk of them, a multiple of 8, a block
   const float* scores;
   const int32_t* finished;
   float* scores_out;
   int32_t *parent_out, *token_out, *finished_out;
-  double* sums;   // workspace: [rows] sum of exp(x - max)
-  float* tops;    // [rows] max
-  float* cand_x;  // [rows][count] the row's best logits, in order
-  int32_t* cand_t;
+  double* sums;    // workspace: [rows][splits] sum of exp(x - max)
+  uint64_t* cand;  // [rows][splits][count] the split's best logits, as rank keys
+  float* tops;     // [rows][splits] max
 };
 
-constexpr int kSelectThreads = 256;
+constexpr int kSelectThreads = 256, kSelectWaves = kSelectThreads / 64;
+constexpr int kPerThread = 16;  // logits of a thread
+constexpr int kMaxChunk = kSelectThreads * kPerThread;
 
 // A logit as the selection sees it.
 template <typename T>
@@ -49,127 +52,273 @@ __device__ __forceinline__ float logit(T v) {
   const float x = (float)v;
   return x != x ? -INFINITY : fminf(x, FLT_MAX);
 }
+// Keys that order as the selection does: larger values first, of equal ones the
+// lower index; no key of a logit is 0.
+__device__ __forceinline__ uint64_t rank_key(float x, uint32_t t) {
+  const uint32_t u = __float_as_uint(x + 0.f);  // (-0 counts as 0)
+  return (uint64_t)((u & 0x80000000u) ? ~u : u | 0x80000000u) << 32 | (uint32_t)~t;
+}
+__device__ __forceinline__ float key_logit(uint64_t k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ uint32_t key_token(uint64_t k) { return ~(uint32_t)k; }
 
-struct Best {
-  float x;
-  int t;
-};
-__device__ __forceinline__ bool better(float ax, int at, float bx, int bt) { return ax > bx || (ax == bx && at < bt); }
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
 
-// Block (row): its maximum, the sum of its exponentials, its `count` best.
+// Whether a live beam's logits count: it exists and is not finished.
+__device__ __forceinline__ bool live(const SelectArgs& a, int r) {
+  return a.scores[r] > -INFINITY && !(a.finished && a.finished[r] != 0);
+}
+
+// Block (split, row): the split's maximum, the sum of its exponentials and its
+// `count` best, of one pass over its logits, which stay in registers.
+//
+// The best: every thread's largest key; of each wave's 64 the count-th, by
+// counting; the largest of those is passed by at least `count` keys of the split
+// and by those of at most count threads a wave, which alone list what they have
+// above it; the few in the list find their ranks by counting.  No order of
+// threads or atomics shows in the result.
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs a) {
-  __shared__ float sx[kSelectThreads / 64];
-  __shared__ int stt[kSelectThreads / 64];
-  __shared__ double ss[kSelectThreads / 64];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int W = 16 / sizeof(T);  // logits of a load
+  struct alignas(16) Load {
+    T v[W];
+  };
+  extern __shared__ uint64_t list[];
+  __shared__ uint64_t s_kth[kSelectWaves];
+  __shared__ float s_max[kSelectWaves];
+  __shared__ double s_sum[kSelectWaves];
+  __shared__ uint32_t s_n;
+  const int r = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (!live(a, r)) return;  // its logits do not matter
   const T* x = static_cast<const T*>(a.logits) + r * a.row;
-  float px = INFINITY;
-  int pt = -1;
-  float m = -INFINITY;
-  for (int k = 0; k < a.count && k < a.vocab; ++k) {
-    float bx = -INFINITY;
-    int bt = INT_MAX;
-    for (int t = tid; t < a.vocab; t += kSelectThreads) {
-      const float v = logit(x[t]);
-      if ((v < px || (v == px && t > pt)) && better(v, t, bx, bt)) {
-        bx = v;
-        bt = t;
-      }
-    }
+  const int from = split * a.chunk, to = min(from + a.chunk, a.vocab);
+  // loads lie on 16 bytes, up to W - 1 logits before the split's first
+  const int skew = (int)(reinterpret_cast<uintptr_t>(x + from) % 16 / sizeof(T));
+  float v[kPerThread + W];
+  constexpr int LOADS = kPerThread / W + 1;  // (the last for what the skew pushes out)
+  const int at = from - skew + tid * W;
 #pragma unroll
-    for (int off = 32; off; off >>= 1) {
-      const float ox = __shfl_xor(bx, off, kWave);
-      const int ot = __shfl_xor(bt, off, kWave);
-      if (better(ox, ot, bx, bt)) {
-        bx = ox;
-        bt = ot;
-      }
-    }
-    __syncthreads();
-    if (lane == 0) {
-      sx[wave] = bx;
-      stt[wave] = bt;
-    }
-    __syncthreads();
-    for (int w = 0; w < kSelectThreads / 64; ++w)
-      if (w == 0 || better(sx[w], stt[w], bx, bt)) {
-        bx = sx[w];
-        bt = stt[w];
-      }
-    if (k == 0) m = bx;
-    px = bx;
-    pt = bt;
-    if (tid == 0) {
-      a.cand_x[(size_t)r * a.count + k] = bx;
-      a.cand_t[(size_t)r * a.count + k] = bt;
+  for (int i = 0; i < LOADS; ++i) {
+    const int t0 = at + i * kSelectThreads * W;
+    if (t0 >= from && t0 + W <= to) {
+      const Load l = *reinterpret_cast<const Load*>(x + t0);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[i * W + e] = logit(l.v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[i * W + e] = t0 + e >= from && t0 + e < to ? logit(x[t0 + e]) : -INFINITY;
     }
   }
+  auto token = [&](int i, int e) { return at + i * kSelectThreads * W + e; };
+  auto mine = [&](int i, int e) { return token(i, e) >= from && token(i, e) < to; };
+  if (tid == 0) s_n = 0;
+  uint64_t best = 0;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      m = fmaxf(m, v[i * W + e]);
+      const uint64_t k = mine(i, e) ? rank_key(v[i * W + e], (uint32_t)token(i, e)) : 0;
+      best = k > best ? k : best;
+    }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
+  int above = 0;  // lanes with a larger key
+#pragma unroll 8
+  for (int l = 0; l < 64; ++l) above += lane_u64(best, l) > best ? 1 : 0;
+  const uint64_t kth = __ballot(above == a.count - 1 && best != 0);
+  if (lane == 0) {
+    s_max[wave] = m;
+    s_kth[wave] = kth ? lane_u64(best, __ffsll((unsigned long long)kth) - 1) : 0;
+  }
+  __syncthreads();
+  uint64_t least = s_kth[0];
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) {
+    least = s_kth[w] > least ? s_kth[w] : least;
+    m = fmaxf(m, s_max[w]);
+  }
+  // (2 to the power of: the argument's rounding is relative to it, and a term that
+  // far below the largest weighs as little)
+  const float base = m == -INFINITY ? 0.f : m;
   double sum = 0.0;
-  const float ms = m == -INFINITY ? 0.f : m;
-  for (int t = tid; t < a.vocab; t += kSelectThreads) sum += (double)expf(logit(x[t]) - ms);
+#pragma unroll
+  for (int i = 0; i < LOADS * W; ++i)
+    sum += (double)__builtin_amdgcn_exp2f((v[i] - base) * 1.4426950408889634f);
 #pragma unroll
   for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, kWave);
-  if (lane == 0) ss[wave] = sum;
+  if (lane == 0) s_sum[wave] = sum;
+  if (best >= least && best != 0) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const uint64_t k = mine(i, e) ? rank_key(v[i * W + e], (uint32_t)token(i, e)) : 0;
+        if (k != 0 && k >= least) list[atomicAdd(&s_n, 1u)] = k;
+      }
+  }
   __syncthreads();
+  const int n = (int)s_n;
+  const size_t out = (size_t)r * a.splits + split;
+  for (int j = tid; j < n; j += kSelectThreads) {
+    const uint64_t k = list[j];
+    int rank = 0;
+    for (int o = 0; o < n; ++o) rank += list[o] > k ? 1 : 0;
+    if (rank < a.count) a.cand[out * a.count + rank] = k;
+  }
+  for (int j = n + tid; j < a.count; j += kSelectThreads) a.cand[out * a.count + j] = 0;
   if (tid == 0) {
-    for (int w = 1; w < kSelectThreads / 64; ++w) sum += ss[w];
-    a.sums[r] = sum;
-    a.tops[r] = m;
+#pragma unroll
+    for (int w = 1; w < kSelectWaves; ++w) sum += s_sum[w];
+    a.sums[out] = sum;
+    a.tops[out] = m;
   }
 }
 
-// Block (group): the best of its beams' candidates.
+// A candidate of a group: its score as a key that orders, its beam and token as
+// one number.
+struct Scored {
+  uint64_t s;
+  uint32_t at;
+  __device__ __forceinline__ bool over(const Scored& o) const { return s > o.s || (s == o.s && at < o.at); }
+};
+__device__ __forceinline__ uint64_t score_key(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+  return (u >> 63) ? ~u : u | (1ull << 63);
+}
+__device__ __forceinline__ double key_score(uint64_t k) {
+  return __longlong_as_double((long long)((k >> 63) ? k & ~(1ull << 63) : ~k));
+}
+
+constexpr int kGroupList = 1024;
+
+// Block (group): the best of its beams' candidates, found as a split's are; a
+// list that overflows (ties of thousands of beams' worth of candidates in few
+// threads) is worked off one by one.
 __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs a) {
-  __shared__ double sv[kMaxBeams * kMaxCount];
-  __shared__ int stt[kMaxBeams * kMaxCount];
-  const int g = blockIdx.x, tid = threadIdx.x, n = a.beams * min(a.count, a.vocab);
-  const int per = min(a.count, a.vocab);
-  for (int c = tid; c < n; c += kSelectThreads) {
-    const int b = c / per, k = c - b * per, r = g * a.beams + b;
-    const float cum = a.scores[r];
-    const bool done = a.finished && a.finished[r] != 0;
-    double s = -INFINITY;
-    int t = k;
-    if (!(cum > -INFINITY)) {
-      // no such beam: the lowest tokens, at -inf
-    } else if (done) {  // the stop token, then the lowest others at -inf
-      t = k == 0 ? a.stop : (k - 1 < a.stop ? k - 1 : k);
-      s = k == 0 ? (double)cum : -INFINITY;
-    } else {
-      const float x = a.cand_x[(size_t)r * a.count + k];
-      t = a.cand_t[(size_t)r * a.count + k];
-      if (x > -INFINITY) s = (double)cum + ((double)x - ((double)a.tops[r] + log(a.sums[r])));
-    }
-    sv[c] = s;
-    stt[c] = t;
+  __shared__ double s_off[kMaxBeams];  // a beam's score less its logits' log sum
+  __shared__ Scored list[kGroupList];
+  __shared__ Scored s_w[kSelectWaves];
+  __shared__ uint32_t s_n;
+  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) s_n = 0;
+  for (int b = tid >> 2; b < a.beams; b += kSelectThreads / 4) {  // four lanes a beam
+    const int r = g * a.beams + b;
+    if (!live(a, r)) continue;
+    const double* sums = a.sums + (size_t)r * a.splits;
+    const float* tops = a.tops + (size_t)r * a.splits;
+    float m = -INFINITY;
+    for (int s = tid & 3; s < a.splits; s += 4) m = fmaxf(m, tops[s]);
+    m = fmaxf(m, __shfl_xor(m, 1, kWave));
+    m = fmaxf(m, __shfl_xor(m, 2, kWave));
+    double sum = 0.0;
+    for (int s = tid & 3; s < a.splits; s += 4)
+      if (tops[s] > -INFINITY) sum += sums[s] * exp((double)tops[s] - (double)m);
+    sum += __shfl_xor(sum, 1, kWave);
+    sum += __shfl_xor(sum, 2, kWave);
+    if ((tid & 3) == 0) s_off[b] = m > -INFINITY ? (double)a.scores[r] - ((double)m + log(sum)) : -INFINITY;
   }
   __syncthreads();
-  for (int c = tid; c < n; c += kSelectThreads) {
-    const int b = c / per, t = stt[c];
-    const double s = sv[c];
-    int rank = 0;
-    for (int o = 0; o < n; ++o) {
-      const double os = sv[o];
-      const int ob = o / per;
-      rank += os > s || (os == s && (ob < b || (ob == b && stt[o] < t)));
+  const int per = a.splits * a.count, n = a.beams * per;
+  const Scored none = {0, 0xffffffffu};
+  auto candidate = [&](int c) -> Scored {
+    const int b = c / per, k = c - b * per, r = g * a.beams + b;
+    const uint32_t first = (uint32_t)b * (uint32_t)a.vocab;
+    const float cum = a.scores[r];
+    if (!live(a, r)) {  // the lowest tokens at -inf; of a finished beam the stop token before them
+      if (k >= a.count || k >= a.vocab) return none;
+      const bool stays = cum > -INFINITY;
+      const int t = !stays ? k : k == 0 ? a.stop : k - 1 < a.stop ? k - 1 : k;
+      return {score_key(stays && k == 0 ? (double)cum : -INFINITY), first + (uint32_t)t};
     }
-    if (rank >= a.count) continue;
+    const uint64_t key = a.cand[(size_t)r * per + k];
+    if (key == 0) return none;
+    const float x = key_logit(key);
+    return {score_key(x > -INFINITY ? (double)x + s_off[b] : -INFINITY), first + key_token(key)};
+  };
+  auto write = [&](const Scored& c, int rank) {
     const size_t at = (size_t)g * a.count + rank;
-    a.scores_out[at] = (float)s;
+    const int b = (int)(c.at / (uint32_t)a.vocab), t = (int)(c.at - (uint32_t)b * (uint32_t)a.vocab);
+    a.scores_out[at] = (float)key_score(c.s);
     a.parent_out[at] = b;
     a.token_out[at] = t;
-    if (a.finished_out)
-      a.finished_out[at] = t == a.stop || (a.finished && a.finished[g * a.beams + b] != 0) ? 1 : 0;
+    if (a.finished_out) a.finished_out[at] = t == a.stop || (a.finished && a.finished[g * a.beams + b] != 0) ? 1 : 0;
+  };
+  Scored best = none;
+  for (int c = tid; c < n; c += kSelectThreads) {
+    const Scored x = candidate(c);
+    if (x.over(best)) best = x;
+  }
+  int above = 0;
+#pragma unroll 8
+  for (int l = 0; l < 64; ++l) {
+    const Scored o = {lane_u64(best.s, l), (uint32_t)__builtin_amdgcn_readlane((int)best.at, l)};
+    above += o.over(best) ? 1 : 0;
+  }
+  const uint64_t kth = __ballot(above == a.count - 1 && best.s != 0);
+  if (lane == 0) {
+    const int l = __ffsll((unsigned long long)kth) - 1;
+    s_w[wave] = kth ? Scored{lane_u64(best.s, l), (uint32_t)__builtin_amdgcn_readlane((int)best.at, l)} : none;
+  }
+  __syncthreads();
+  Scored least = s_w[0];
+#pragma unroll
+  for (int w = 1; w < kSelectWaves; ++w)
+    if (s_w[w].over(least)) least = s_w[w];
+  if (best.s != 0 && !least.over(best))
+    for (int c = tid; c < n; c += kSelectThreads) {
+      const Scored x = candidate(c);
+      if (x.s == 0 || least.over(x)) continue;
+      const uint32_t i = atomicAdd(&s_n, 1u);
+      if (i < kGroupList) list[i] = x;
+    }
+  __syncthreads();
+  const int m = (int)s_n;
+  if (m <= kGroupList) {
+    for (int j = tid; j < m; j += kSelectThreads) {
+      const Scored x = list[j];
+      int rank = 0;
+      for (int o = 0; o < m; ++o) rank += list[o].over(x) ? 1 : 0;
+      if (rank < a.count) write(x, rank);
+    }
+    return;
+  }
+  Scored last = {~0ull, 0};
+  for (int k = 0; k < a.count; ++k) {
+    best = none;
+    for (int c = tid; c < n; c += kSelectThreads) {
+      const Scored x = candidate(c);
+      if (last.over(x) && x.over(best)) best = x;
+    }
+#pragma unroll
+    for (int off = 32; off; off >>= 1) {
+      const Scored o = {__shfl_xor((unsigned long long)best.s, off, kWave), (uint32_t)__shfl_xor((int)best.at, off, kWave)};
+      if (o.over(best)) best = o;
+    }
+    __syncthreads();
+    if (lane == 0) s_w[wave] = best;
+    __syncthreads();
+    last = s_w[0];
+    for (int w = 1; w < kSelectWaves; ++w)
+      if (s_w[w].over(last)) last = s_w[w];
+    if (tid == 0) write(last, k);
   }
 }
 
 bool select_in_range(const mit2cfm_beam_select& a) {
   return a.dtype >= MIT2CFM_DTYPE_F32 && a.dtype <= MIT2CFM_DTYPE_BF16 && a.beams >= 1 && a.beams <= (uint32_t)kMaxBeams &&
          a.vocab >= 1 && a.vocab <= (1u << 24) && a.count >= 1 && a.count <= (uint32_t)kMaxCount &&
-         a.count <= (uint64_t)a.beams * a.vocab && (uint64_t)a.groups * a.beams <= (1u << 20);
+         a.count <= (uint64_t)a.beams * a.vocab && (uint64_t)a.groups * a.beams <= 65535;
 }
 size_t align16(size_t b) { return (b + 15) & ~size_t(15); }
+// A row's logits in even splits of at most kMaxChunk.
+int select_splits(uint32_t vocab) { return (int)((vocab + kMaxChunk - 1) / kMaxChunk); }
 
 // ------------------------------------------------------------------ reorder
 struct ReorderArgs {
@@ -257,8 +406,8 @@ __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(ReorderArgs a)
 
 uint64_t beam_select_workspace(const mit2cfm_beam_select& a) {
   if (!select_in_range(a)) return 0;
-  const size_t rows = (size_t)a.groups * a.beams;
-  return align16(rows * 8) + align16(rows * 4) + 2 * align16(rows * a.count * 4) + 16;
+  const size_t parts = (size_t)a.groups * a.beams * select_splits(a.vocab);
+  return align16(parts * 8) + align16(parts * a.count * 8) + align16(parts * 4) + 16;
 }
 
 void beam_select(const mit2cfm_beam_select& p, hipStream_t s) {
@@ -271,29 +420,32 @@ void beam_select(const mit2cfm_beam_select& p, hipStream_t s) {
   need(aligned(p.logits, (size_t)kv_elem_bytes(p.dtype)), "logits must be aligned to its type");
   need(p.workspace && p.workspace_bytes >= beam_select_workspace(p), "workspace is NULL or too small");
   need(aligned(p.workspace, 16), "workspace must be 16-byte aligned");
-  const size_t rows = (size_t)p.groups * p.beams;
   SelectArgs a;
   a.logits = p.logits;
   a.row = (int64_t)p.logits_row;
-  a.groups = (int)p.groups; a.beams = (int)p.beams; a.vocab = (int)p.vocab; a.count = (int)p.count;
+  a.beams = (int)p.beams; a.vocab = (int)p.vocab; a.count = (int)p.count;
   a.stop = p.stop_token;
+  a.splits = select_splits(p.vocab);
+  a.chunk = (int)((p.vocab + a.splits - 1) / a.splits + 7) / 8 * 8;
   a.scores = p.scores; a.finished = p.finished;
   a.scores_out = p.scores_out; a.parent_out = p.parent_out; a.token_out = p.token_out; a.finished_out = p.finished_out;
+  const uint32_t rows = p.groups * p.beams;
+  const size_t parts = (size_t)rows * a.splits;
   char* w = static_cast<char*>(p.workspace);
   a.sums = reinterpret_cast<double*>(w);
-  w += align16(rows * 8);
+  w += align16(parts * 8);
+  a.cand = reinterpret_cast<uint64_t*>(w);
+  w += align16(parts * a.count * 8);
   a.tops = reinterpret_cast<float*>(w);
-  w += align16(rows * 4);
-  a.cand_x = reinterpret_cast<float*>(w);
-  w += align16(rows * a.count * 4);
-  a.cand_t = reinterpret_cast<int32_t*>(w);
-  const dim3 grid((uint32_t)rows), block(kSelectThreads);
+  const dim3 grid(a.splits, rows), block(kSelectThreads);
+  // the list holds all logits of count threads a wave
+  const size_t lds = std::min<size_t>((size_t)kSelectWaves * a.count * (kPerThread + 8), kMaxChunk) * 8;
   if (p.dtype == MIT2CFM_DTYPE_F32)
-    hipLaunchKernelGGL((select_rows_kernel<float>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((select_rows_kernel<float>), grid, block, lds, s, a);
   else if (p.dtype == MIT2CFM_DTYPE_F16)
-    hipLaunchKernelGGL((select_rows_kernel<half_t>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((select_rows_kernel<half_t>), grid, block, lds, s, a);
   else
-    hipLaunchKernelGGL((select_rows_kernel<bf16_t>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((select_rows_kernel<bf16_t>), grid, block, lds, s, a);
   launched(hipGetLastError());
   hipLaunchKernelGGL(select_group_kernel, dim3(p.groups), block, 0, s, a);
   launched(hipGetLastError());
