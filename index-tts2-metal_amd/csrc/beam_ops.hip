@@ -16,6 +16,7 @@ namespace mit2hip {
 namespace {
 
 typedef __bf16 bf16_t;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 void need(bool ok, const char* what) {
   if (!ok) throw std::invalid_argument(what);
@@ -64,9 +65,21 @@ __device__ __forceinline__ float key_logit(uint64_t k) {
 }
 __device__ __forceinline__ uint32_t key_token(uint64_t k) { return ~(uint32_t)k; }
 
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
-         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+// The order of floats as unsigned integers; of no float 0.
+__device__ __forceinline__ uint32_t float_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+// The largest number that at least n of a wave's keys reach (0: fewer than n are
+// over 0), built from its top bit by votes.
+__device__ __forceinline__ uint32_t reached_by(uint32_t key, int n) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = t | 1u << bit;
+    t = __popcll(__ballot(key >= c)) >= n ? c : t;
+  }
+  return t;
 }
 
 // Whether a live beam's logits count: it exists and is not finished.
@@ -77,11 +90,11 @@ __device__ __forceinline__ bool live(const SelectArgs& a, int r) {
 // Block (split, row): the split's maximum, the sum of its exponentials and its
 // `count` best, of one pass over its logits, which stay in registers.
 //
-// The best: every thread's largest key; of each wave's 64 the count-th, by
-// counting; the largest of those is passed by at least `count` keys of the split
-// and by those of at most count threads a wave, which alone list what they have
-// above it; the few in the list find their ranks by counting.  No order of
-// threads or atomics shows in the result.
+// The best: every thread's largest logit, ties to the lower token; of each wave's
+// 64 the count-th, by votes; the largest of those is reached by at least `count`
+// logits of the split and by those of at most count threads a wave, which
+// alone list what they have from it on; the few in the list find their ranks by
+// counting.  No order of threads or atomics shows in the result.
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs a) {
   constexpr int W = 16 / sizeof(T);  // logits of a load
@@ -99,8 +112,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
   const int from = split * a.chunk, to = min(from + a.chunk, a.vocab);
   // loads lie on 16 bytes, up to W - 1 logits before the split's first
   const int skew = (int)(reinterpret_cast<uintptr_t>(x + from) % 16 / sizeof(T));
-  float v[kPerThread + W];
   constexpr int LOADS = kPerThread / W + 1;  // (the last for what the skew pushes out)
+  float v[LOADS * W];  // NaN: outside the split
   const int at = from - skew + tid * W;
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
@@ -111,31 +124,40 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
       for (int e = 0; e < W; ++e) v[i * W + e] = logit(l.v[e]);
     } else {
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[i * W + e] = t0 + e >= from && t0 + e < to ? logit(x[t0 + e]) : -INFINITY;
+      for (int e = 0; e < W; ++e) v[i * W + e] = t0 + e >= from && t0 + e < to ? logit(x[t0 + e]) : NAN;
     }
   }
-  auto token = [&](int i, int e) { return at + i * kSelectThreads * W + e; };
-  auto mine = [&](int i, int e) { return token(i, e) >= from && token(i, e) < to; };
   if (tid == 0) s_n = 0;
-  uint64_t best = 0;
-  float m = -INFINITY;
+  // (a comparison with NaN is false, a maximum takes the other number)
+  float top = -INFINITY;
+  int best_t = -1;
 #pragma unroll
   for (int i = 0; i < LOADS; ++i)
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      m = fmaxf(m, v[i * W + e]);
-      const uint64_t k = mine(i, e) ? rank_key(v[i * W + e], (uint32_t)token(i, e)) : 0;
-      best = k > best ? k : best;
+      const bool up = v[i * W + e] > top;
+      top = up ? v[i * W + e] : top;
+      best_t = up ? at + i * kSelectThreads * W + e : best_t;
     }
+  if (best_t < 0) {  // nothing over -inf: the first that there is
+#pragma unroll
+    for (int i = LOADS - 1; i >= 0; --i)
+#pragma unroll
+      for (int e = W - 1; e >= 0; --e)
+        best_t = v[i * W + e] == v[i * W + e] ? at + i * kSelectThreads * W + e : best_t;
+  }
+  float m = top;
 #pragma unroll
   for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
-  int above = 0;  // lanes with a larger key
-#pragma unroll 8
-  for (int l = 0; l < 64; ++l) above += lane_u64(best, l) > best ? 1 : 0;
-  const uint64_t kth = __ballot(above == a.count - 1 && best != 0);
+  const uint32_t key = best_t < 0 ? 0u : float_key(top);
+  const uint32_t t32 = reached_by(key, a.count);
+  uint64_t kth = (uint64_t)t32 << 32;
+  const int ties = __popcll(__ballot(key == t32)), over = __popcll(__ballot(key > t32));
+  if (t32 != 0 && over + ties > a.count)  // of equal ones the lowest tokens
+    kth |= reached_by(key == t32 ? ~(uint32_t)best_t : 0u, a.count - over);
   if (lane == 0) {
     s_max[wave] = m;
-    s_kth[wave] = kth ? lane_u64(best, __ffsll((unsigned long long)kth) - 1) : 0;
+    s_kth[wave] = kth;
   }
   __syncthreads();
   uint64_t least = s_kth[0];
@@ -145,22 +167,29 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
     m = fmaxf(m, s_max[w]);
   }
   // (2 to the power of: the argument's rounding is relative to it, and a term that
-  // far below the largest weighs as little)
+  // far below the largest weighs as little; a thread's few terms are summed in
+  // fp32, in pairs)
   const float base = m == -INFINITY ? 0.f : m;
-  double sum = 0.0;
+  float part[LOADS * W];
 #pragma unroll
   for (int i = 0; i < LOADS * W; ++i)
-    sum += (double)__builtin_amdgcn_exp2f((v[i] - base) * 1.4426950408889634f);
+    part[i] = __builtin_amdgcn_exp2f(fmaxf((v[i] - base) * 1.4426950408889634f, -INFINITY));
+#pragma unroll
+  for (int w = LOADS * W; w > 1; w = (w + 1) / 2)
+#pragma unroll
+    for (int i = 0; i < w / 2; ++i) part[i] += part[w - 1 - i];
+  double sum = (double)part[0];
 #pragma unroll
   for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, kWave);
   if (lane == 0) s_sum[wave] = sum;
-  if (best >= least && best != 0) {
+  const uint64_t best = best_t < 0 ? 0 : rank_key(top, (uint32_t)best_t);
+  if (best != 0 && best >= least) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        const uint64_t k = mine(i, e) ? rank_key(v[i * W + e], (uint32_t)token(i, e)) : 0;
-        if (k != 0 && k >= least) list[atomicAdd(&s_n, 1u)] = k;
+        const uint64_t k = rank_key(v[i * W + e], (uint32_t)(at + i * kSelectThreads * W + e));
+        if (v[i * W + e] == v[i * W + e] && k >= least) list[atomicAdd(&s_n, 1u)] = k;
       }
   }
   __syncthreads();
@@ -197,50 +226,80 @@ __device__ __forceinline__ double key_score(uint64_t k) {
 }
 
 constexpr int kGroupList = 1024;
+constexpr int kHeldCandidates = 8;  // of a thread, kept in registers
 
-// Block (group): the best of its beams' candidates, found as a split's are; a
-// list that overflows (ties of thousands of beams' worth of candidates in few
-// threads) is worked off one by one.
+// Block (group): the best of its beams' candidates, found as a split's are (by
+// the scores rounded to fp32, which keeps their order, until the list is made);
+// a list that overflows, as with ties of very many candidates, is worked off one
+// by one.
 __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs a) {
-  __shared__ double s_off[kMaxBeams];  // a beam's score less its logits' log sum
+  __shared__ double s_off[kMaxBeams];   // a beam's score less its logits' log sum
+  __shared__ float s_cum[kMaxBeams];    // its score
+  __shared__ uint8_t s_kind[kMaxBeams]; // bit 0: finished, bit 1: does not exist
   __shared__ Scored list[kGroupList];
   __shared__ Scored s_w[kSelectWaves];
+  __shared__ uint32_t s_kth[kSelectWaves];
   __shared__ uint32_t s_n;
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) s_n = 0;
   for (int b = tid >> 2; b < a.beams; b += kSelectThreads / 4) {  // four lanes a beam
     const int r = g * a.beams + b;
-    if (!live(a, r)) continue;
-    const double* sums = a.sums + (size_t)r * a.splits;
-    const float* tops = a.tops + (size_t)r * a.splits;
-    float m = -INFINITY;
-    for (int s = tid & 3; s < a.splits; s += 4) m = fmaxf(m, tops[s]);
-    m = fmaxf(m, __shfl_xor(m, 1, kWave));
-    m = fmaxf(m, __shfl_xor(m, 2, kWave));
-    double sum = 0.0;
-    for (int s = tid & 3; s < a.splits; s += 4)
-      if (tops[s] > -INFINITY) sum += sums[s] * exp((double)tops[s] - (double)m);
-    sum += __shfl_xor(sum, 1, kWave);
-    sum += __shfl_xor(sum, 2, kWave);
-    if ((tid & 3) == 0) s_off[b] = m > -INFINITY ? (double)a.scores[r] - ((double)m + log(sum)) : -INFINITY;
+    const float cum = a.scores[r];
+    const int kind = (cum > -INFINITY ? 0 : 2) | (a.finished && a.finished[r] != 0 ? 1 : 0);
+    double off = -INFINITY;
+    if (kind == 0) {
+      const double* sums = a.sums + (size_t)r * a.splits;
+      const float* tops = a.tops + (size_t)r * a.splits;
+      float m = -INFINITY;
+      for (int s = tid & 3; s < a.splits; s += 4) m = fmaxf(m, tops[s]);
+      m = fmaxf(m, __shfl_xor(m, 1, kWave));
+      m = fmaxf(m, __shfl_xor(m, 2, kWave));
+      double sum = 0.0;
+      for (int s = tid & 3; s < a.splits; s += 4)
+        if (tops[s] > -INFINITY) sum += sums[s] * exp((double)tops[s] - (double)m);
+      sum += __shfl_xor(sum, 1, kWave);
+      sum += __shfl_xor(sum, 2, kWave);
+      if (m > -INFINITY) off = (double)cum - ((double)m + log(sum));
+    }
+    if ((tid & 3) == 0) {
+      s_off[b] = off;
+      s_cum[b] = cum;
+      s_kind[b] = (uint8_t)kind;
+    }
   }
-  __syncthreads();
   const int per = a.splits * a.count, n = a.beams * per;
   const Scored none = {0, 0xffffffffu};
-  auto candidate = [&](int c) -> Scored {
-    const int b = c / per, k = c - b * per, r = g * a.beams + b;
+  const uint64_t* cand = a.cand + (size_t)g * n;
+  // the stored keys of this thread's first candidates, asked for before the sums are known
+  uint64_t key[kHeldCandidates];
+#pragma unroll
+  for (int i = 0; i < kHeldCandidates; ++i) {
+    const int c = tid + i * kSelectThreads;
+    key[i] = c < n ? cand[c] : 0;  // (what a beam without a pass left there is not used)
+  }
+  __syncthreads();
+  auto candidate = [&](int c, uint64_t stored) -> Scored {
+    const int b = c / per, k = c - b * per, kind = s_kind[b];
     const uint32_t first = (uint32_t)b * (uint32_t)a.vocab;
-    const float cum = a.scores[r];
-    if (!live(a, r)) {  // the lowest tokens at -inf; of a finished beam the stop token before them
+    if (kind != 0) {  // the lowest tokens at -inf; of a finished beam the stop token before them
       if (k >= a.count || k >= a.vocab) return none;
-      const bool stays = cum > -INFINITY;
-      const int t = !stays ? k : k == 0 ? a.stop : k - 1 < a.stop ? k - 1 : k;
-      return {score_key(stays && k == 0 ? (double)cum : -INFINITY), first + (uint32_t)t};
+      const int t = kind & 2 ? k : k == 0 ? a.stop : k - 1 < a.stop ? k - 1 : k;
+      return {score_key(kind == 1 && k == 0 ? (double)s_cum[b] : -INFINITY), first + (uint32_t)t};
     }
-    const uint64_t key = a.cand[(size_t)r * per + k];
-    if (key == 0) return none;
-    const float x = key_logit(key);
-    return {score_key(x > -INFINITY ? (double)x + s_off[b] : -INFINITY), first + key_token(key)};
+    if (stored == 0) return none;
+    const float x = key_logit(stored);
+    return {score_key(x > -INFINITY ? (double)x + s_off[b] : -INFINITY), first + key_token(stored)};
+  };
+  Scored held[kHeldCandidates];
+#pragma unroll
+  for (int i = 0; i < kHeldCandidates; ++i) {
+    const int c = tid + i * kSelectThreads;
+    held[i] = c < n ? candidate(c, key[i]) : none;
+  }
+  auto each = [&](auto&& f) {  // every candidate of this thread
+#pragma unroll
+    for (int i = 0; i < kHeldCandidates; ++i) f(held[i]);
+    for (int c = tid + kHeldCandidates * kSelectThreads; c < n; c += kSelectThreads) f(candidate(c, cand[c]));
   };
   auto write = [&](const Scored& c, int rank) {
     const size_t at = (size_t)g * a.count + rank;
@@ -248,42 +307,30 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
     a.scores_out[at] = (float)key_score(c.s);
     a.parent_out[at] = b;
     a.token_out[at] = t;
-    if (a.finished_out) a.finished_out[at] = t == a.stop || (a.finished && a.finished[g * a.beams + b] != 0) ? 1 : 0;
+    if (a.finished_out) a.finished_out[at] = t == a.stop || (s_kind[b] & 1) ? 1 : 0;
   };
-  Scored best = none;
-  for (int c = tid; c < n; c += kSelectThreads) {
-    const Scored x = candidate(c);
-    if (x.over(best)) best = x;
-  }
-  int above = 0;
-#pragma unroll 8
-  for (int l = 0; l < 64; ++l) {
-    const Scored o = {lane_u64(best.s, l), (uint32_t)__builtin_amdgcn_readlane((int)best.at, l)};
-    above += o.over(best) ? 1 : 0;
-  }
-  const uint64_t kth = __ballot(above == a.count - 1 && best.s != 0);
-  if (lane == 0) {
-    const int l = __ffsll((unsigned long long)kth) - 1;
-    s_w[wave] = kth ? Scored{lane_u64(best.s, l), (uint32_t)__builtin_amdgcn_readlane((int)best.at, l)} : none;
-  }
+  auto rounded = [](const Scored& x) { return x.s == 0 ? 0u : float_key((float)key_score(x.s)); };
+  uint32_t best = 0;
+  each([&](const Scored& x) { best = max(best, rounded(x)); });
+  const uint32_t kth = reached_by(best, a.count);
+  if (lane == 0) s_kth[wave] = kth;
   __syncthreads();
-  Scored least = s_w[0];
+  uint32_t least = 1;
 #pragma unroll
-  for (int w = 1; w < kSelectWaves; ++w)
-    if (s_w[w].over(least)) least = s_w[w];
-  if (best.s != 0 && !least.over(best))
-    for (int c = tid; c < n; c += kSelectThreads) {
-      const Scored x = candidate(c);
-      if (x.s == 0 || least.over(x)) continue;
+  for (int w = 0; w < kSelectWaves; ++w) least = max(least, s_kth[w]);
+  if (best >= least)
+    each([&](const Scored& x) {
+      if (rounded(x) < least) return;
       const uint32_t i = atomicAdd(&s_n, 1u);
       if (i < kGroupList) list[i] = x;
-    }
+    });
   __syncthreads();
   const int m = (int)s_n;
   if (m <= kGroupList) {
     for (int j = tid; j < m; j += kSelectThreads) {
       const Scored x = list[j];
       int rank = 0;
+#pragma unroll 4
       for (int o = 0; o < m; ++o) rank += list[o].over(x) ? 1 : 0;
       if (rank < a.count) write(x, rank);
     }
@@ -291,18 +338,17 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
   }
   Scored last = {~0ull, 0};
   for (int k = 0; k < a.count; ++k) {
-    best = none;
-    for (int c = tid; c < n; c += kSelectThreads) {
-      const Scored x = candidate(c);
-      if (last.over(x) && x.over(best)) best = x;
-    }
+    Scored next = none;
+    each([&](const Scored& x) {
+      if (last.over(x) && x.over(next)) next = x;
+    });
 #pragma unroll
     for (int off = 32; off; off >>= 1) {
-      const Scored o = {__shfl_xor((unsigned long long)best.s, off, kWave), (uint32_t)__shfl_xor((int)best.at, off, kWave)};
-      if (o.over(best)) best = o;
+      const Scored o = {__shfl_xor((unsigned long long)next.s, off, kWave), (uint32_t)__shfl_xor((int)next.at, off, kWave)};
+      if (o.over(next)) next = o;
     }
     __syncthreads();
-    if (lane == 0) s_w[wave] = best;
+    if (lane == 0) s_w[wave] = next;
     __syncthreads();
     last = s_w[0];
     for (int w = 1; w < kSelectWaves; ++w)
@@ -342,11 +388,12 @@ struct ReorderArgs {
 constexpr int kReorderThreads = 256;
 
 // Block (new beam, part): part 0 writes the beam's table row and states, part 1
-// + 2 l (+ 1) copies the part page's k (v) of layer l, for a beam that is not
-// its parent's first child.  Each block finds whose pages are whose by itself,
-// from the group's parents as bits: a beam is a further child when an earlier
-// one has its parent, its rank among those is its index less the distinct
-// parents before it, and there are as many beams without children.
+// + l copies the part page's rows of layer l, for a beam that is not its
+// parent's first child.  Each block finds whose pages are whose by itself, from
+// the group's parents as bits: a beam is a further child when an earlier one
+// has its parent, its rank among those is its index less the distinct parents
+// before it, and there are as many beams without children.
+constexpr int kCopyBatch = 4;  // 16-byte loads of a thread in flight, of k and of v each
 __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(ReorderArgs a) {
   const int r = blockIdx.x, g = r / a.beams, b = r - g * a.beams;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -390,15 +437,26 @@ __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(ReorderArgs a)
   if (!further || part == 0) return;
   const int src = from[full], dst = priv[full];
   if ((unsigned)src >= (unsigned)a.pages || (unsigned)dst >= (unsigned)a.pages) return;
-  const int y = blockIdx.y - 1;
-  uint4* base = reinterpret_cast<uint4*>(y & 1 ? a.v : a.k) + (y >> 1) * a.layer16;
-  const int per = part * a.row16;  // a head's vectors
-  const int64_t head = (int64_t)a.row16 << a.page_shift;
-  const uint4* s = base + (int64_t)src * a.kv_heads * head;
-  uint4* d = base + (int64_t)dst * a.kv_heads * head;
-  for (int i = tid; i < per * a.kv_heads; i += kReorderThreads) {
-    const int h = i / per, e = i - h * per;
-    d[h * head + e] = s[h * head + e];
+  const int64_t layer = (int64_t)(blockIdx.y - 1) * a.layer16, head = (int64_t)a.row16 << a.page_shift;
+  const int per = part * a.row16, n = per * a.kv_heads;  // 16-byte vectors: a head's, all
+  u32x4 *k = reinterpret_cast<u32x4*>(a.k) + layer, *v = reinterpret_cast<u32x4*>(a.v) + layer;
+  const int64_t s = (int64_t)src * a.kv_heads * head, d = (int64_t)dst * a.kv_heads * head;
+  for (int i0 = tid; i0 < n; i0 += kReorderThreads * kCopyBatch) {
+    u32x4 x[kCopyBatch], y[kCopyBatch];
+    int64_t at[kCopyBatch];
+#pragma unroll
+    for (int u = 0; u < kCopyBatch; ++u) {
+      const int i = min(i0 + u * kReorderThreads, n - 1), h = i / per;
+      at[u] = h * head + (i - h * per);
+      x[u] = k[s + at[u]];
+      y[u] = v[s + at[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < kCopyBatch; ++u)
+      if (i0 + u * kReorderThreads < n) {
+        k[d + at[u]] = x[u];
+        v[d + at[u]] = y[u];
+      }
   }
 }
 
@@ -485,7 +543,7 @@ void beam_reorder(const mit2cfm_kv_cache& c, const mit2cfm_beam_reorder& p, hipS
   a.state_words = (int)p.state_words;
   a.token = p.token;
   a.place = p.place;
-  hipLaunchKernelGGL(reorder_kernel, dim3(p.groups * p.beams, 1 + 2 * p.layers), dim3(kReorderThreads), 0, s, a);
+  hipLaunchKernelGGL(reorder_kernel, dim3(p.groups * p.beams, 1 + p.layers), dim3(kReorderThreads), 0, s, a);
   launched(hipGetLastError());
 }
 
