@@ -483,6 +483,20 @@ mit2cfm_status mit2cfm_gpt_kv_sample(mit2cfm_ctx* ctx, const float* prefix, uint
                                      int32_t* first_stop_step, float* last_logits,
                                      float* last_processed_logits, double* timings_ms);
 
+/* Beam search over the mel codes: the `beams` (1 .. 8) hypotheses of the
+ * largest sum of log probabilities, from the start token, for up to `steps` (>= 1)
+ * tokens after prefix [prefix_tokens][1280].  One that takes the stop token
+ * stays as it is, and the search ends when all have.  Positions as for
+ * mit2cfm_gpt_kv_greedy.  Outputs (host): predicted_tokens [beams][steps], best
+ * first, n_predicted [beams] (the stop token included), scores [beams],
+ * timings_ms [2] (may be NULL).  Weights f16, all else fp32, by plain launches;
+ * the beams' caches are paged and share the prefix (the operators below).
+ * Host pointers, synchronous.  No reference counterpart (its decoder holds one
+ * sequence). */
+mit2cfm_status mit2cfm_gpt_kv_beam(mit2cfm_ctx* ctx, const float* prefix, uint32_t prefix_tokens, uint32_t steps,
+                                   int32_t hf_generate_positions, uint32_t beams, uint32_t* predicted_tokens,
+                                   uint32_t* n_predicted, float* scores, double* timings_ms);
+
 /* Replaces run_gpt_cached_decode_metal (runtime/impl/gpt.cpp:1427; CPU
  * definition run_gpt_cached_decode_cpu :1400): rows [prefix_tokens + 1][1280];
  * the first prefix_tokens rows fill the key/value caches, the last row is

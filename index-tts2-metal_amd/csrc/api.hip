@@ -920,6 +920,31 @@ mit2cfm_status mit2cfm_gpt_kv_sample(mit2cfm_ctx* ctx, const float* prefix, uint
   });
 }
 
+mit2cfm_status mit2cfm_gpt_kv_beam(mit2cfm_ctx* ctx, const float* prefix, uint32_t prefix_tokens, uint32_t steps,
+                                   int32_t hf_generate_positions, uint32_t beams, uint32_t* predicted_tokens,
+                                   uint32_t* n_predicted, float* scores, double* timings_ms) {
+  if (!ctx) return fail(nullptr, MIT2CFM_E_ARG, "ctx must not be NULL");
+  return guarded(ctx, [&] {
+    require(prefix_tokens == 0 || prefix != nullptr, "prefix must not be NULL");
+    require(prefix_tokens <= (1u << 16), "prefix_tokens must be <= 65536");
+    require(steps >= 1 && steps <= (uint32_t)mit2hip::GptDecoder::kPositions, "steps must be in [1, 1818]");
+    require(beams >= 1 && beams <= (uint32_t)mit2hip::GptDecoder::kMaxBeams, "beams must be in [1, 8]");
+    require(predicted_tokens && n_predicted && scores, "predicted_tokens, n_predicted and scores must not be NULL");
+    mit2hip::GptDecoder::Beams b;
+    ctx->eng->gpt().kv_beam(prefix, (int)prefix_tokens, (int)steps, hf_generate_positions != 0, (int)beams, b);
+    for (uint32_t i = 0; i < beams; ++i) {
+      n_predicted[i] = (uint32_t)b.predicted[i].size();
+      if (!b.predicted[i].empty())
+        std::memcpy(predicted_tokens + (size_t)i * steps, b.predicted[i].data(), b.predicted[i].size() * 4);
+      scores[i] = b.scores[i];
+    }
+    if (timings_ms) {
+      timings_ms[0] = b.prefill_ms;
+      timings_ms[1] = b.decode_ms;
+    }
+  });
+}
+
 mit2cfm_status mit2cfm_gpt_cached_decode(mit2cfm_ctx* ctx, const float* rows, uint32_t prefix_tokens,
                                          float* ln_f, float* final_norm, float* logits, uint32_t* argmax) {
   if (!ctx) return fail(nullptr, MIT2CFM_E_ARG, "ctx must not be NULL");

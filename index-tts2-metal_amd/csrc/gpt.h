@@ -82,6 +82,18 @@ class GptDecoder {
   void kv_sample(const float* prefix, int prefix_tokens, int steps, bool hf_generate_positions,
                  const Sampling& sampling, Greedy& out);
 
+  // Beam search of up to `steps` tokens (no reference counterpart: its decoder
+  // holds one sequence).  A hypothesis that takes the stop token stays in the
+  // search with its score, the sum of its tokens' log probabilities; the search
+  // ends when all have.  The prefix is kept once, in pages that the beams share.
+  static constexpr int kMaxBeams = 8;
+  struct Beams {
+    std::vector<std::vector<uint32_t>> predicted;  // best first; the stop token included
+    std::vector<float> scores;
+    double prefill_ms = 0, decode_ms = 0;
+  };
+  void kv_beam(const float* prefix, int prefix_tokens, int steps, bool hf_generate_positions, int beams, Beams& out);
+
   // run_gpt_cached_decode (gpt.cpp:1400): HOST rows [prefix_tokens + 1][1280];
   // the last row is decoded against the caches of the others.  Outputs (host,
   // any may be null): ln_f [1280], final_norm [1280], logits [8194].  Returns

@@ -57,9 +57,11 @@
 #include "device_common.h"
 #include "engine.h"
 #include "gpt_prefill.h"
+#include "beam_ops.h"
 #include "gpt_state.h"
 #include "gpt_token.h"
 #include "image_io.h"
+#include "kv_ops.h"
 
 namespace mit2hip {
 
@@ -1142,6 +1144,30 @@ __global__ __launch_bounds__(64) void attn_combine_kernel(const GptState* st, co
   out[(size_t)z * kW + h * kHD + d] = O / L;
 }
 
+// ---- beam search (kv_beam): what a step reads and moves on by itself
+struct BeamState {
+  int32_t step;                     // steps taken
+  int32_t start[kPlainRows + 1];    // one new row a beam
+  int32_t length[kPlainRows];       // cached rows of each beam with the step's
+  int32_t token[kPlainRows];        // the beams' last tokens
+  int32_t parent[kPlainRows];
+  int32_t prefix[2];                // the prefix as one sequence: its bounds
+};
+
+// x[b] = mel_embedding[token] + mel_pos_embedding[position], as embed_kernel.
+__global__ __launch_bounds__(320) void beam_embed_kernel(const BeamState* st, int hf, const float* mel_emb,
+                                                         const float* pos_emb, float* x) {
+  const int i = threadIdx.x, b = blockIdx.x, step = st->step;
+  const int tok = min(max(st->token[b], 0), kVocab - 1), pos = min(hf && step > 0 ? step + 1 : step, kPos - 1);
+  const float4 e = reinterpret_cast<const float4*>(mel_emb + (size_t)tok * kW)[i];
+  const float4 p = reinterpret_cast<const float4*>(pos_emb + (size_t)pos * kW)[i];
+  reinterpret_cast<float4*>(x + (size_t)b * kW)[i] = make_float4(e.x + p.x, e.y + p.y, e.z + p.z, e.w + p.w);
+}
+__global__ void beam_advance_kernel(BeamState* st) {
+  if (threadIdx.x < kPlainRows) st->length[threadIdx.x] += 1;
+  if (threadIdx.x == 0) st->step += 1;
+}
+
 // Launch shapes: rows per block = WAVES * (64 / LPR) * UR.
 template <int K, int LPR, int WAVES, int UR, int PRO, int EPI>
 void launch_gemv(const GemvArgs& a, hipStream_t s) {
@@ -1633,6 +1659,172 @@ struct GptDecoder::Impl {
     GPT_OK(hipGraphLaunch(graph[which], s));
   }
 
+  // ---- beam search: the beams' paged caches (one page table for all layers) and
+  // the step's buffers, all of it in two of what a selection reorders
+  static constexpr int kBeamPage = 64;
+  Arena bw;
+  int beam_cap[3] = {0, 0, 0};  // beams, cached rows, steps
+  int beam_entries = 0, beam_pages = 0, beams_held = 0, steps_held = 0;
+  size_t beam_layer = 0;        // floats of a layer's keys (values)
+  BeamState* bst = nullptr;
+  GptState* brow = nullptr;     // tells the row kernels how many rows there are
+  float *bk = nullptr, *bv = nullptr, *bx, *bq, *batt, *bfc, *blogits, *new_k, *new_v, *bscore[2];
+  int32_t *btable[2], *bdone[2];
+  uint32_t* bhist[2];
+  void *battend = nullptr, *bselect = nullptr;
+  size_t battend_bytes = 0, bselect_bytes = 0;
+
+  mit2cfm_kv_cache beam_cache(int l, int side) const {
+    mit2cfm_kv_cache c{};
+    c.k = bk + (size_t)l * beam_layer;
+    c.v = bv + (size_t)l * beam_layer;
+    c.table = btable[side];
+    c.pages = (uint32_t)beam_pages;
+    c.page_rows = kBeamPage;
+    c.kv_heads = kHeads;
+    c.head_dim = kHD;
+    c.table_stride = (uint32_t)beam_entries;
+    c.dtype = MIT2CFM_DTYPE_F32;
+    return c;
+  }
+  mit2cfm_kv_rows beam_rows(int n, int max_length) const {
+    mit2cfm_kv_rows r{};
+    r.start = bst->start;
+    r.length = bst->length;
+    r.seqs = r.rows = (uint32_t)n;
+    r.max_length = (uint32_t)max_length;
+    return r;
+  }
+  mit2cfm_beam_select beam_pick(int n, int side) const {
+    mit2cfm_beam_select a{};
+    a.logits = blogits;
+    a.logits_row = kVocab;
+    a.dtype = MIT2CFM_DTYPE_F32;
+    a.groups = 1;
+    a.beams = a.count = (uint32_t)n;
+    a.vocab = kVocab;
+    a.scores = bscore[side];
+    a.finished = bdone[side];
+    a.stop_token = kStop;
+    a.scores_out = bscore[1 - side];
+    a.finished_out = bdone[1 - side];
+    a.parent_out = bst->parent;
+    a.token_out = bst->token;
+    a.workspace = bselect;
+    a.workspace_bytes = bselect_bytes;
+    return a;
+  }
+  mit2cfm_beam_reorder beam_move(int n, int side, int steps) const {
+    mit2cfm_beam_reorder a{};
+    a.groups = 1;
+    a.beams = a.parent_stride = (uint32_t)n;
+    a.layers = (uint32_t)L;
+    a.layer_stride = beam_layer;
+    a.parent = bst->parent;
+    a.length = bst->length;
+    a.table_out = btable[1 - side];
+    a.state = bhist[side];
+    a.state_out = bhist[1 - side];
+    a.state_words = (uint32_t)steps;
+    a.token = reinterpret_cast<const uint32_t*>(bst->token);
+    a.place = &bst->step;
+    return a;
+  }
+
+  void ensure_beams(int n, int rows, int steps) {
+    beam_cap[0] = std::max(n, beam_cap[0]);
+    beam_cap[1] = std::max(rows, beam_cap[1]);
+    beam_cap[2] = std::max(steps, beam_cap[2]);
+    const int N = beam_cap[0], pages_before = beam_pages, entries = (beam_cap[1] + kBeamPage - 1) / kBeamPage;
+    // (what this call's plans need: the sizes' pointers do not matter)
+    BeamState none{};
+    BeamState* const held = bst;
+    bst = &none;
+    beam_entries = entries;
+    beam_pages = N * entries;
+    beam_layer = (size_t)beam_pages * kBeamPage * kW;
+    const size_t attend_bytes = kv_attention_workspace(beam_cache(0, 0), beam_rows(n, rows), kHeads);
+    const size_t select_bytes = beam_select_workspace(beam_pick(n, 0));
+    bst = held;
+    const bool fits = held && beam_pages == pages_before && N == beams_held && beam_cap[2] == steps_held &&
+                      attend_bytes <= battend_bytes && select_bytes <= bselect_bytes;
+    if (fits) return;
+    beams_held = N;
+    steps_held = beam_cap[2];
+    battend_bytes = std::max(attend_bytes, battend_bytes);
+    bselect_bytes = std::max(select_bytes, bselect_bytes);
+    const size_t f = sizeof(float);
+    const size_t sizes[] = {sizeof(BeamState), sizeof(GptState), (size_t)L * beam_layer * f, (size_t)L * beam_layer * f,
+                            (size_t)N * kW * f, (size_t)N * kW * f, (size_t)N * kW * f, (size_t)N * kMLP * f,
+                            (size_t)N * kVocab * f, (size_t)kPlainRows * kW * f, (size_t)kPlainRows * kW * f,
+                            (size_t)N * f, (size_t)N * f, (size_t)beam_pages * 4, (size_t)beam_pages * 4,
+                            (size_t)N * 4, (size_t)N * 4, (size_t)N * beam_cap[2] * 4, (size_t)N * beam_cap[2] * 4,
+                            battend_bytes, bselect_bytes};
+    size_t total = 0;
+    for (size_t b : sizes) total += align256(std::max<size_t>(b, 16));
+    bw.reserve(total);
+    int i = 0;
+    auto take = [&](auto*& p) { p = static_cast<std::remove_reference_t<decltype(p)>>(bw.take(std::max<size_t>(sizes[i++], 16))); };
+    take(bst); take(brow); take(bk); take(bv); take(bx); take(bq); take(batt); take(bfc); take(blogits); take(new_k);
+    take(new_v); take(bscore[0]); take(bscore[1]); take(btable[0]); take(btable[1]); take(bdone[0]); take(bdone[1]);
+    take(bhist[0]); take(bhist[1]);
+    battend = bw.take(std::max<size_t>(battend_bytes, 16));
+    bselect = bw.take(std::max<size_t>(bselect_bytes, 16));
+  }
+
+  // A step of n beams, whose tables, scores and histories are those of `side`;
+  // the new ones go to the other.
+  void enqueue_beams(int n, int side, bool hf, int max_length, int steps) {
+    hipLaunchKernelGGL(beam_embed_kernel, dim3(n), dim3(320), 0, s, bst, hf ? 1 : 0, mel_emb, pos_emb, bx);
+    const mit2cfm_kv_rows rows = beam_rows(n, max_length);
+    for (int l = 0; l < L; ++l) {
+      const GptLayerDev& w = layer[l];
+      GemvArgs a;
+      a.st = brow;
+      a.w = w.attn_w; a.bias = w.attn_b; a.N = kQKV; a.x = bx; a.g1 = w.ln1_w; a.b1 = w.ln1_b;
+      a.q = bq; a.kc = new_k; a.vc = new_v;
+      launch_qkv_rows(a, s);
+      const mit2cfm_kv_cache cache = beam_cache(l, side);
+      mit2cfm_kv_append put{};
+      put.k = new_k; put.v = new_v;
+      put.k_row = put.v_row = kHD;
+      put.k_head = put.v_head = kPlainRows * kHD;
+      kv_append(cache, rows, put, s);
+      mit2cfm_kv_attention att{};
+      att.q = bq; att.out = batt;
+      att.q_row = att.out_row = kW;
+      att.q_head = att.out_head = kHD;
+      att.q_heads = kHeads;
+      att.scale = 0.125f;
+      att.workspace = battend;
+      att.workspace_bytes = battend_bytes;
+      kv_attention(cache, rows, att, s);
+      a = GemvArgs();
+      a.st = brow;
+      a.w = w.proj_w; a.bias = w.proj_b; a.N = kW; a.x = batt; a.y = bx;
+      launch_attn_proj_rows(a, s);
+      a.w = w.fc_w; a.bias = w.fc_b; a.N = kMLP; a.x = bx; a.g1 = w.ln2_w; a.b1 = w.ln2_b; a.y = bfc;
+      launch_fc_rows(a, s);
+      a = GemvArgs();
+      a.st = brow;
+      a.w = w.mp_w; a.bias = w.mp_b; a.N = kW; a.x = bfc; a.y = bx;
+      launch_mlp_proj_rows(a, s);
+    }
+    for (int b = 0; b < n; ++b) {
+      GemvArgs a;
+      a.st = brow; a.check_stop = 0;
+      a.w = head_w; a.bias = head_b; a.N = kVocab; a.x = bx + (size_t)b * kW; a.g1 = lnf_w; a.b1 = lnf_b; a.g2 = fn_w;
+      a.b2 = fn_b; a.y = blogits + (size_t)b * kVocab; a.blk_val = blk_val; a.blk_idx = blk_idx; a.lnf_out = lnf;
+      a.fn_out = fn;
+      launch_head(a, s);
+    }
+    GPT_OK(hipGetLastError());
+    beam_select(beam_pick(n, side), s);
+    beam_reorder(beam_cache(0, side), beam_move(n, side, steps), s);
+    hipLaunchKernelGGL(beam_advance_kernel, dim3(1), dim3(64), 0, s, bst);
+    GPT_OK(hipGetLastError());
+  }
+
   // Prefix rows into the caches: as row products in chunks of up to
   // kPrefillRows rows (returns the last row's hidden state) ...
   const float* prefill(int n) {
@@ -1920,6 +2112,143 @@ void GptDecoder::generate(const float* prefix, int prefix_tokens, int steps, boo
   if (steps > 0)
     GPT_OK(hipMemcpy(out.last_processed_logits.data(), sampling ? d.proc : d.logits, kVocab * sizeof(float),
                      hipMemcpyDeviceToHost));
+  float ms = 0.f;
+  GPT_OK(hipEventElapsedTime(&ms, d.ev[0], d.ev[1]));
+  out.prefill_ms = ms;
+  GPT_OK(hipEventElapsedTime(&ms, d.ev[1], d.ev[2]));
+  out.decode_ms = ms;
+}
+
+void GptDecoder::kv_beam(const float* prefix, int prefix_tokens, int steps, bool hf, int beams, Beams& out) {
+  Impl& d = *d_;
+  if (beams < 1 || beams > kMaxBeams)
+    throw std::invalid_argument("gpt: beams must be in [1, " + std::to_string(kMaxBeams) + "]");
+  if (prefix_tokens < 0 || steps < 1) throw std::invalid_argument("gpt: prefix_tokens must be >= 0, steps >= 1");
+  if (prefix_tokens > 0 && !prefix) throw std::invalid_argument("gpt: prefix must not be NULL");
+  if ((hf && steps > 1 ? steps : steps - 1) >= kPos)
+    throw std::invalid_argument("gpt: " + std::to_string(steps) + " steps pass the " + std::to_string(kPos) +
+                                "-row mel position table");
+  const int max_length = prefix_tokens + steps;
+  d.ensure(prefix_tokens + 1, prefix_tokens + 1, 1);
+  d.ensure_beams(beams, max_length, steps);
+  GPT_OK(hipEventRecord(d.ev[0], d.s));
+  if (prefix_tokens > 0) {  // the prefix through the layers, as generate() takes it
+    GPT_OK(hipMemcpyAsync(d.rows, prefix, (size_t)prefix_tokens * kW * sizeof(float), hipMemcpyHostToDevice, d.s));
+    bool plain = d.row_prefill();
+    for (;;) {
+      d.reset_state(prefix_tokens, prefix_tokens, plain ? 0 : prefix_tokens, hf, 1);
+      if (plain)
+        d.prefill_plain(prefix_tokens);
+      else
+        d.prefill(prefix_tokens);
+      GPT_OK(hipMemcpyAsync(d.host_state, d.st, sizeof(GptState), hipMemcpyDeviceToHost, d.s));
+      GPT_OK(hipStreamSynchronize(d.s));
+      if (plain || !d.host_state->overflow) break;
+      d.counts.range_reruns += 1;
+      plain = true;
+    }
+  }
+  // One search: the prefix goes to beam 0's pages, and the others become its
+  // children, sharing its full pages.
+  BeamState h{};
+  for (int b = 0; b <= kPlainRows; ++b) h.start[b] = std::min(b, beams);
+  for (int b = 0; b < kPlainRows; ++b) {
+    h.length[b] = prefix_tokens;
+    h.token[b] = kStart;
+  }
+  h.prefix[1] = prefix_tokens;
+  GptState rows_state{};
+  rows_state.pend = beams;
+  rows_state.cap = kPlainRows;
+  rows_state.rows = beams;
+  std::vector<int32_t> table((size_t)beams * d.beam_entries);
+  for (size_t i = 0; i < table.size(); ++i) table[i] = (int32_t)i;
+  std::vector<float> score(beams, -INFINITY);
+  score[0] = 0.f;
+  const std::vector<int32_t> zeros(beams, 0);
+  GPT_OK(hipMemcpyAsync(d.bst, &h, sizeof(h), hipMemcpyHostToDevice, d.s));
+  GPT_OK(hipMemcpyAsync(d.brow, &rows_state, sizeof(rows_state), hipMemcpyHostToDevice, d.s));
+  GPT_OK(hipMemcpyAsync(d.btable[1], table.data(), table.size() * 4, hipMemcpyHostToDevice, d.s));
+  GPT_OK(hipMemcpyAsync(d.bscore[0], score.data(), score.size() * 4, hipMemcpyHostToDevice, d.s));
+  GPT_OK(hipMemcpyAsync(d.bdone[0], zeros.data(), zeros.size() * 4, hipMemcpyHostToDevice, d.s));
+  for (int l = 0; l < d.L && prefix_tokens > 0; ++l) {
+    mit2cfm_kv_rows r{};
+    r.start = d.bst->prefix;
+    r.length = d.bst->length;
+    r.seqs = 1;
+    r.rows = (uint32_t)prefix_tokens;
+    mit2cfm_kv_append put{};
+    put.k = d.kc + (size_t)l * d.cap * kW;
+    put.v = d.vc + (size_t)l * d.cap * kW;
+    put.k_row = put.v_row = kHD;
+    put.k_head = put.v_head = (uint64_t)d.cap * kHD;
+    kv_append(d.beam_cache(l, 1), r, put, d.s);
+  }
+  mit2cfm_beam_reorder share = d.beam_move(beams, 1, steps);
+  share.state = nullptr;
+  share.token = nullptr;
+  beam_reorder(d.beam_cache(0, 1), share, d.s);
+  hipLaunchKernelGGL(beam_advance_kernel, dim3(1), dim3(64), 0, d.s, d.bst);  // the first step's rows, ...
+  const int32_t zero = 0;
+  GPT_OK(hipMemcpyAsync(&d.bst->step, &zero, 4, hipMemcpyHostToDevice, d.s));  // ... but step 0
+  GPT_OK(hipEventRecord(d.ev[1], d.s));
+  GPT_OK(hipStreamSynchronize(d.s));
+
+  // Two steps, one from each side, replayed as a graph.
+  hipGraphExec_t pair = nullptr;
+  struct Drop {
+    hipGraphExec_t& g;
+    ~Drop() {
+      if (g) (void)hipGraphExecDestroy(g);
+    }
+  } drop{pair};
+  if (d.use_graph && steps >= kStepsPerCheck) {
+    hipGraph_t g = nullptr;
+    GPT_OK(hipStreamBeginCapture(d.s, hipStreamCaptureModeThreadLocal));
+    try {
+      d.enqueue_beams(beams, 0, hf, max_length, steps);
+      d.enqueue_beams(beams, 1, hf, max_length, steps);
+    } catch (...) {
+      (void)hipStreamEndCapture(d.s, &g);
+      if (g) (void)hipGraphDestroy(g);
+      throw;
+    }
+    GPT_OK(hipStreamEndCapture(d.s, &g));
+    const hipError_t err = hipGraphInstantiate(&pair, g, nullptr, nullptr, 0);
+    (void)hipGraphDestroy(g);
+    GPT_OK(err);
+  }
+  std::vector<int32_t> finished(beams);
+  int done = 0;
+  while (done < steps) {
+    const int n = std::min(kStepsPerCheck, steps - done);
+    for (int i = 0; i < n;) {
+      if (pair && i + 2 <= n) {
+        GPT_OK(hipGraphLaunch(pair, d.s));
+        i += 2;
+      } else {
+        d.enqueue_beams(beams, (done + i) & 1, hf, max_length, steps);
+        i += 1;
+      }
+    }
+    done += n;
+    GPT_OK(hipMemcpyAsync(finished.data(), d.bdone[done & 1], (size_t)beams * 4, hipMemcpyDeviceToHost, d.s));
+    GPT_OK(hipStreamSynchronize(d.s));
+    if (std::all_of(finished.begin(), finished.end(), [](int32_t f) { return f != 0; })) break;
+  }
+  d.counts.plain_steps += (uint64_t)done;
+  GPT_OK(hipEventRecord(d.ev[2], d.s));
+  GPT_OK(hipStreamSynchronize(d.s));
+  std::vector<uint32_t> hist((size_t)beams * steps);
+  out.scores.resize(beams);
+  GPT_OK(hipMemcpy(hist.data(), d.bhist[done & 1], hist.size() * 4, hipMemcpyDeviceToHost));
+  GPT_OK(hipMemcpy(out.scores.data(), d.bscore[done & 1], (size_t)beams * 4, hipMemcpyDeviceToHost));
+  out.predicted.assign(beams, {});
+  for (int b = 0; b < beams; ++b)
+    for (int i = 0; i < done; ++i) {
+      out.predicted[b].push_back(hist[(size_t)b * steps + i]);
+      if (out.predicted[b].back() == kStopToken) break;
+    }
   float ms = 0.f;
   GPT_OK(hipEventElapsedTime(&ms, d.ev[0], d.ev[1]));
   out.prefill_ms = ms;

@@ -131,6 +131,8 @@ def lib() -> ctypes.CDLL:
         "mit2cfm_gpt_kv_sample": (st, [vp, _f32p, u32, u32, i32, ctypes.POINTER(_GptSampling), _u32p, u32, _u32p,
                                        _u32p, _u32p, _u32p, ctypes.POINTER(i32), _f32p, _f32p,
                                        ctypes.POINTER(ctypes.c_double)]),
+        "mit2cfm_gpt_kv_beam": (st, [vp, _f32p, u32, u32, i32, u32, _u32p, _u32p, _f32p,
+                                     ctypes.POINTER(ctypes.c_double)]),
         "mit2cfm_gpt_profile_launch": (st, [vp, i32, u32, ctypes.POINTER(ctypes.c_double),
                                             ctypes.POINTER(ctypes.c_char_p)]),
         "mit2cfm_kv_attention_workspace": (u64, [ctypes.POINTER(KvCache), ctypes.POINTER(KvRows), u32]),
@@ -777,6 +779,21 @@ class Context:
         return {"predicted": pred[:n_pred[0]].copy(), "input_tokens": inp[:n_in[0]].copy(),
                 "first_stop_step": int(stop.value), "last_logits": logits if steps > 0 else None,
                 "last_processed_logits": proc if steps > 0 else None,
+                "prefill_ms": float(t[0]), "decode_ms": float(t[1])}
+
+    def gpt_kv_beam(self, prefix, steps: int, beams: int = 3, hf_generate_positions: bool = False) -> dict:
+        """Beam search over the mel codes: prefix [P, 1280] -> dict with predicted (a
+        uint32 array for each hypothesis, best first), scores [beams] (sums of log
+        probabilities) and prefill_ms / decode_ms (device time)."""
+        x = _f32(prefix).reshape(-1, GPT_WIDTH)
+        P = x.shape[0]
+        pred = np.zeros((max(beams, 1), max(steps, 1)), np.uint32)
+        n_pred = np.zeros(max(beams, 1), np.uint32)
+        scores = np.zeros(max(beams, 1), np.float32)
+        t = (ctypes.c_double * 2)()
+        self._c(lib().mit2cfm_gpt_kv_beam(self._h, _p(x) if P else None, P, steps, 1 if hf_generate_positions else 0,
+                                          beams, _pu(pred), _pu(n_pred), _p(scores), t))
+        return {"predicted": [pred[b, :n].copy() for b, n in enumerate(n_pred)], "scores": scores,
                 "prefill_ms": float(t[0]), "decode_ms": float(t[1])}
 
     def gpt_cached_decode(self, rows, prefix_tokens: int):

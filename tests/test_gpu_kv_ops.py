@@ -352,6 +352,33 @@ def test_offsets_past_32_bits(mit2, ctx):
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,new", [(64, (20, 20), [25, 1, 9]), (128, (32, 8), [63, 40, 0, 12]), (96, (6, 2), [40, 3])])
+def test_drafted_trees_appended_and_attended(mit2, ctx, dtype, dim, heads, new):
+    """A draft's check as it is used: the trees' rows appended at their depths' positions, their queries rotated on the way, and
+    attended over the cache, one call behind the other."""
+    b = Batch(new, [n + 70 * (s + 1) for s, n in enumerate(new)], page=16, q_heads=heads[0], kv_heads=heads[1], dim=dim, dtype=dtype, seed=dim, tail_rows=1)
+    mask, depth = ops_ref.trees(b, 21)
+    position = np.zeros(b.rows, np.int32)
+    for row, s, _, before in b.each_row():
+        position[row] = before + depth[row]
+    on = On(mit2, b)
+    put, att = on.append_args(position=position, rot=dim), on.attention_args(mask=mask)
+    out = torch.full_like(on.out, math.nan)
+    att.q, att.out = on.out.data_ptr(), out.data_ptr()
+    torch.cuda.synchronize()
+    ctx.kv_append_device(on.cache, on.rows, put)
+    ctx.kv_attention_device(on.cache, on.rows, att, sync=True)
+    q, k, v = ops_ref.append64(b, position, dim, False, 10000.0)
+    for got, want, step in ((on.out, q, 1.0), (on.k, k, 1.0), (on.v, v, 0.0)):
+        off = (got.double().cpu() - want).abs().nan_to_num(0.0)
+        assert bool((off <= step * (HALF_STEP[dtype] * want.abs().nan_to_num(0.0) + 2e-6 * 8)).all())
+    b.q, b.k, b.v = on.out.cpu(), on.k.cpu(), on.v.cpu()  # (what the attention was given)
+    ref, tol = ops_ref.attention64(b, dim ** -0.5, mask)
+    mine = _mine(b)
+    _check(out.double().cpu()[mine], ref[mine], tol[mine], f"trees {dtype} {dim}")
+
+
 class Graph:
     """The context's stream captured into a graph."""
 
