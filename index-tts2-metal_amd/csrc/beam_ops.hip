@@ -6,6 +6,7 @@
 #include <cfloat>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "device_common.h"
 #include "engine.h"
@@ -70,16 +71,22 @@ __device__ __forceinline__ uint32_t float_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-// The largest number that at least n of a wave's keys reach (0: fewer than n are
-// over 0), built from its top bit by votes.
+// The largest number that at least n of a wave's keys, of BITS bits, reach (0: fewer
+// than n are over 0), built from its top bit by votes.
+template <int BITS>
 __device__ __forceinline__ uint32_t reached_by(uint32_t key, int n) {
   uint32_t t = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = BITS - 1; bit >= 0; --bit) {
     const uint32_t c = t | 1u << bit;
     t = __popcll(__ballot(key >= c)) >= n ? c : t;
   }
   return t;
+}
+
+// The key that a wave's lanes with `has` (some have) share.
+__device__ __forceinline__ uint32_t key_of_wave(uint32_t key, bool has) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)key, __ffsll((unsigned long long)__ballot(has)) - 1);
 }
 
 // Whether a live beam's logits count: it exists and is not finished.
@@ -90,14 +97,19 @@ __device__ __forceinline__ bool live(const SelectArgs& a, int r) {
 // Block (split, row): the split's maximum, the sum of its exponentials and its
 // `count` best, of one pass over its logits, which stay in registers.
 //
-// The best: every thread's largest logit, ties to the lower token; of each wave's
-// 64 the count-th, by votes; the largest of those is reached by at least `count`
-// logits of the split and by those of at most count threads a wave, which
-// alone list what they have from it on; the few in the list find their ranks by
-// counting.  No order of threads or atomics shows in the result.
+// The best: every thread's largest logit; of each wave's 64 the count-th, by
+// votes, and where more than count threads reach it (ties) the lowest tokens among
+// them; the largest of those bounds is reached by at least `count` logits of the
+// split and by those of at most count threads a wave, which alone list what they
+// have from it on; the few in the list find their ranks by counting.  No order
+// of threads or atomics shows in the result.
+//
+// Bound by its own steps (votes, ranks) more than by the loads: 17 us for 256 rows
+// of 50001 bf16, whose 26 MB take 6; 6.3 us for three rows of 8194, which is one
+// block's way through.  With 32 logits a thread 17 and 8 us.
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs a) {
-  constexpr int W = 16 / sizeof(T);  // logits of a load
+  constexpr int W = 16 / sizeof(T), LOADS = kPerThread / W;  // logits of a load
   struct alignas(16) Load {
     T v[W];
   };
@@ -107,14 +119,12 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
   __shared__ double s_sum[kSelectWaves];
   __shared__ uint32_t s_n;
   const int r = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (!live(a, r)) return;  // its logits do not matter
   const T* x = static_cast<const T*>(a.logits) + r * a.row;
-  const int from = split * a.chunk, to = min(from + a.chunk, a.vocab);
-  // loads lie on 16 bytes, up to W - 1 logits before the split's first
-  const int skew = (int)(reinterpret_cast<uintptr_t>(x + from) % 16 / sizeof(T));
-  constexpr int LOADS = kPerThread / W + 1;  // (the last for what the skew pushes out)
-  float v[LOADS * W];  // NaN: outside the split
-  const int at = from - skew + tid * W;
+  // splits begin on 16 bytes, the first up to W - 1 logits before the row
+  const int skew = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+  const int begin = split * a.chunk - skew, from = max(begin, 0), to = min(begin + a.chunk, a.vocab);
+  float v[kPerThread];  // -inf outside the split
+  const int at = begin + tid * W;
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int t0 = at + i * kSelectThreads * W;
@@ -124,37 +134,39 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
       for (int e = 0; e < W; ++e) v[i * W + e] = logit(l.v[e]);
     } else {
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[i * W + e] = t0 + e >= from && t0 + e < to ? logit(x[t0 + e]) : NAN;
+      for (int e = 0; e < W; ++e) v[i * W + e] = t0 + e >= from && t0 + e < to ? logit(x[t0 + e]) : -INFINITY;
     }
   }
+  if (!live(a, r)) return;  // its logits do not matter (looked up behind the loads, not before them)
   if (tid == 0) s_n = 0;
-  // (a comparison with NaN is false, a maximum takes the other number)
-  float top = -INFINITY;
-  int best_t = -1;
+  auto token = [&](int k) { return at + k / W * kSelectThreads * W + k % W; };
+  auto inside = [&](int k) { return token(k) >= from && token(k) < to; };
+  float top = v[0];
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-      const bool up = v[i * W + e] > top;
-      top = up ? v[i * W + e] : top;
-      best_t = up ? at + i * kSelectThreads * W + e : best_t;
-    }
-  if (best_t < 0) {  // nothing over -inf: the first that there is
-#pragma unroll
-    for (int i = LOADS - 1; i >= 0; --i)
-#pragma unroll
-      for (int e = W - 1; e >= 0; --e)
-        best_t = v[i * W + e] == v[i * W + e] ? at + i * kSelectThreads * W + e : best_t;
-  }
+  for (int k = 1; k < kPerThread; ++k) top = fmaxf(top, v[k]);
   float m = top;
 #pragma unroll
   for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
-  const uint32_t key = best_t < 0 ? 0u : float_key(top);
-  const uint32_t t32 = reached_by(key, a.count);
-  uint64_t kth = (uint64_t)t32 << 32;
-  const int ties = __popcll(__ballot(key == t32)), over = __popcll(__ballot(key > t32));
-  if (t32 != 0 && over + ties > a.count)  // of equal ones the lowest tokens
-    kth |= reached_by(key == t32 ? ~(uint32_t)best_t : 0u, a.count - over);
+  // a thread that has any logit: its first load's last, or a later load's first, is inside
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) any |= at + i * kSelectThreads * W + W > from && at + i * kSelectThreads * W < to;
+  // (a 16-bit type's values differ in their upper bits alone)
+  constexpr int LOW = sizeof(T) == 4 ? 0 : std::is_same<T, half_t>::value ? 13 : 16;
+  const uint32_t key = any ? float_key(top) : 0u, high = key >> LOW, t32 = reached_by<32 - LOW>(high, a.count);
+  uint64_t kth = (uint64_t)(t32 << LOW) << 32;
+  const int over = __popcll(__ballot(high > t32)), ties = __popcll(__ballot(high == t32));
+  if (t32 != 0 && over + ties > a.count) {
+    int first = 0;  // the thread's lowest token of that value
+#pragma unroll
+    for (int k = kPerThread - 1; k >= 0; --k) first = v[k] == top && inside(k) ? token(k) : first;
+    constexpr int PLACES = 15;  // of a chunk's tokens, counted from its end
+    static_assert(kMaxChunk < 1 << PLACES, "a chunk's tokens fit the search");
+    const uint32_t place =
+        reached_by<PLACES>(high == t32 ? (uint32_t)(kMaxChunk - (first - begin)) : 0u, a.count - over);
+    const uint32_t tied = key_of_wave(key, high == t32);
+    kth = (uint64_t)tied << 32 | ~(uint32_t)(begin + kMaxChunk - (int)place);
+  }
   if (lane == 0) {
     s_max[wave] = m;
     s_kth[wave] = kth;
@@ -170,27 +182,23 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
   // far below the largest weighs as little; a thread's few terms are summed in
   // fp32, in pairs)
   const float base = m == -INFINITY ? 0.f : m;
-  float part[LOADS * W];
+  float part[kPerThread];
 #pragma unroll
-  for (int i = 0; i < LOADS * W; ++i)
-    part[i] = __builtin_amdgcn_exp2f(fmaxf((v[i] - base) * 1.4426950408889634f, -INFINITY));
+  for (int k = 0; k < kPerThread; ++k) part[k] = __builtin_amdgcn_exp2f((v[k] - base) * 1.4426950408889634f);
 #pragma unroll
-  for (int w = LOADS * W; w > 1; w = (w + 1) / 2)
+  for (int w = kPerThread / 2; w >= 1; w /= 2)
 #pragma unroll
-    for (int i = 0; i < w / 2; ++i) part[i] += part[w - 1 - i];
+    for (int k = 0; k < w; ++k) part[k] += part[k + w];
   double sum = (double)part[0];
 #pragma unroll
   for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, kWave);
   if (lane == 0) s_sum[wave] = sum;
-  const uint64_t best = best_t < 0 ? 0 : rank_key(top, (uint32_t)best_t);
-  if (best != 0 && best >= least) {
+  if (key != 0 && key >= (uint32_t)(least >> 32)) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const uint64_t k = rank_key(v[i * W + e], (uint32_t)(at + i * kSelectThreads * W + e));
-        if (v[i * W + e] == v[i * W + e] && k >= least) list[atomicAdd(&s_n, 1u)] = k;
-      }
+    for (int k = 0; k < kPerThread; ++k) {
+      const uint64_t rk = rank_key(v[k], (uint32_t)token(k));
+      if (inside(k) && rk >= least) list[atomicAdd(&s_n, 1u)] = rk;
+    }
   }
   __syncthreads();
   const int n = (int)s_n;
@@ -242,7 +250,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
   __shared__ uint32_t s_n;
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) s_n = 0;
-  for (int b = tid >> 2; b < a.beams; b += kSelectThreads / 4) {  // four lanes a beam
+  for (int b = tid >> 4; b < a.beams; b += kSelectThreads / 16) {  // sixteen lanes a beam
     const int r = g * a.beams + b;
     const float cum = a.scores[r];
     const int kind = (cum > -INFINITY ? 0 : 2) | (a.finished && a.finished[r] != 0 ? 1 : 0);
@@ -251,17 +259,17 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
       const double* sums = a.sums + (size_t)r * a.splits;
       const float* tops = a.tops + (size_t)r * a.splits;
       float m = -INFINITY;
-      for (int s = tid & 3; s < a.splits; s += 4) m = fmaxf(m, tops[s]);
-      m = fmaxf(m, __shfl_xor(m, 1, kWave));
-      m = fmaxf(m, __shfl_xor(m, 2, kWave));
+      for (int s = tid & 15; s < a.splits; s += 16) m = fmaxf(m, tops[s]);
+#pragma unroll
+      for (int w = 1; w < 16; w *= 2) m = fmaxf(m, __shfl_xor(m, w, kWave));
       double sum = 0.0;
-      for (int s = tid & 3; s < a.splits; s += 4)
+      for (int s = tid & 15; s < a.splits; s += 16)
         if (tops[s] > -INFINITY) sum += sums[s] * exp((double)tops[s] - (double)m);
-      sum += __shfl_xor(sum, 1, kWave);
-      sum += __shfl_xor(sum, 2, kWave);
+#pragma unroll
+      for (int w = 1; w < 16; w *= 2) sum += __shfl_xor(sum, w, kWave);
       if (m > -INFINITY) off = (double)cum - ((double)m + log(sum));
     }
-    if ((tid & 3) == 0) {
+    if ((tid & 15) == 0) {
       s_off[b] = off;
       s_cum[b] = cum;
       s_kind[b] = (uint8_t)kind;
@@ -312,7 +320,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
   auto rounded = [](const Scored& x) { return x.s == 0 ? 0u : float_key((float)key_score(x.s)); };
   uint32_t best = 0;
   each([&](const Scored& x) { best = max(best, rounded(x)); });
-  const uint32_t kth = reached_by(best, a.count);
+  const uint32_t kth = reached_by<32>(best, a.count);
   if (lane == 0) s_kth[wave] = kth;
   __syncthreads();
   uint32_t least = 1;
@@ -327,12 +335,14 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
   __syncthreads();
   const int m = (int)s_n;
   if (m <= kGroupList) {
-    for (int j = tid; j < m; j += kSelectThreads) {
+    for (int j = tid >> 2; j < m; j += kSelectThreads / 4) {  // four lanes a candidate
       const Scored x = list[j];
       int rank = 0;
 #pragma unroll 4
-      for (int o = 0; o < m; ++o) rank += list[o].over(x) ? 1 : 0;
-      if (rank < a.count) write(x, rank);
+      for (int o = tid & 3; o < m; o += 4) rank += list[o].over(x) ? 1 : 0;
+      rank += __shfl_xor(rank, 1, kWave);
+      rank += __shfl_xor(rank, 2, kWave);
+      if ((tid & 3) == 0 && rank < a.count) write(x, rank);
     }
     return;
   }
@@ -363,8 +373,9 @@ bool select_in_range(const mit2cfm_beam_select& a) {
          a.count <= (uint64_t)a.beams * a.vocab && (uint64_t)a.groups * a.beams <= 65535;
 }
 size_t align16(size_t b) { return (b + 15) & ~size_t(15); }
-// A row's logits in even splits of at most kMaxChunk.
-int select_splits(uint32_t vocab) { return (int)((vocab + kMaxChunk - 1) / kMaxChunk); }
+// A row's logits in even splits of at most kMaxChunk, which begin up to 7 logits
+// before it.
+int select_splits(uint32_t vocab) { return (int)((vocab + 7 + kMaxChunk - 1) / kMaxChunk); }
 
 // ------------------------------------------------------------------ reorder
 struct ReorderArgs {
@@ -484,7 +495,7 @@ void beam_select(const mit2cfm_beam_select& p, hipStream_t s) {
   a.beams = (int)p.beams; a.vocab = (int)p.vocab; a.count = (int)p.count;
   a.stop = p.stop_token;
   a.splits = select_splits(p.vocab);
-  a.chunk = (int)((p.vocab + a.splits - 1) / a.splits + 7) / 8 * 8;
+  a.chunk = (int)((p.vocab + 7 + a.splits - 1) / a.splits + 7) / 8 * 8;
   a.scores = p.scores; a.finished = p.finished;
   a.scores_out = p.scores_out; a.parent_out = p.parent_out; a.token_out = p.token_out; a.finished_out = p.finished_out;
   const uint32_t rows = p.groups * p.beams;
@@ -497,7 +508,7 @@ void beam_select(const mit2cfm_beam_select& p, hipStream_t s) {
   a.tops = reinterpret_cast<float*>(w);
   const dim3 grid(a.splits, rows), block(kSelectThreads);
   // the list holds all logits of count threads a wave
-  const size_t lds = std::min<size_t>((size_t)kSelectWaves * a.count * (kPerThread + 8), kMaxChunk) * 8;
+  const size_t lds = std::min<size_t>((size_t)kSelectWaves * a.count * kPerThread, kMaxChunk) * 8;
   if (p.dtype == MIT2CFM_DTYPE_F32)
     hipLaunchKernelGGL((select_rows_kernel<float>), grid, block, lds, s, a);
   else if (p.dtype == MIT2CFM_DTYPE_F16)

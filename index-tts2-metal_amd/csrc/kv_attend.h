@@ -114,16 +114,23 @@ __device__ __forceinline__ int chunk_of(int len, int chunk, int splits) {
   return max(chunk, (least + kChunkStep - 1) / kChunkStep * kChunkStep);
 }
 
-// The sequence and its tile (of `mtile` query rows) that tile number t of the
-// whole batch is; false past the last.
-__device__ __forceinline__ bool find_tile(const RowView& r, int group, int mtile, int t, int& seq, int& in_seq) {
+// The sequence that tile number t of the whole batch (of `mtile` query rows)
+// belongs to, its number there, the sequence's bounds and its length; false past
+// the last.  A wave's lanes look at 64 sequences at a time.
+struct Found {
+  int seq, in_seq, start, stop, length;
+};
+__device__ __forceinline__ bool find_tile(const RowView& r, int group, int mtile, int t, Found& f) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int base = 0; base < r.seqs; base += 64) {
-    int n = 0;
+    int n = 0, s0 = 0, s1 = 0, length = 0;
     if (base + lane < r.seqs) {
-      const int s0 = max(r.start[base + lane], 0), s1 = min(r.start[base + lane + 1], r.rows);
-      n = s1 > s0 ? (int)(((int64_t)(s1 - s0) * group + mtile - 1) / mtile) : 0;
+      s0 = r.start[base + lane];
+      s1 = r.start[base + lane + 1];
+      length = r.length[base + lane];
+      const int rows = min(s1, r.rows) - max(s0, 0);
+      n = rows > 0 ? (int)(((int64_t)rows * group + mtile - 1) / mtile) : 0;
     }
     int incl = n;
 #pragma unroll
@@ -134,11 +141,14 @@ __device__ __forceinline__ bool find_tile(const RowView& r, int group, int mtile
     const uint64_t past = __ballot(before + incl > t);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      seq = __builtin_amdgcn_readfirstlane(base + l);
-      in_seq = __builtin_amdgcn_readfirstlane(t - (before + __shfl(incl - n, l, kWave)));
+      f.seq = __builtin_amdgcn_readfirstlane(base + l);
+      f.in_seq = t - before - __builtin_amdgcn_readlane(incl - n, l);
+      f.start = __builtin_amdgcn_readlane(s0, l);
+      f.stop = __builtin_amdgcn_readlane(s1, l);
+      f.length = __builtin_amdgcn_readlane(length, l);
       return true;
     }
-    before += __shfl(incl, 63, kWave);
+    before += __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
 }
@@ -156,7 +166,7 @@ struct Part {
   bool whole;            // one split holds all keys: results are final
 };
 __device__ __forceinline__ bool find_part(const AttendArgs& a, const AttendPlan& plan, int mtile, Part& p) {
-  int in_seq, tile = blockIdx.x, unit = blockIdx.y;
+  int tile = blockIdx.x, unit = blockIdx.y;
   if (plan.by_xcd) {
     const int slot = blockIdx.x >> 3;
     unit = slot / plan.tiles * 8 + (blockIdx.x & 7);
@@ -165,12 +175,14 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, const AttendPlan&
   }
   p.kvh = unit % a.c.kv_heads;
   p.split = unit / a.c.kv_heads;
-  if (!find_tile(a.r, a.group, mtile, tile, p.seq, in_seq)) return false;
-  p.raw_start = a.r.start[p.seq];
-  const int stop = a.r.start[p.seq + 1], length = a.r.length[p.seq];
+  Found f;
+  if (!find_tile(a.r, a.group, mtile, tile, f)) return false;
+  p.seq = f.seq;
+  p.raw_start = f.start;
+  const int stop = f.stop, length = f.length;
   p.start = max(p.raw_start, 0);
   p.mrows = (min(stop, a.r.rows) - p.start) * a.group;
-  p.m0 = in_seq * mtile;
+  p.m0 = f.in_seq * mtile;
   p.first = length - (stop - p.raw_start);
   p.len = min(length, a.c.capacity());
   const int chunk = chunk_of(p.len, plan.chunk, plan.splits);
