@@ -32,6 +32,14 @@ struct AttendArgs {
   float scale2;        // |scale| log2(e): scores in powers of two
 };
 
+// What splits leave for their join: [row][query head][split] outputs, maxima and
+// weights' sums, [row][query head] the number of splits.
+struct Parts {
+  float* o;
+  float2* ml;
+  int32_t* n;
+};
+
 // How a launch is laid out (attend_plan, kv_ops.hip).
 struct AttendPlan {
   int form;    // query tiles a wave (1, 2, 4), kWide: the block kernel
@@ -41,7 +49,8 @@ struct AttendPlan {
   int by_xcd;  // blocks of a key head and split on one XCD (see find_part)
 };
 constexpr int kWide = 0;
-constexpr int kChunkStep = 128;  // a split's keys are a multiple of it
+// A split's keys are a multiple of this: a tile for each of a block's waves.
+constexpr int chunk_step(bool f32) { return f32 ? 64 : 128; }
 
 // Launches a plan's kernels; throws HipError.
 void launch_attend_f32(const AttendArgs& a, const AttendPlan& plan, int D, void* workspace, hipStream_t s);
@@ -110,8 +119,8 @@ struct alignas(N * sizeof(T) % 16 == 0 ? 16 : N * sizeof(T) % 8 == 0 ? 8 : 4) Pi
 
 // Keys of a split of a sequence of len keys.
 __device__ __forceinline__ int chunk_of(int len, int chunk, int splits) {
-  const int least = (max(len, 0) + splits - 1) / splits;
-  return max(chunk, (least + kChunkStep - 1) / kChunkStep * kChunkStep);
+  const int least = (max(len, 0) + splits - 1) / splits, step = chunk_step(false);
+  return max(chunk, (least + step - 1) / step * step);
 }
 
 // The sequence that tile number t of the whole batch (of `mtile` query rows)
@@ -163,6 +172,7 @@ struct Part {
   int mrows, m0;         // the sequence's query rows; the tile's first
   int first, len;        // cached rows before the new ones, and all
   int begin, end;        // the split's keys
+  int parts;             // splits that hold keys
   bool whole;            // one split holds all keys: results are final
 };
 __device__ __forceinline__ bool find_part(const AttendArgs& a, const AttendPlan& plan, int mtile, Part& p) {
@@ -189,6 +199,7 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, const AttendPlan&
   p.begin = p.split * chunk;
   p.end = min(p.begin + chunk, p.len);
   p.whole = p.len <= chunk;
+  p.parts = p.whole ? 1 : (p.len + chunk - 1) / chunk;
   return p.split == 0 || p.begin < p.len;
 }
 
@@ -391,8 +402,7 @@ constexpr int kAttendWaves = 4, kAttendThreads = kAttendWaves * 64;
 // from memory straight into operands: nothing passes LDS until the join.
 // BIG: a tile of keys lies in one page, whose entry is the same for all lanes.
 template <typename T, int D, int MT, bool BIG>
-__global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a, AttendPlan plan, float* part_o,
-                                                                float2* part_ml) {
+__global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a, AttendPlan plan, Parts part) {
   typedef Dims<T, D> S;
   typedef typename Mat<T>::op Op;
   constexpr int KT = S::KT, NT = S::NT, DP = S::DP, DC = S::DC, NV = S::NV;
@@ -558,9 +568,10 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a, At
       } else {
         const size_t at = ((size_t)x.row * a.q_heads + x.h) * plan.splits + p.split;
 #pragma unroll
-        for (int d = 0; d < DP; ++d) part_o[at * D + d0 + d] = O[d];
-        if ((tid & 15) == 0) part_ml[at] = make_float2(mm, L);
+        for (int d = 0; d < DP; ++d) part.o[at * D + d0 + d] = O[d];
+        if ((tid & 15) == 0) part.ml[at] = make_float2(mm, L);
       }
+      if (p.split == 0 && plan.splits > 1 && (tid & 15) == 0) part.n[(size_t)x.row * a.q_heads + x.h] = p.parts;
     }
   }
 }
@@ -597,8 +608,7 @@ __device__ __forceinline__ void load_to_lds(const void* src, lds_ptr_t* lds) {
 // The ring's buffers are objects of their own, named by constants in the usual
 // path: a read that might alias any of them would wait for every load.
 template <typename T, int D>
-__global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendArgs a, AttendPlan plan, float* part_o,
-                                                                     float2* part_ml) {
+__global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendArgs a, AttendPlan plan, Parts part) {
   typedef Dims<T, D> S;
   typedef typename Mat<T>::op Op;
   constexpr int KT = S::KT, NT = S::NT, DP = S::DP, DC = S::DC, NV = S::NV;
@@ -625,6 +635,9 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
     p.end = min(p.end, max(p.first + x.i + 1, p.begin));
   }
   const Query last_q(a, p, min(wm0 + 16 * WMT, p.mrows) - 1);
+  // Keys before this one are seen by all of the wave's rows: of a chain's new rows
+  // those up to the wave's first.
+  const int open = a.mask ? p.first : p.first + Query(a, p, min(wm0, p.mrows - 1)).i + 1;
 
   // This thread's rows of a buffer, and its place of them.
   const int row0 = tid / CPR;
@@ -773,12 +786,12 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
     there1 = there2;
     b0 += KEYS;
   };
-  // All rows see all keys of the buffers up to the first that holds a new row or
-  // misses one: a loop of its own, whose turns follow each other without a branch
+  // All rows see all keys of the buffers up to the first that holds a row which
+  // not all see, or misses one: a loop of its own, whose turns follow each other without a branch
   // that could meet the outputs' registers (merged, they were kept twice).
   int b0 = p.begin, buf = 0;
   if (works) {
-    auto plain = [&] { return there0 == all_keys && b0 + KEYS <= p.first && b0 < p.end; };
+    auto plain = [&] { return there0 == all_keys && b0 + KEYS <= open && b0 < p.end; };
     auto one = [&](auto buf_) {
       constexpr int B = decltype(buf_)::value;
       turn(B, b0);
@@ -840,32 +853,38 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int d = 0; d < DP; d += 4)
-          *reinterpret_cast<float4*>(part_o + at * D + d0 + DP * r + d) =
-              make_float4(run[mt].o[d][r], run[mt].o[d + 1][r], run[mt].o[d + 2][r], run[mt].o[d + 3][r]);
-      if (grp == 0) part_ml[at] = make_float2(run[mt].mx, L);
+          *reinterpret_cast<floatx4*>(part.o + at * D + d0 + DP * r + d) =
+              floatx4{run[mt].o[d][r], run[mt].o[d + 1][r], run[mt].o[d + 2][r], run[mt].o[d + 3][r]};
+      if (grp == 0) part.ml[at] = make_float2(run[mt].mx, L);
     }
+    if (p.split == 0 && plan.splits > 1 && grp == 0) part.n[(size_t)x.row * a.q_heads + x.h] = p.parts;
   }
 }
 
 // Joins a row and query head's splits, WAVES waves for each: lane groups of D/4
 // take every so manyth split, four elements a lane.  One wave where there are
-// at most kFewSplits: blocks of a wave each then fill the chip with less.
-constexpr int kFewSplits = 8, kMaxSplits = 256;
+// at most kFewSplits: blocks of a wave each then fill the chip with less, and
+// each asks for all it may need at once (what its loads wait for is most of its
+// time: 3.0 us with the row's sequence looked up first, 2.1 so).
+constexpr int kFewSplits = 16, kMaxSplits = 256;
 template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void combine_kernel(AttendArgs a, AttendPlan plan, const float* part_o,
-                                                             const float2* part_ml) {
+__global__ __launch_bounds__(WAVES * 64) void combine_kernel(AttendArgs a, AttendPlan plan, Parts part) {
   constexpr int L4 = D / 4, G = WAVES * 64 / L4;
-  __shared__ float4 sO[G][L4];
+  constexpr int AHEAD = (kFewSplits + G - 1) / G;  // loads of a lane ahead of the weights
+  __shared__ floatx4 sO[G][L4];
   __shared__ float sF[kMaxSplits], sW[WAVES], sL[WAVES];
   const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const int seq = seq_of_row(a.r, row);
-  if (seq < 0) return;
-  const int len = min(a.r.length[seq], a.c.capacity());
-  const int chunk = chunk_of(len, plan.chunk, plan.splits);
-  if (len <= chunk) return;
-  const int n = (len + chunk - 1) / chunk;
-  const size_t at = ((size_t)row * a.q_heads + h) * plan.splits;
-  const float2 ml = tid < n ? part_ml[at + tid] : make_float2(-INFINITY, 0.f);
+  const size_t pair = (size_t)row * a.q_heads + h, at = pair * plan.splits;
+  const int g = tid / L4, l4 = tid - g * L4;
+  const floatx4* po = reinterpret_cast<const floatx4*>(part.o + at * D) + l4;
+  const int n = min(part.n[pair], plan.splits);  // (splits the row has)
+  const bool mine = row >= a.r.start[0] && row < a.r.start[a.r.seqs];
+  float2 ml = tid < plan.splits ? part.ml[at + tid] : make_float2(-INFINITY, 0.f);
+  floatx4 x[AHEAD];
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) x[u] = po[(size_t)min(g + u * G, plan.splits - 1) * L4];
+  if (!mine || n <= 1) return;  // nobody's row, or final already
+  if (tid >= n) ml = make_float2(-INFINITY, 0.f);
   float mm = ml.x;
 #pragma unroll
   for (int off = 32; off; off >>= 1) mm = fmaxf(mm, __shfl_xor(mm, off, kWave));
@@ -884,39 +903,35 @@ __global__ __launch_bounds__(WAVES * 64) void combine_kernel(AttendArgs a, Atten
   L = 0.f;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) L += sL[w];
-  const int g = tid / L4, l4 = tid - g * L4;
   if (g < G) {
-    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    floatx4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (g + u * G < n) O += sF[g + u * G] * x[u];
 #pragma unroll 4
-    for (int s = g; s < n; s += G) {
-      const float w = sF[s];
-      const float4 x = reinterpret_cast<const float4*>(part_o + (at + s) * D)[l4];
-      O.x += w * x.x; O.y += w * x.y; O.z += w * x.z; O.w += w * x.w;
-    }
+    for (int s = g + AHEAD * G; s < n; s += G) O += sF[s] * po[(size_t)s * L4];
     sO[g][l4] = O;
   }
   __syncthreads();
   if (tid >= L4) return;
-  float4 O = sO[0][tid];
+  floatx4 O = sO[0][tid];
 #pragma unroll
-  for (int w = 1; w < G; ++w) {
-    const float4 x = sO[w][tid];
-    O.x += x.x; O.y += x.y; O.z += x.z; O.w += x.w;
-  }
+  for (int w = 1; w < G; ++w) O += sO[w][tid];
   const float inv = 1.f / L;
   T* out = reinterpret_cast<T*>(a.out) + row * a.o_row + h * a.o_head + 4 * tid;
-  const float r[4] = {O.x, O.y, O.z, O.w};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(L == 0.f ? 0.f : r[e] * inv);
+  for (int e = 0; e < 4; ++e) out[e] = (T)(L == 0.f ? 0.f : O[e] * inv);
 }
 
 void attend_launched(hipError_t e);  // throws HipError (kv_ops.hip)
 
 template <typename T, int D>
 void launch_attend(const AttendArgs& a, const AttendPlan& plan, void* workspace, hipStream_t s) {
-  const size_t n = (size_t)a.r.rows * a.q_heads * plan.splits;
-  float* po = static_cast<float*>(workspace);
-  float2* pm = reinterpret_cast<float2*>(po + n * D);
+  const size_t pairs = (size_t)a.r.rows * a.q_heads, n = pairs * plan.splits;
+  Parts part;
+  part.o = static_cast<float*>(workspace);
+  part.ml = reinterpret_cast<float2*>(part.o + n * D);
+  part.n = reinterpret_cast<int32_t*>(part.ml + n);
   const int units = a.c.kv_heads * plan.splits;
   const dim3 grid = plan.by_xcd ? dim3(8 * ((units + 7) / 8) * plan.tiles) : dim3(plan.tiles, units);
   const dim3 block(kAttendThreads);
@@ -924,14 +939,14 @@ void launch_attend(const AttendArgs& a, const AttendPlan& plan, void* workspace,
   auto tiles = [&](auto big_page) {
     constexpr bool BIG = decltype(big_page)::value;
     if (plan.form == 1)
-      hipLaunchKernelGGL((attend_kernel<T, D, 1, BIG>), grid, block, 0, s, a, plan, po, pm);
+      hipLaunchKernelGGL((attend_kernel<T, D, 1, BIG>), grid, block, 0, s, a, plan, part);
     else if (plan.form == 2)
-      hipLaunchKernelGGL((attend_kernel<T, D, 2, BIG>), grid, block, 0, s, a, plan, po, pm);
+      hipLaunchKernelGGL((attend_kernel<T, D, 2, BIG>), grid, block, 0, s, a, plan, part);
     else if constexpr (D <= 128)
-      hipLaunchKernelGGL((attend_kernel<T, D, 4, BIG>), grid, block, 0, s, a, plan, po, pm);
+      hipLaunchKernelGGL((attend_kernel<T, D, 4, BIG>), grid, block, 0, s, a, plan, part);
   };
   if (plan.form == kWide) {
-    if constexpr (wide_dim(D)) hipLaunchKernelGGL((attend_wide_kernel<T, D>), grid, block, 0, s, a, plan, po, pm);
+    if constexpr (wide_dim(D)) hipLaunchKernelGGL((attend_wide_kernel<T, D>), grid, block, 0, s, a, plan, part);
   } else if (big) {
     tiles(std::true_type{});
   } else {
@@ -940,9 +955,9 @@ void launch_attend(const AttendArgs& a, const AttendPlan& plan, void* workspace,
   attend_launched(hipGetLastError());
   if (plan.splits == 1) return;
   if (plan.splits <= kFewSplits)
-    hipLaunchKernelGGL((combine_kernel<T, D, 1>), dim3(a.r.rows, a.q_heads), dim3(64), 0, s, a, plan, po, pm);
+    hipLaunchKernelGGL((combine_kernel<T, D, 1>), dim3(a.r.rows, a.q_heads), dim3(64), 0, s, a, plan, part);
   else
-    hipLaunchKernelGGL((combine_kernel<T, D, 4>), dim3(a.r.rows, a.q_heads), dim3(256), 0, s, a, plan, po, pm);
+    hipLaunchKernelGGL((combine_kernel<T, D, 4>), dim3(a.r.rows, a.q_heads), dim3(256), 0, s, a, plan, part);
   attend_launched(hipGetLastError());
 }
 

@@ -216,9 +216,9 @@ AttendPlan attend_plan(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint
   p.tiles = (int)std::min(by_fill, by_row);
   const uint64_t blocks = (uint64_t)p.tiles * c.kv_heads, wanted = p.form == kWide ? wide_wanted(D, f32) : kBlocksWanted;
   const uint64_t len = std::max<uint64_t>(1, std::min<uint64_t>(r.max_length, (uint64_t)c.table_stride * c.page_rows));
-  const uint64_t most = std::min<uint64_t>((len + kChunkStep - 1) / kChunkStep, kMostSplits);
+  const uint64_t step = chunk_step(f32), most = std::min<uint64_t>((len + step - 1) / step, kMostSplits);
   const uint64_t splits = std::min<uint64_t>(most, (wanted + blocks - 1) / blocks);
-  p.chunk = (int)(((len + splits - 1) / splits + kChunkStep - 1) / kChunkStep * kChunkStep);
+  p.chunk = (int)(((len + splits - 1) / splits + step - 1) / step * step);
   p.splits = (int)((len + p.chunk - 1) / p.chunk);
   const uint64_t units = (uint64_t)c.kv_heads * p.splits;
   p.by_xcd = p.form == kWide && (units % 8 == 0 || units >= 32);
@@ -307,7 +307,7 @@ uint64_t kv_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows
     return 0;
   const AttendPlan plan = attend_plan(c, r, q_heads);
   if (plan.splits == 1) return 0;
-  return (uint64_t)r.rows * q_heads * plan.splits * (c.head_dim + 2) * sizeof(float);
+  return (uint64_t)r.rows * q_heads * (plan.splits * (uint64_t)(c.head_dim + 2) + 1) * sizeof(float);
 }
 
 void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, hipStream_t s) {
