@@ -207,6 +207,55 @@ def test_attention_of_trees(mit2, ctx, dtype, dim, heads):
     _check_attention(ctx, mit2, b, mask=ops_ref.trees(b, dim)[0])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("page", [1, 4, 8, 16, 64, 256])
+@pytest.mark.parametrize("dim,heads,new", [(64, (4, 2), [14]), (128, (4, 2), [30, 29]), (64, (2, 2), [100, 81]), (128, (8, 2), [65, 40, 90]),
+                                           (256, (2, 1), [70])])
+def test_attention_of_many_rows_over_pages(mit2, ctx, dtype, page, dim, heads, new):
+    """Each form of the tiles (28, 60, 90 and 260 query rows on average, large heads), pages smaller and larger than a tile."""
+    b = Batch(new, [n + (130, 7, 300)[s] for s, n in enumerate(new)], page=page, q_heads=heads[0], kv_heads=heads[1], dim=dim, dtype=dtype,
+              seed=page + dim, lead_rows=3, tail_rows=1)
+    _check_attention(ctx, mit2, b)
+    _check_attention(ctx, mit2, b, mask=ops_ref.trees(b, page)[0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_many_rows_with_missing_pages_and_splits(mit2, ctx, dtype, dim):
+    b = Batch([150, 3, 200], [2900, 3, 1500], page=32, q_heads=2, kv_heads=1, dim=dim, dtype=dtype, seed=dim)
+    b.table[0, 5], b.table[0, 60], b.table[2, 0], b.table[2, 46] = -1, b.pages, -7, 2 ** 31 - 1
+    _check_attention(ctx, mit2, b)
+    _check_attention(ctx, mit2, b, mask=ops_ref.trees(b, 1)[0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,tree", [(64, (2, 2), True), (128, (8, 2), True), (64, (2, 2), False), (128, (4, 1), False), (96, (4, 1), False)])
+def test_many_rows_are_blind_to_what_they_do_not_see(mit2, ctx, dtype, dim, heads, tree):
+    """The same for tiles of many rows: NaN and infinities among the new rows and behind the sequences' ends."""
+    b = Batch([100, 70], [230, 75], page=16, q_heads=heads[0], kv_heads=heads[1], dim=dim, dtype=dtype, seed=22)
+    mask = ops_ref.trees(b, 9)[0] if tree else None
+    clean = On(mit2, b).attend(ctx, mask=mask)
+    used = np.zeros((b.pages, b.page), bool)
+    for s, n in enumerate(b.length):
+        for j in range(n):
+            used[b.page_of(s, j), j % b.page] = True
+    for cache in (b.k, b.v):
+        cache.permute(0, 2, 1, 3)[torch.from_numpy(~used)] = math.nan
+    assert torch.equal(On(mit2, b).attend(ctx, mask=mask), clean)
+    sees = torch.zeros(b.rows, 2, dtype=torch.bool)  # row sees the NaN, the infinity
+    for which, (s, i, value) in enumerate(((0, 61, math.nan), (1, 20, -math.inf))):
+        j = b.length[s] - b.new[s] + i
+        b.v[b.page_of(s, j), :, j % b.page, 5] = value
+        for row, s2, i2, _ in b.each_row():
+            sees[row, which] = s2 == s and bool(i2 >= i if mask is None else mask[row, i // 32] >> np.uint32(i % 32) & 1)
+    got = On(mit2, b).attend(ctx, mask=mask)
+    hit = sees.any(1)
+    assert torch.equal(got[~hit], clean[~hit])
+    assert bool(torch.isnan(got[sees[:, 0]][:, :, 5]).all()) and bool((got[sees[:, 1]][:, :, 5] == -math.inf).all())
+    rest = [d for d in range(dim) if d != 5]
+    assert torch.equal(got[hit][:, :, rest], clean[hit][:, :, rest])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attention_of_a_mask_of_too_few_words(mit2, ctx, dtype):
     """New rows past the mask's words are seen by none."""
