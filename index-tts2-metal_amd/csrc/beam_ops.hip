@@ -151,8 +151,9 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
   bool any = false;
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) any |= at + i * kSelectThreads * W + W > from && at + i * kSelectThreads * W < to;
-  // (a 16-bit type's values differ in their upper bits alone)
-  constexpr int LOW = sizeof(T) == 4 ? 0 : std::is_same<T, half_t>::value ? 13 : 16;
+  // (a 16-bit type's values differ in their upper bits alone; bf16's and FLT_MAX,
+  // which stands for +inf, in bit 15 too)
+  constexpr int LOW = sizeof(T) == 4 ? 0 : std::is_same<T, half_t>::value ? 13 : 15;
   const uint32_t key = any ? float_key(top) : 0u, high = key >> LOW, t32 = reached_by<32 - LOW>(high, a.count);
   uint64_t kth = (uint64_t)(t32 << LOW) << 32;
   const int over = __popcll(__ballot(high > t32)), ties = __popcll(__ballot(high == t32));

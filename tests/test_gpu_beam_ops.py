@@ -117,6 +117,17 @@ def test_select_of_masked_and_odd_logits(mit2, ctx):
     _check_select(mit2, ctx, x, np.zeros((1, 2)), 10, dtype="f16")
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_select_orders_infinities_before_the_largest_finite(mit2, ctx, dtype):
+    """Many logits at the type's largest finite value, a few at +inf (which counts as fp32's largest): those come first."""
+    x = torch.full((1, 2, 900), torch.finfo(TORCH[dtype]).max)
+    x[0, 0, ::64] = math.inf
+    x[0, 1, [3, 500, 777]] = math.inf
+    x[0, 1, 100:400] = 0.0
+    for count in (2, 5, 20, 64):
+        _check_select(mit2, ctx, x, np.zeros((1, 2)), count, dtype=dtype)
+
+
 def test_select_row_stride_and_large_values(mit2, ctx):
     g = torch.Generator().manual_seed(3)
     x = torch.randn(2, 3, 333, generator=g) * 1000 + 50000
