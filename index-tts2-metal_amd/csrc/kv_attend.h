@@ -274,7 +274,13 @@ __device__ __forceinline__ bool sees(const AttendArgs& a, const Query& x, int j,
 // vote): up to there the probabilities, at most 2^kSlack, stay exact in fp32 sums
 // and in range as 16-bit operands, where they round to the type, as the product
 // needs; the sum of the weights keeps fp32.
+//
+// f16's weights are 2^7 times theirs throughout, the sum's too: with the slack up to
+// 2^15, in range, and normal down to 2^-21 of the largest.  (As they were, many
+// keys that are light beside one, e^-18 of it, added up to nothing.)
 constexpr float kSlack = 8.f;
+template <typename T>
+constexpr float kLift = std::is_same<T, half_t>::value ? 7.f : 0.f;
 
 template <typename T, int D>
 struct Running {
@@ -303,10 +309,10 @@ struct Running {
 #pragma unroll
       for (int d = 0; d < S::DP; ++d) o[d] *= alpha;
     }
-    const float base = mx == -INFINITY ? 0.f : mx;
+    const float base = mx == -INFINITY ? 0.f : kLift<T> - mx;
 #pragma unroll
     for (int e = 0; e < S::NV; ++e) {
-      s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -base));
+      s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, base));
       l += s[e];
     }
   }

@@ -326,6 +326,28 @@ def test_attention_of_large_and_equal_scores(mit2, ctx, dtype):
     _check_attention(ctx, mit2, b, scale=-0.25)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 20, 130])
+@pytest.mark.parametrize("light", [13.4, 17.9])
+def test_attention_of_many_light_keys(mit2, ctx, dtype, new, light):
+    """One heavy key in 32, with values of 0, beside keys whose weights are e^-light of it: what they add up to is all there is."""
+    b = Batch([new], [1500], dim=64, dtype=dtype, seed=31)
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    for j in range(1500):
+        page, slot = b.page_of(0, j), j % b.page
+        b.k[page, :, slot, 0] = 0.0 if j % 32 == 0 else -light
+        b.v[page, :, slot] = 0.0 if j % 32 == 0 else b.v[page, :, slot].abs() * 16 + 16
+    on = On(mit2, b)
+    got = on.attend(ctx, scale=1.0)
+    ref, tol = ops_ref.attention64(b, 1.0)
+    if dtype == "f16":
+        # weights are taken at 2^7 times their size: below the type's smallest normal each is off by at most half its step, 2^-25, of that; 31
+        # of them to a weight of 1.  A result below the smallest normal is rounded by as much.
+        tol = tol + 31 * 2.0 ** -32 * float(b.v.abs().max()) + 2.0 ** -25
+    _check(got[_mine(b)], ref[_mine(b)], tol[_mine(b)], f"light keys {dtype} {new} {light}")
+
+
 def test_attention_strides(mit2, ctx):
     """Queries in a projection's rows at an odd stride, outputs head by head."""
     b = Batch([1, 12, 33], [60, 70, 200], q_heads=4, kv_heads=2, dim=64, dtype="f16", seed=12)
