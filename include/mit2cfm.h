@@ -563,7 +563,7 @@ typedef struct mit2cfm_kv_cache {
   uint32_t page_rows;    /* a power of two, 1 .. 1024 */
   uint32_t kv_heads;     /* 1 .. 1024 */
   uint32_t head_dim;     /* 32, 64, 96, 128, 192 or 256 */
-  uint32_t table_stride; /* entries of a table row; page_rows * table_stride < 2^31 */
+  uint32_t table_stride; /* entries of a table row; page_rows * table_stride <= 2^30 */
   int32_t dtype;         /* MIT2CFM_DTYPE_F32, _F16 or _BF16: of the cache and of every row given with it */
 } mit2cfm_kv_cache;
 
@@ -618,7 +618,7 @@ typedef struct mit2cfm_kv_attention {
   const void* q; /* [rows][q_heads][head_dim] by q_row, q_head */
   void* out;     /* the same by out_row, out_head; no overlap with q */
   uint64_t q_row, q_head, out_row, out_head;
-  uint32_t q_heads; /* a multiple of kv_heads, <= 4096 */
+  uint32_t q_heads; /* a multiple of kv_heads, <= 4096; rows * q_heads <= 2^28 */
   float scale;      /* finite */
   const uint32_t* mask;
   uint32_t mask_words; /* words of a mask row: new rows from 32 * mask_words on are seen by none */
@@ -645,7 +645,7 @@ mit2cfm_status mit2cfm_kv_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_ca
  * count as -inf).  Candidates of -inf fill the list when others run out.
  * count = beams keeps a search going; 2 * beams leaves as many after stop
  * tokens are taken out.  Sums are fp64 of fp32 terms, candidates compared in
- * fp64. */
+ * fp64 (where one beam's agree there, those of the larger logits are taken). */
 typedef struct mit2cfm_beam_select {
   const void* logits; /* [groups * beams][vocab], rows logits_row elements apart */
   uint64_t logits_row;
@@ -660,7 +660,8 @@ typedef struct mit2cfm_beam_select {
   float* scores_out;        /* [groups][count]; no overlap with scores */
   int32_t* parent_out;      /* the beam it continues, 0 .. beams - 1 */
   int32_t* token_out;
-  int32_t* finished_out;    /* the parent was finished, or the token is the stop token; may be NULL */
+  int32_t* finished_out;    /* the parent was finished, or the token is the stop token; may be NULL; no
+                             * overlap with finished */
   void* workspace;          /* 16-byte aligned, of mit2cfm_beam_select_workspace bytes; calls that may
                              * run at the same time need one each */
   uint64_t workspace_bytes;

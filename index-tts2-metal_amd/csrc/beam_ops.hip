@@ -488,6 +488,11 @@ void beam_select(const mit2cfm_beam_select& p, hipStream_t s) {
   need(p.logits && p.scores && p.scores_out && p.parent_out && p.token_out,
        "logits, scores, scores_out, parent_out and token_out must not be NULL");
   need(aligned(p.logits, (size_t)kv_elem_bytes(p.dtype)), "logits must be aligned to its type");
+  need(p.scores_out != p.scores && (!p.finished || p.finished_out != p.finished),
+       "scores_out must not be scores, nor finished_out finished");
+  need(aligned(p.scores, 4) && aligned(p.finished, 4) && aligned(p.scores_out, 4) && aligned(p.parent_out, 4) &&
+           aligned(p.token_out, 4) && aligned(p.finished_out, 4),
+       "scores, finished and the outputs must be 4-byte aligned");
   need(p.workspace && p.workspace_bytes >= beam_select_workspace(p), "workspace is NULL or too small");
   need(aligned(p.workspace, 16), "workspace must be 16-byte aligned");
   SelectArgs a;
@@ -534,6 +539,9 @@ void beam_reorder(const mit2cfm_kv_cache& c, const mit2cfm_beam_reorder& p, hipS
   need(p.state == nullptr || (p.state_out && p.state_out != p.state && p.state_words >= 1 && p.state_words < (1u << 31)),
        "state needs a state_out of its own and state_words in [1, 2^31)");
   need(p.token == nullptr || (p.state && p.place), "token needs state and place");
+  need(aligned(p.parent, 4) && aligned(p.length, 4) && aligned(p.table_out, 4) && aligned(p.state, 4) &&
+           aligned(p.state_out, 4) && aligned(p.token, 4) && aligned(p.place, 4),
+       "parent, length, table_out, the states, token and place must be 4-byte aligned");
   ReorderArgs a;
   a.k = static_cast<char*>(c.k);
   a.v = static_cast<char*>(c.v);

@@ -229,6 +229,12 @@ void check_rows(const mit2cfm_kv_rows& r) {
   need(r.seqs <= 65535, "seqs must be <= 65535");
   need(r.rows < (1u << 24), "rows must be below 2^24");
   need(r.seqs == 0 || r.rows == 0 || (r.start && r.length), "start and length must not be NULL");
+  need(aligned(r.start, 4) && aligned(r.length, 4), "start and length must be 4-byte aligned");
+}
+
+// What attend_plan's numbers, and the kernels' 32-bit ones of query rows, are made for.
+bool attention_in_range(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
+  return q_heads >= 1 && q_heads <= 4096 && q_heads % c.kv_heads == 0 && (uint64_t)r.rows * q_heads <= (1u << 28);
 }
 
 // An output's rows and heads must not lie on one another.
@@ -242,7 +248,8 @@ void attend_launched(hipError_t e) { launched(e); }
 
 int kv_elem_bytes(int32_t dtype) { return dtype == MIT2CFM_DTYPE_F32 ? 4 : 2; }
 
-void check_kv_cache(const mit2cfm_kv_cache& c) {
+namespace {
+void check_kv_sizes(const mit2cfm_kv_cache& c) {
   need(c.dtype >= MIT2CFM_DTYPE_F32 && c.dtype <= MIT2CFM_DTYPE_BF16, "the cache's dtype must be f32, f16 or bf16");
   need(c.page_rows >= 1 && c.page_rows <= 1024 && (c.page_rows & (c.page_rows - 1)) == 0,
        "page_rows must be a power of two in [1, 1024]");
@@ -251,10 +258,16 @@ void check_kv_cache(const mit2cfm_kv_cache& c) {
            c.head_dim == 256,
        "head_dim must be 32, 64, 96, 128, 192 or 256");
   need(c.pages >= 1 && c.pages < (1u << 31), "pages must be in [1, 2^31)");
-  need(c.table_stride >= 1 && (uint64_t)c.table_stride * c.page_rows < (1ull << 31),
-       "table_stride must be >= 1, page_rows * table_stride below 2^31");
+  need(c.table_stride >= 1 && (uint64_t)c.table_stride * c.page_rows <= (1u << 30),
+       "table_stride must be >= 1, page_rows * table_stride <= 2^30");
+}
+}  // namespace
+
+void check_kv_cache(const mit2cfm_kv_cache& c) {
+  check_kv_sizes(c);
   need(c.k && c.v && c.table, "the cache's k, v and table must not be NULL");
-  need(aligned(c.k, 16) && aligned(c.v, 16), "the cache's k and v must be 16-byte aligned");
+  need(aligned(c.k, 16) && aligned(c.v, 16) && aligned(c.table, 4),
+       "the cache's k and v must be 16-byte aligned, its table 4-byte aligned");
 }
 
 void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_append& p, hipStream_t s) {
@@ -270,6 +283,7 @@ void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cf
   const size_t e = (size_t)kv_elem_bytes(c.dtype);
   need(aligned(p.k, e) && aligned(p.v, e) && aligned(p.q, e) && aligned(p.q_out, e),
        "k, v, q and q_out must be aligned to their type");
+  need(aligned(p.position, 4), "position must be 4-byte aligned");
   if (with_q) {
     check_out(p.q_out_row, p.q_out_head, r.rows, p.q_heads, c.head_dim, "q_out's rows and heads overlap");
     need(p.q != p.q_out || (p.q_row == p.q_out_row && p.q_head == p.q_out_head),
@@ -301,10 +315,13 @@ void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cf
 }
 
 uint64_t kv_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
-  if (c.kv_heads < 1 || c.kv_heads > 1024 || c.head_dim < 32 || c.head_dim > 256 || c.page_rows < 1 || c.table_stride < 1 ||
-      q_heads < 1 || q_heads > 4096 || q_heads % c.kv_heads || r.seqs < 1 || r.seqs > 65535 || r.rows < 1 ||
-      r.rows >= (1u << 24))
+  try {
+    check_kv_sizes(c);
+    check_rows(r);
+  } catch (const std::invalid_argument&) {
     return 0;
+  }
+  if (r.seqs == 0 || r.rows == 0 || !attention_in_range(c, r, q_heads)) return 0;
   const AttendPlan plan = attend_plan(c, r, q_heads);
   if (plan.splits == 1) return 0;
   return (uint64_t)r.rows * q_heads * (plan.splits * (uint64_t)(c.head_dim + 2) + 1) * sizeof(float);
@@ -313,13 +330,14 @@ uint64_t kv_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows
 void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, hipStream_t s) {
   check_kv_cache(c);
   check_rows(r);
-  need(p.q_heads >= 1 && p.q_heads <= 4096 && p.q_heads % c.kv_heads == 0,
-       "q_heads must be a multiple of kv_heads, <= 4096");
+  need(attention_in_range(c, r, p.q_heads),
+       "q_heads must be a multiple of kv_heads, <= 4096, rows * q_heads <= 2^28");
   need(std::isfinite(p.scale), "scale must be finite");
   need(p.mask == nullptr || p.mask_words >= 1, "mask_words must be >= 1 with a mask");
   need(p.mask_words < (1u << 24), "mask_words must be below 2^24");
+  need(aligned(p.mask, 4), "mask must be 4-byte aligned");
   if (r.seqs == 0 || r.rows == 0) return;
-  need(p.q && p.out, "q and out must not be NULL");
+  need(p.q && p.out && p.q != p.out, "q and out must not be NULL, nor the same");
   const size_t e = (size_t)kv_elem_bytes(c.dtype);
   need(aligned(p.q, e) && aligned(p.out, e), "q and out must be aligned to their type");
   check_out(p.out_row, p.out_head, r.rows, p.q_heads, c.head_dim, "out's rows and heads overlap");
