@@ -119,9 +119,16 @@ void Arena::reserve(size_t bytes) {
     HIP_OK(hipFree(base_));
     base_ = nullptr;
   }
+  cap_ = used_ = 0;
+  if (bytes) {
+    const hipError_t e = hipMalloc(reinterpret_cast<void**>(&base_), bytes);
+    if (e != hipSuccess) {
+      base_ = nullptr;
+      (void)hipGetLastError();  // (or the next launch's check would report it)
+      HIP_OK(e);
+    }
+  }
   cap_ = bytes;
-  used_ = 0;
-  if (bytes) HIP_OK(hipMalloc(reinterpret_cast<void**>(&base_), bytes));
 }
 
 void* Arena::take(size_t bytes) {

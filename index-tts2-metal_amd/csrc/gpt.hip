@@ -1423,6 +1423,7 @@ struct GptDecoder::Impl {
   void ensure(int kv_rows, int prefix_rows, int steps) {
     if (kv_rows <= cap && prefix_rows <= rows_cap && steps <= pred_cap && st) return;
     drop_graphs();
+    const int was[] = {cap, rows_cap, pred_cap, chunk_cap};
     cap = std::max(std::max(kv_rows, cap), 256);
     cap = (cap + kChunk - 1) / kChunk * kChunk;
     rows_cap = std::max(std::max(prefix_rows, rows_cap), 16);
@@ -1439,7 +1440,13 @@ struct GptDecoder::Impl {
                    align256((size_t)GptDecoder::kMaxHistory * 4) + align256(sizeof(TokenMail)) +
                    align256(kTokWG * 4) +
                    align256((size_t)2 * L * chunk_cap * 4);
-    ws.reserve(bytes);
+    st = nullptr;  // (nothing is held should this fail)
+    try {
+      ws.reserve(bytes);
+    } catch (...) {
+      cap = was[0]; rows_cap = was[1]; pred_cap = was[2]; chunk_cap = was[3];
+      throw;
+    }
     st = static_cast<GptState*>(ws.take(sizeof(GptState)));
     predicted = static_cast<uint32_t*>(ws.take((size_t)pred_cap * 4));
     inputs = static_cast<uint32_t*>(ws.take(((size_t)pred_cap + 1) * 4));
@@ -1732,6 +1739,7 @@ struct GptDecoder::Impl {
   }
 
   void ensure_beams(int n, int rows, int steps) {
+    const int was[] = {beam_cap[0], beam_cap[1], beam_cap[2]};
     beam_cap[0] = std::max(n, beam_cap[0]);
     beam_cap[1] = std::max(rows, beam_cap[1]);
     beam_cap[2] = std::max(steps, beam_cap[2]);
@@ -1762,7 +1770,13 @@ struct GptDecoder::Impl {
                             battend_bytes, bselect_bytes};
     size_t total = 0;
     for (size_t b : sizes) total += align256(std::max<size_t>(b, 16));
-    bw.reserve(total);
+    bst = nullptr;  // (nothing is held should this fail)
+    try {
+      bw.reserve(total);
+    } catch (...) {
+      std::copy(was, was + 3, beam_cap);
+      throw;
+    }
     int i = 0;
     auto take = [&](auto*& p) { p = static_cast<std::remove_reference_t<decltype(p)>>(bw.take(std::max<size_t>(sizes[i++], 16))); };
     take(bst); take(brow); take(bk); take(bv); take(bx); take(bq); take(batt); take(bfc); take(blogits); take(new_k);

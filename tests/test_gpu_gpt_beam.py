@@ -1,5 +1,5 @@
 """Beam search of mel codes (mit2cfm_gpt_kv_beam), which runs on the paged-cache and beam operators, against a plain search over the
-CPU oracle's single-row decode; one beam against the greedy decode; and the operators' calls put together by hand."""
+CPU oracle's single-row decode; one beam against the greedy decode; and calls of other sizes, or too large, in between."""
 from __future__ import annotations
 
 import math
@@ -110,6 +110,25 @@ def test_calls_of_changing_sizes_and_beside_greedy(ctx2):
     assert [h.tolist() for h in again["predicted"]] == [h.tolist() for h in first["predicted"]]
     assert again["scores"].tolist() == first["scores"].tolist()
     assert ctx2.gpt_kv_greedy(prefix, 12)["predicted"].tolist() == greedy["predicted"].tolist()
+
+
+def test_a_search_that_does_not_fit_leaves_the_context_usable(mit2, ctx2):
+    """With little GPU memory left, a long prefix's pages cannot be had: an error of the call; the next searches are as before."""
+    torch = pytest.importorskip("torch")
+    prefix = _prefix(40, 8)
+    first = ctx2.gpt_kv_beam(prefix, 6, 3)
+    free, _ = torch.cuda.mem_get_info()
+    held = torch.empty(max(free - (3 << 30), 0), dtype=torch.uint8, device="cuda:0")
+    try:
+        with pytest.raises(mit2.Mit2CfmError) as e:
+            ctx2.gpt_kv_beam(np.zeros((30000, 1280), np.float32), 6, 8)  # (its pages: 5 GB)
+        assert e.value.status == mit2.E_HIP
+        again = ctx2.gpt_kv_beam(prefix, 6, 3)
+    finally:
+        del held
+        torch.cuda.empty_cache()
+    assert [h.tolist() for h in again["predicted"]] == [h.tolist() for h in first["predicted"]]
+    assert again["scores"].tolist() == first["scores"].tolist()
 
 
 def test_refusals(mit2, ctx2, tensors):
