@@ -1,6 +1,6 @@
 """The beam operators (mit2cfm_beam_select_device, mit2cfm_beam_reorder_device) on the GPU against plain restatements
 (ops_ref.py): ties, beams that do not exist yet or are finished, rows without a finite logit, bad parents and pages,
-part pages, and a small search run with all four operators."""
+part pages, and a small search run with all four operators, eager and as a graph."""
 from __future__ import annotations
 
 import math
@@ -220,3 +220,152 @@ def test_reorder_takes_a_longer_selection(mit2, ctx):
     c["token"] = rng.integers(0, 9000, (3, 8)).astype(np.int32)
     length = np.array([3, 9, 20], np.int32)
     _same(_reorder(mit2, ctx, parent=parent, length=length, **c), ops_ref.reorder(parent=parent, length=length, **c))
+
+
+# ------------------------------------------------------------------ together
+class Search:
+    """A search over a toy model: a token's query, keys and values are rows of tables, and the attention's output is its logits.  Layer 1 of the
+    cache takes keys and values the other way round and is read at the end alone."""
+    GROUPS, BEAMS, HEADS, DIM, VOCAB, PAGE, ENTRIES, STEPS, START, STOP = 2, 3, 2, 32, 60, 4, 6, 10, 7, 11
+    PREFIX = (5, 8)
+
+    def __init__(self, mit2, ctx):
+        self.mit2, self.ctx = mit2, ctx
+        g = torch.Generator().manual_seed(41)
+        n, d = self.GROUPS * self.BEAMS, self.DIM
+        self.emb = [torch.randn(self.VOCAB, h * d, generator=g) * f for h, f in ((self.HEADS, 2.0), (1, 1.0), (1, 3.0))]  # q, k, v
+        self.prefix = [[torch.randn(p, d, generator=g) for _ in range(2)] for p in self.PREFIX]
+        self.pages = n * self.ENTRIES
+        z = dict(device=DEV)
+        self.tables = [e.to(DEV) for e in self.emb]
+        self.q, self.k, self.v = (torch.zeros(n, h * d, **z) for h in (self.HEADS, 1, 1))
+        self.qr, self.logits = torch.zeros(n, self.HEADS * d, **z), torch.zeros(n, self.HEADS * d, **z)
+        self.cache_k, self.cache_v = (torch.zeros(2, self.pages, 1, self.PAGE, d, **z) for _ in range(2))
+        ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32, **z)  # noqa: E731
+        self.start = torch.arange(n + 1, dtype=torch.int32, **z)
+        self.length, self.glength, self.place = ints(n), ints(self.GROUPS), ints(self.GROUPS)
+        self.token, self.parent = ints(n), ints(n)
+        self.score, self.done = [torch.zeros(n, **z) for _ in range(2)], [ints(n) for _ in range(2)]
+        self.table, self.hist = [ints(n, self.ENTRIES) for _ in range(2)], [ints(n, self.STEPS) for _ in range(2)]
+        self.ws = torch.zeros(1 << 20, dtype=torch.uint8, **z)
+        self.stream = torch.cuda.ExternalStream(ctx.stream)
+
+    def cache(self, layer, side):
+        return self.mit2.KvCache(k=self.cache_k[layer].data_ptr(), v=self.cache_v[layer].data_ptr(), table=self.table[side].data_ptr(),
+                                 pages=self.pages, page_rows=self.PAGE, kv_heads=1, head_dim=self.DIM, table_stride=self.ENTRIES,
+                                 dtype=self.mit2.DTYPE_F32)
+
+    def append(self, layer, side, rows, k, v, rot, **q):
+        self.ctx.kv_append_device(self.cache(layer, side), rows, self.mit2.KvAppend(
+            k=k.data_ptr(), v=v.data_ptr(), k_row=self.DIM, k_head=self.DIM, v_row=self.DIM, v_head=self.DIM, rotary_dim=rot, theta=10000.0, **q))
+
+    def move(self, side, state=True):
+        h = self.hist
+        self.ctx.beam_reorder_device(self.cache(0, side), self.mit2.BeamReorder(
+            groups=self.GROUPS, beams=self.BEAMS, layers=2, layer_stride=self.cache_k[0].numel(), parent=self.parent.data_ptr(),
+            parent_stride=self.BEAMS, length=self.glength.data_ptr(), table_out=self.table[1 - side].data_ptr(),
+            state=h[side].data_ptr() if state else None, state_out=h[1 - side].data_ptr() if state else None, state_words=self.STEPS,
+            token=self.token.data_ptr() if state else None, place=self.place.data_ptr()))
+
+    def begin(self):
+        """Every group's prefix in its first beam's pages, the other beams its children."""
+        with torch.cuda.stream(self.stream):
+            for t in (self.cache_k, self.cache_v, *self.hist, *self.done, self.parent, self.place):
+                t.zero_()
+            self.table[1].copy_(torch.arange(self.pages, dtype=torch.int32).view(-1, self.ENTRIES))
+            self.score[0].fill_(-math.inf)
+            self.score[0][:: self.BEAMS] = 0.0
+            self.token.fill_(self.START)
+            self.glength.copy_(torch.tensor(self.PREFIX, dtype=torch.int32))
+            self.length.copy_(torch.tensor(self.PREFIX, dtype=torch.int32).repeat_interleave(self.BEAMS))
+            bounds = [torch.tensor([0, p], dtype=torch.int32, device=DEV) for p in self.PREFIX]
+            kv = [[t.to(DEV) for t in pair] for pair in self.prefix]
+            self.stream.synchronize()
+            for grp, p in enumerate(self.PREFIX):
+                rows = self.mit2.KvRows(start=bounds[grp].data_ptr(), length=self.glength[grp:].data_ptr(), seqs=1, rows=p, max_length=p)
+                whole, self.table[1] = self.table[1], self.table[1][grp * self.BEAMS:]
+                self.append(0, 1, rows, *kv[grp], self.DIM)
+                self.append(1, 1, rows, *kv[grp][::-1], 0)
+                self.table[1] = whole
+            self.move(1, state=False)
+            self.stream.synchronize()
+
+    def step(self, side):
+        m, n, d = self.mit2, self.GROUPS * self.BEAMS, self.DIM
+        with torch.cuda.stream(self.stream):
+            self.length.add_(1)
+            self.glength.add_(1)
+            for t, to in zip(self.tables, (self.q, self.k, self.v)):
+                torch.index_select(t, 0, self.token, out=to)
+            rows = m.KvRows(start=self.start.data_ptr(), length=self.length.data_ptr(), seqs=n, rows=n, max_length=self.PAGE * self.ENTRIES)
+            wide = dict(q_row=self.HEADS * d, q_head=d, q_heads=self.HEADS)
+            self.append(0, side, rows, self.k, self.v, d, q=self.q.data_ptr(), q_out=self.qr.data_ptr(), q_out_row=self.HEADS * d, q_out_head=d, **wide)
+            self.append(1, side, rows, self.v, self.k, 0)
+            self.ctx.kv_attention_device(self.cache(0, side), rows, m.KvAttention(
+                q=self.qr.data_ptr(), out=self.logits.data_ptr(), out_row=self.HEADS * d, out_head=d, scale=d ** -0.5,
+                workspace=self.ws.data_ptr(), workspace_bytes=self.ws.numel(), **wide))
+            self.ctx.beam_select_device(m.BeamSelect(
+                logits=self.logits.data_ptr(), logits_row=self.HEADS * d, dtype=m.DTYPE_F32, groups=self.GROUPS, beams=self.BEAMS, vocab=self.VOCAB,
+                count=self.BEAMS, scores=self.score[side].data_ptr(), finished=self.done[side].data_ptr(), stop_token=self.STOP,
+                scores_out=self.score[1 - side].data_ptr(), parent_out=self.parent.data_ptr(), token_out=self.token.data_ptr(),
+                finished_out=self.done[1 - side].data_ptr(), workspace=self.ws.data_ptr(), workspace_bytes=self.ws.numel()))
+            self.move(side)
+            self.place.add_(1)
+
+    def result(self):
+        self.stream.synchronize()
+        return self.hist[0].cpu().clone(), self.score[0].cpu().clone(), self.cache_k.cpu().clone(), self.cache_v.cpu().clone(), self.table[0].cpu().clone()
+
+
+def test_a_search_of_all_four_operators(mit2, ctx):
+    """Every hypothesis' score is that of its own history, recomputed in 64 bits from nothing but the history, and both layers' caches hold it;
+    replays of the steps as a graph, with the search begun anew in between, give the same bits."""
+    from test_gpu_kv_ops import Graph
+    s = Search(mit2, ctx)
+    s.begin()
+    for i in range(s.STEPS):
+        s.step(i & 1)
+    first = s.result()
+    hist, score, ck, cv, table = first
+    q_emb, k_emb, v_emb = (e.double() for e in s.emb)
+    for r in range(s.GROUPS * s.BEAMS):
+        grp, told = r // s.BEAMS, hist[r].tolist()
+        P, total = s.PREFIX[grp], 0.0
+        inputs = [s.START] + told[:-1]
+        keys = [ops_ref.rotate64(x.view(1, -1), i, s.DIM, False, 10000.0)[0] for i, x in enumerate(s.prefix[grp][0])]
+        vals = list(s.prefix[grp][1].double())
+        for i, (x, t) in enumerate(zip(inputs, told)):
+            keys.append(ops_ref.rotate64(k_emb[x].view(1, -1), P + i, s.DIM, False, 10000.0)[0])
+            vals.append(v_emb[x])
+            if s.STOP in told[:i]:
+                assert t == s.STOP
+                continue
+            q = ops_ref.rotate64(q_emb[x].view(s.HEADS, -1), P + i, s.DIM, False, 10000.0)
+            out = torch.softmax(q @ torch.stack(keys).t() * s.DIM ** -0.5, -1) @ torch.stack(vals)
+            total += float(torch.log_softmax(out.reshape(-1)[: s.VOCAB], -1)[t])
+        # a score of the attention is off by 8 fp32 half steps of sum |q k| (the turns' and the sums'), at most about 2 * 32 * 2 * scale = 23 here; an
+        # output by twice that of values up to 12; a log probability by twice that, a step
+        assert abs(total - float(score[r])) <= s.STEPS * 2 * 12 * 2 * 8 * 23 * U, (r, total, float(score[r]))
+        for j in range(P + s.STEPS):
+            page, slot = int(table[r, j // s.PAGE]), j % s.PAGE
+            x = s.prefix[grp] if j < P else None
+            k1, v1 = (x[1][j], x[0][j]) if j < P else (s.emb[2][inputs[j - P]], s.emb[1][inputs[j - P]])
+            assert torch.equal(ck[1, page, 0, slot], k1) and torch.equal(cv[1, page, 0, slot], v1), (r, j)
+            assert (ck[0, page, 0, slot].double() - keys[j]).abs().max() <= 8 * U * 5 and torch.equal(cv[0, page, 0, slot].double(), vals[j])
+    assert len({tuple(h) for h in hist[: s.BEAMS].tolist()}) == s.BEAMS
+
+    def pair():
+        s.step(0)
+        s.step(1)
+
+    torch.cuda.synchronize()
+    g = Graph(ctx, pair)
+    try:
+        for _ in range(3):
+            s.begin()
+            for _ in range(s.STEPS // 2):
+                g.replay()
+            for a, b in zip(first, s.result()):
+                assert torch.equal(a, b)
+    finally:
+        g.close()
