@@ -47,6 +47,7 @@ struct SelectArgs {
 constexpr int kSelectThreads = 256, kSelectWaves = kSelectThreads / 64;
 constexpr int kPerThread = 16;  // logits of a thread
 constexpr int kMaxChunk = kSelectThreads * kPerThread;
+constexpr int kListed = 2;  // times count: threads of a wave that may list their logits
 
 // A logit as the selection sees it.
 template <typename T>
@@ -98,10 +99,10 @@ __device__ __forceinline__ bool live(const SelectArgs& a, int r) {
 // `count` best, of one pass over its logits, which stay in registers.
 //
 // The best: every thread's largest logit; of each wave's 64 the count-th, by
-// votes, and where more than count threads reach it (ties) the lowest tokens among
-// them; the largest of those bounds is reached by at least `count` logits of the
-// split and by those of at most count threads a wave, which alone list what they
-// have from it on; the few in the list find their ranks by counting.  No order
+// votes, and where more than twice that many threads reach it (ties) the lowest
+// tokens among them; the largest of those bounds is reached by at least `count`
+// logits of the split and by those of few threads a wave, which alone list what
+// they have from it on; the few in the list find their ranks by counting.  No order
 // of threads or atomics shows in the result.
 //
 // Bound by its own steps (votes, ranks) more than by the loads: 17 us for 256 rows
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
   const uint32_t key = any ? float_key(top) : 0u, high = key >> LOW, t32 = reached_by<32 - LOW>(high, a.count);
   uint64_t kth = (uint64_t)(t32 << LOW) << 32;
   const int over = __popcll(__ballot(high > t32)), ties = __popcll(__ballot(high == t32));
-  if (t32 != 0 && over + ties > a.count) {
+  if (t32 != 0 && over + ties > kListed * a.count) {
     int first = 0;  // the thread's lowest token of that value
 #pragma unroll
     for (int k = kPerThread - 1; k >= 0; --k) first = v[k] == top && inside(k) ? token(k) : first;
@@ -195,10 +196,16 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
   for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, kWave);
   if (lane == 0) s_sum[wave] = sum;
   if (key != 0 && key >= (uint32_t)(least >> 32)) {
+    const float bound = (uint32_t)(least >> 32) <= float_key(-INFINITY) ? -INFINITY : key_logit(least);
+    uint32_t hits = 0;
 #pragma unroll
-    for (int k = 0; k < kPerThread; ++k) {
-      const uint64_t rk = rank_key(v[k], (uint32_t)token(k));
-      if (inside(k) && rk >= least) list[atomicAdd(&s_n, 1u)] = rk;
+    for (int k = 0; k < kPerThread; ++k) hits |= v[k] >= bound ? 1u << k : 0u;
+    const bool one = (hits & (hits - 1)) == 0;  // the thread's largest
+    for (; hits; hits &= hits - 1) {
+      const int t = token(__ffs(hits) - 1);
+      if (t < from || t >= to) continue;
+      const uint64_t rk = rank_key(one ? top : logit(x[t]), (uint32_t)t);
+      if (rk >= least) list[atomicAdd(&s_n, 1u)] = rk;
     }
   }
   __syncthreads();
@@ -235,23 +242,24 @@ __device__ __forceinline__ double key_score(uint64_t k) {
 }
 
 constexpr int kGroupList = 1024;
-constexpr int kHeldCandidates = 8;  // of a thread, kept in registers
+constexpr int kGroupThreads = 512, kGroupWaves = kGroupThreads / 64;
+constexpr int kHeldCandidates = 4;  // of a thread, kept in registers
 
 // Block (group): the best of its beams' candidates, found as a split's are (by
 // the scores rounded to fp32, which keeps their order, until the list is made);
 // a list that overflows, as with ties of very many candidates, is worked off one
 // by one.
-__global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs a) {
+__global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs a) {
   __shared__ double s_off[kMaxBeams];   // a beam's score less its logits' log sum
   __shared__ float s_cum[kMaxBeams];    // its score
   __shared__ uint8_t s_kind[kMaxBeams]; // bit 0: finished, bit 1: does not exist
   __shared__ Scored list[kGroupList];
-  __shared__ Scored s_w[kSelectWaves];
-  __shared__ uint32_t s_kth[kSelectWaves];
+  __shared__ Scored s_w[kGroupWaves];
+  __shared__ uint32_t s_kth[kGroupWaves];
   __shared__ uint32_t s_n;
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) s_n = 0;
-  for (int b = tid >> 4; b < a.beams; b += kSelectThreads / 16) {  // sixteen lanes a beam
+  for (int b = tid >> 4; b < a.beams; b += kGroupThreads / 16) {  // sixteen lanes a beam
     const int r = g * a.beams + b;
     const float cum = a.scores[r];
     const int kind = (cum > -INFINITY ? 0 : 2) | (a.finished && a.finished[r] != 0 ? 1 : 0);
@@ -283,7 +291,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
   uint64_t key[kHeldCandidates];
 #pragma unroll
   for (int i = 0; i < kHeldCandidates; ++i) {
-    const int c = tid + i * kSelectThreads;
+    const int c = tid + i * kGroupThreads;
     key[i] = c < n ? cand[c] : 0;  // (what a beam without a pass left there is not used)
   }
   __syncthreads();
@@ -302,13 +310,13 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
   Scored held[kHeldCandidates];
 #pragma unroll
   for (int i = 0; i < kHeldCandidates; ++i) {
-    const int c = tid + i * kSelectThreads;
+    const int c = tid + i * kGroupThreads;
     held[i] = c < n ? candidate(c, key[i]) : none;
   }
   auto each = [&](auto&& f) {  // every candidate of this thread
 #pragma unroll
     for (int i = 0; i < kHeldCandidates; ++i) f(held[i]);
-    for (int c = tid + kHeldCandidates * kSelectThreads; c < n; c += kSelectThreads) f(candidate(c, cand[c]));
+    for (int c = tid + kHeldCandidates * kGroupThreads; c < n; c += kGroupThreads) f(candidate(c, cand[c]));
   };
   auto write = [&](const Scored& c, int rank) {
     const size_t at = (size_t)g * a.count + rank;
@@ -326,7 +334,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
   __syncthreads();
   uint32_t least = 1;
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) least = max(least, s_kth[w]);
+  for (int w = 0; w < kGroupWaves; ++w) least = max(least, s_kth[w]);
   if (best >= least)
     each([&](const Scored& x) {
       if (rounded(x) < least) return;
@@ -336,7 +344,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
   __syncthreads();
   const int m = (int)s_n;
   if (m <= kGroupList) {
-    for (int j = tid >> 2; j < m; j += kSelectThreads / 4) {  // four lanes a candidate
+    for (int j = tid >> 2; j < m; j += kGroupThreads / 4) {  // four lanes a candidate
       const Scored x = list[j];
       int rank = 0;
 #pragma unroll 4
@@ -362,7 +370,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_group_kernel(SelectArgs
     if (lane == 0) s_w[wave] = next;
     __syncthreads();
     last = s_w[0];
-    for (int w = 1; w < kSelectWaves; ++w)
+    for (int w = 1; w < kGroupWaves; ++w)
       if (s_w[w].over(last)) last = s_w[w];
     if (tid == 0) write(last, k);
   }
@@ -513,8 +521,8 @@ void beam_select(const mit2cfm_beam_select& p, hipStream_t s) {
   w += align16(parts * a.count * 8);
   a.tops = reinterpret_cast<float*>(w);
   const dim3 grid(a.splits, rows), block(kSelectThreads);
-  // the list holds all logits of count threads a wave
-  const size_t lds = std::min<size_t>((size_t)kSelectWaves * a.count * kPerThread, kMaxChunk) * 8;
+  // the list holds all logits of as many threads a wave as may list them
+  const size_t lds = std::min<size_t>((size_t)kSelectWaves * kListed * a.count * kPerThread, kMaxChunk) * 8;
   if (p.dtype == MIT2CFM_DTYPE_F32)
     hipLaunchKernelGGL((select_rows_kernel<float>), grid, block, lds, s, a);
   else if (p.dtype == MIT2CFM_DTYPE_F16)
@@ -522,7 +530,7 @@ void beam_select(const mit2cfm_beam_select& p, hipStream_t s) {
   else
     hipLaunchKernelGGL((select_rows_kernel<bf16_t>), grid, block, lds, s, a);
   launched(hipGetLastError());
-  hipLaunchKernelGGL(select_group_kernel, dim3(p.groups), block, 0, s, a);
+  hipLaunchKernelGGL(select_group_kernel, dim3(p.groups), dim3(kGroupThreads), 0, s, a);
   launched(hipGetLastError());
 }
 
