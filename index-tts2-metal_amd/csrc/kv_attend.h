@@ -655,6 +655,10 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
   // row's comes by a shuffle.  (Looked up a buffer ahead, each wait for one
   // waited for the loads in flight as well.)
   int held = INT_MIN, entries = 0;
+  const bool in_a_page = (1 << a.c.page_shift) >= KEYS;  // (buffers start at multiples of KEYS)
+  uint32_t mine[PASSES];  // this thread's elements of a buffer that lies in one page
+#pragma unroll
+  for (int u = 0; u < PASSES; ++u) mine[u] = (row0 + STEP * u) * D + ((tid % CPR) ^ ((row0 + STEP * u) & XM)) * E16;
   auto entry_of = [&](int j) { return __shfl(entries, (j >> a.c.page_shift) - held, kWave); };
   // Starts a buffer's loads (rows that are not there read page 0); which keys are
   // there, as bits (lanes past KEYS repeat).
@@ -666,6 +670,18 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
       __asm__ volatile("" : "+v"(entries));  // (waits here, not wherever it is used)
     }
     u32x4 *k = bufK(buf) + 64 * wave, *v = bufV(buf) + 64 * wave;
+    const int j = j0 + (lane & (KEYS - 1));
+    if (in_a_page) {  // one entry for all, and only the page differs from buffer to buffer
+      const int entry = __builtin_amdgcn_readlane(entries, (at0 >> a.c.page_shift) - held);
+      const bool ok = (unsigned)entry < (unsigned)a.c.pages;
+      const int64_t page = a.c.row_in(ok ? entry : 0, j0, D);
+#pragma unroll
+      for (int u = 0; u < PASSES; ++u) {
+        load_to_lds(K + page + mine[u], (lds_ptr_t*)(k + kAttendThreads * u));
+        load_to_lds(V + page + mine[u], (lds_ptr_t*)(v + kAttendThreads * u));
+      }
+      return (uint64_t)__ballot(ok && j < p.len);
+    }
 #pragma unroll
     for (int u = 0; u < PASSES; ++u) {
       const int r = row0 + STEP * u;
@@ -674,16 +690,8 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
       load_to_lds(K + at, (lds_ptr_t*)(k + kAttendThreads * u));
       load_to_lds(V + at, (lds_ptr_t*)(v + kAttendThreads * u));
     }
-    const int j = j0 + (lane & (KEYS - 1));
     return (uint64_t)__ballot((unsigned)entry_of(min(j, p.len - 1)) < (unsigned)a.c.pages && j < p.len);
   };
-  // The keys that are there, of this buffer, the next and the one after.
-  constexpr uint64_t all_keys = ~0ull;
-  uint64_t there0 = 0, there1 = 0, there2 = 0;
-  if (p.begin < p.end) {
-    there0 = load(p.begin, 0);
-    there1 = load(p.begin + KEYS, 1);
-  }
 
   int qm[WMT];
   Op qv[WMT][DC];
@@ -695,115 +703,96 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
     run[mt].clear();
   }
 
-  bool dirty = false;
-  // Tile `sub` of the buffer that starts at key b0.  SOME: keys may be missing or
-  // new, so that not all rows see them all.
-  auto work = [&](auto some_, int b0, int sub, const u32x4* tk, const u32x4* tv) {
-    constexpr bool SOME = decltype(some_)::value;
-    const int j0 = b0 + sub * KT;
-    // (past the end, or past what a chain's rows of this wave see)
-    if (SOME && (j0 >= p.end || (!a.mask && j0 - p.first > last_q.i))) return;
-    tk += sub * KT * CPR;
-    tv += sub * KT * CPR;
-    uint32_t there = (1u << NV) - 1u;
-    // An empty statement between the lane's numbers and the LDS addresses that
-    // follow from them: formed here, a few operations, instead of held for all
-    // buffers throughout (about 100 registers).
-    int lq_ = lq, grp_ = grp;
-    __asm__ volatile("" : "+v"(lq_), "+v"(grp_));
-    if (SOME) {
-      const uint32_t bits = (uint32_t)(there0 >> (sub * KT)) >> (4 * grp_);
-      there = NT == 2 ? (bits & 15u) | (bits >> 12 & 0xf0u) : bits & 15u;
-    }
-    // (the rare form takes its query tiles one after the other, for fewer registers)
-    constexpr int MB = SOME ? 1 : WMT;
+  // The keys that are there, of this buffer, the next and the one after.
+  constexpr uint64_t all_keys = ~0ull;
+  uint64_t there0 = 0, there1 = 0, there2 = 0;
+  if (p.begin < p.end) {
+    there0 = load(p.begin, 0);
+    there1 = load(p.begin + KEYS, 1);
+    there2 = load(p.begin + 2 * KEYS, 2);
+    wait_loads<4 * PASSES>();
+    meet();
+  }
+
+  // A tile's keys and values from a buffer.  Of the places that a lane reads, those
+  // of other rows are constants away, and those of other pieces of a row are an
+  // XOR of the number's low bits.  The empty statement keeps the compiler
+  // from holding each such address for each buffer throughout (about 100 registers).
+  const int k_place = lq * CPR + ((sizeof(T) == 2 ? grp : DC / 4 * grp) ^ (lq & XM));
+  constexpr int PB = DP * sizeof(T), PV = PB <= 16 ? 1 : PB / 16;  // bytes of a lane's piece of a value, 16-byte places
+  const int v_place = (4 * grp * CPR + ((lq * PB / 16) ^ (4 * grp & XM))) * 16 + (PB < 16 ? lq * PB % 16 : 0);
+  auto read_keys = [&](const u32x4* tk, Op(&kv)[NT][DC]) {
+    int at = k_place;
+    __asm__ volatile("" : "+v"(at));
 #pragma unroll
-    for (int m0 = 0; m0 < WMT; m0 += MB) {
-      float s[MB][NV];
-      {
-        Op kv[NT][DC];
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int r = 16 * t + lq_;
-          if constexpr (sizeof(T) == 2) {
+        for (int c = 0; c < DC; ++c) kv[t][c] = *reinterpret_cast<const Op*>(&tk[(at ^ 4 * c) + 16 * t * CPR]);
+      } else {
 #pragma unroll
-            for (int c = 0; c < DC; ++c)
-              kv[t][c] = *reinterpret_cast<const Op*>(&tk[r * CPR + ((4 * c + grp_) ^ (r & XM))]);
-          } else {
-#pragma unroll
-            for (int c = 0; c < DC; c += 4) {
-              const floatx4 x =
-                  *reinterpret_cast<const floatx4*>(&tk[r * CPR + ((DC / 4 * grp_ + c / 4) ^ (r & XM))]);
-              kv[t][c] = x[0]; kv[t][c + 1] = x[1]; kv[t][c + 2] = x[2]; kv[t][c + 3] = x[3];
-            }
-          }
-        }
-#pragma unroll
-        for (int mt = 0; mt < MB; ++mt) {
-          uint32_t seen = there;
-          if (SOME) {
-            int m = qm[m0 + mt];
-            __asm__ volatile("" : "+v"(m));
-            seen = seen_keys<NV>(a, Query(a, p, m), j0, p.first, grp_, there);
-          }
-          score_tile<T, D>(kv, qv[m0 + mt], SOME, seen, s[mt]);
+        for (int c = 0; c < DC; c += 4) {
+          const floatx4 x = *reinterpret_cast<const floatx4*>(&tk[(at ^ c / 4) + 16 * t * CPR]);
+          kv[t][c] = x[0]; kv[t][c + 1] = x[1]; kv[t][c + 2] = x[2]; kv[t][c + 3] = x[3];
         }
       }
-      Piece<T, DP> vv[NV];
-#pragma unroll
-      for (int e = 0; e < NV; ++e) {
-        const int r = key_of(e, grp_);
-        constexpr int PB = DP * sizeof(T);  // 8, 16 or 32 bytes of a lane
-        const char* base = reinterpret_cast<const char*>(&tv[r * CPR]);
-        if constexpr (PB <= 16) {
-          vv[e] = *reinterpret_cast<const Piece<T, DP>*>(base + ((lq_ * PB / 16) ^ (r & XM)) * 16 + lq_ * PB % 16);
-        } else {
-#pragma unroll
-          for (int u = 0; u < PB / 16; ++u) {
-            const Piece<T, DP / (PB / 16)> x =
-                *reinterpret_cast<const Piece<T, DP / (PB / 16)>*>(base + ((lq_ * (PB / 16) + u) ^ (r & XM)) * 16);
-#pragma unroll
-            for (int d = 0; d < DP / (PB / 16); ++d) vv[e].v[u * (DP / (PB / 16)) + d] = x.v[d];
-          }
-        }
-      }
-      if (SOME) {
-#pragma unroll
-        for (int e = 0; e < NV; ++e)
-#pragma unroll
-          for (int d = 0; d < DP; ++d) vv[e].v[d] = there >> e & 1u ? vv[e].v[d] : (T)0.f;
-        const bool odd = take_out(vv);
-        dirty = dirty || odd;
-      }
-#pragma unroll
-      for (int mt = 0; mt < MB; ++mt) run[m0 + mt].weigh(s[mt], a.scale2);
-      add_values<T, D, MB>(vv, s, run + m0);
     }
   };
-  // A buffer's turn: its loads have landed, for every wave; the one after the next
-  // is filled where the last one was.
-  auto turn = [&](int buf, int b0) {
+  auto read_values = [&](const u32x4* tv, Piece<T, DP>(&vv)[NV]) {
+    int at = v_place;
+    __asm__ volatile("" : "+v"(at));
+    const char* base = reinterpret_cast<const char*>(tv);
+#pragma unroll
+    for (int e = 0; e < NV; ++e) {
+      const int row = (16 * (e >> 2) + (e & 3)) * CPR * 16;
+#pragma unroll
+      for (int u = 0; u < PV; ++u) {
+        const Piece<T, DP / PV> x = *reinterpret_cast<const Piece<T, DP / PV>*>(base + (at ^ ((e & 3) ^ u) * 16) + row);
+#pragma unroll
+        for (int d = 0; d < DP / PV; ++d) vv[e].v[u * (DP / PV) + d] = x.v[d];
+      }
+    }
+  };
+  // This buffer is read, by every wave, and the next has landed; the one after the
+  // two to come is filled in its place.
+  auto advance = [&](int buf, int& b0) {
     wait_loads<2 * PASSES>();
     meet();
-    there2 = load(b0 + 2 * KEYS, buf == 0 ? 2 : buf - 1);
-  };
-  auto done = [&](int& b0) {
     there0 = there1;
     there1 = there2;
+    there2 = load(b0 + 3 * KEYS, buf);
     b0 += KEYS;
   };
+
   // All rows see all keys of the buffers up to the first that holds a row which
   // not all see, or misses one: a loop of its own, whose turns follow each other without a branch
-  // that could meet the outputs' registers (merged, they were kept twice).
+  // that could meet the outputs' registers (merged, they were kept twice).  A tile's
+  // values are on their way during its weights, the next tile's keys during its
+  // second products.
   int b0 = p.begin, buf = 0;
   if (works) {
     auto plain = [&] { return there0 == all_keys && b0 + KEYS <= open && b0 < p.end; };
+    Op kv[NT][DC];
+    if (plain()) read_keys(bufK(0), kv);
     auto one = [&](auto buf_) {
-      constexpr int B = decltype(buf_)::value;
-      turn(B, b0);
+      constexpr int B = decltype(buf_)::value, TILES = KEYS / KT;
 #pragma unroll
-      for (int sub = 0; sub < KEYS / KT; ++sub) work(std::false_type{}, b0, sub, bufK(B), bufV(B));
-      done(b0);
+      for (int sub = 0; sub < TILES; ++sub) {
+        float s[WMT][NV];
+        Piece<T, DP> vv[NV];
+#pragma unroll
+        for (int mt = 0; mt < WMT; ++mt) score_tile<T, D>(kv, qv[mt], false, 0u, s[mt]);
+        read_values(bufV(B) + sub * KT * CPR, vv);
+#pragma unroll
+        for (int mt = 0; mt < WMT; ++mt) run[mt].weigh(s[mt], a.scale2);
+        if (sub + 1 < TILES) {
+          read_keys(bufK(B) + (sub + 1) * KT * CPR, kv);
+        } else {
+          advance(B, b0);
+          read_keys(bufK(B == 2 ? 0 : B + 1), kv);
+        }
+        add_values<T, D, WMT>(vv, s, run);
+      }
     };
     for (;;) {
       buf = 0;
@@ -817,12 +806,43 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
       one(std::integral_constant<int, 2>{});
     }
   }
+  // The other buffers: keys may be missing or new, so that not all rows see them all
+  // (query tiles one after the other, for fewer registers).
+  bool dirty = false;
+  auto rest = [&](int j0, uint32_t bits, const u32x4* tk, const u32x4* tv) {
+    // (past the end, or past what a chain's rows of this wave see)
+    if (j0 >= p.end || (!a.mask && j0 - p.first > last_q.i)) return;
+    bits >>= 4 * grp;
+    const uint32_t there = NT == 2 ? (bits & 15u) | (bits >> 12 & 0xf0u) : bits & 15u;
+#pragma unroll
+    for (int mt = 0; mt < WMT; ++mt) {
+      float s[1][NV];
+      {
+        Op kv[NT][DC];
+        read_keys(tk, kv);
+        int m = qm[mt];
+        __asm__ volatile("" : "+v"(m));
+        const uint32_t seen = seen_keys<NV>(a, Query(a, p, m), j0, p.first, grp, there);
+        score_tile<T, D>(kv, qv[mt], true, seen, s[0]);
+      }
+      Piece<T, DP> vv[NV];
+      read_values(tv, vv);
+#pragma unroll
+      for (int e = 0; e < NV; ++e)
+#pragma unroll
+        for (int d = 0; d < DP; ++d) vv[e].v[d] = there >> e & 1u ? vv[e].v[d] : (T)0.f;
+      const bool odd = take_out(vv);
+      dirty = dirty || odd;
+      run[mt].weigh(s[0], a.scale2);
+      add_values<T, D, 1>(vv, s, run + mt);
+    }
+  };
   for (; b0 < p.end; buf = buf == 2 ? 0 : buf + 1) {
-    turn(buf, b0);
     if (works)
 #pragma unroll 1
-      for (int sub = 0; sub < KEYS / KT; ++sub) work(std::true_type{}, b0, sub, bufK(buf), bufV(buf));
-    done(b0);
+      for (int sub = 0; sub < KEYS / KT; ++sub)
+        rest(b0 + sub * KT, (uint32_t)(there0 >> (sub * KT)), bufK(buf) + sub * KT * CPR, bufV(buf) + sub * KT * CPR);
+    advance(buf, b0);
   }
   wait_loads<0>();  // (LDS must not be written after the block's end)
 
