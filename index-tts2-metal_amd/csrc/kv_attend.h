@@ -782,6 +782,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
         Piece<T, DP> vv[NV];
 #pragma unroll
         for (int mt = 0; mt < WMT; ++mt) score_tile<T, D>(kv, qv[mt], false, 0u, s[mt]);
+        __builtin_amdgcn_s_setprio(0);
         read_values(bufV(B) + sub * KT * CPR, vv);
 #pragma unroll
         for (int mt = 0; mt < WMT; ++mt) run[mt].weigh(s[mt], a.scale2);
@@ -791,6 +792,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
           advance(B, b0);
           read_keys(bufK(B == 2 ? 0 : B + 1), kv);
         }
+        __builtin_amdgcn_s_setprio(1);
         add_values<T, D, WMT>(vv, s, run);
       }
     };
