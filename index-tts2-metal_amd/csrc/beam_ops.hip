@@ -105,9 +105,9 @@ __device__ __forceinline__ bool live(const SelectArgs& a, int r) {
 // they have from it on; the few in the list find their ranks by counting.  No order
 // of threads or atomics shows in the result.
 //
-// Bound by its own steps (votes, ranks) more than by the loads: 17 us for 256 rows
-// of 50001 bf16, whose 26 MB take 6; 6.3 us for three rows of 8194, which is one
-// block's way through.  With 32 logits a thread 17 and 8 us.
+// Bound by its own instructions and waits (votes, barriers, ranks) more than by the
+// loads: 14 us for 256 rows of 50001 bf16, whose 26 MB take 6; 5.6 us for three rows of
+// 8194, which is one block's way through.  With 32 logits a thread 15 and 6.4 us.
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs a) {
   constexpr int W = 16 / sizeof(T), LOADS = kPerThread / W;  // logits of a load
@@ -248,7 +248,8 @@ constexpr int kHeldCandidates = 4;  // of a thread, kept in registers
 // Block (group): the best of its beams' candidates, found as a split's are (by
 // the scores rounded to fp32, which keeps their order, until the list is made);
 // a list that overflows, as with ties of very many candidates, is worked off one
-// by one.
+// by one.  A group's block waits for the chip, not the chip for it: 6.5 us for 32
+// groups of 1664 candidates (10 with 256 threads, as much with 1024), 4.4 for 54.
 __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs a) {
   __shared__ double s_off[kMaxBeams];   // a beam's score less its logits' log sum
   __shared__ float s_cum[kMaxBeams];    // its score
@@ -413,6 +414,11 @@ constexpr int kReorderThreads = 256;
 // the group's parents as bits: a beam is a further child when an earlier one
 // has its parent, its rank among those is its index less the distinct parents
 // before it, and there are as many beams without children.
+//
+// Bound by the part pages' copies: 32 searches of 8 beams, 24 layers of 8 heads of 64
+// bf16, 135 MB in 28 us when the last step left them in the caches, else in 42; three
+// beams of 20 fp32 heads take 3.7 us, most of it four waits in a row (parents,
+// length, table, rows).
 constexpr int kCopyBatch = 4;  // 16-byte loads of a thread in flight, of k and of v each
 __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(ReorderArgs a) {
   const int r = blockIdx.x, g = r / a.beams, b = r - g * a.beams;

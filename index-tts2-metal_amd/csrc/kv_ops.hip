@@ -50,23 +50,27 @@ struct AppendArgs {
   double log2_theta;
 };
 
-// A block takes R rows' items (blockIdx.y: its share of them).  An item is two
+// A block takes a row's items (blockIdx.y: its share of them).  An item is two
 // vectors of VEC elements of a head, chosen so that a rotated pair's two
 // elements are both in it: (i, i + rot/2), or neighbours when interleaved and
-// past the rotated part.  The rows' angles go through LDS once for all heads:
+// past the rotated part.  The row's angles go through LDS once for all heads:
 // the angle in turns, fp64, brought to [-1/2, 1/2] there, and its cosine and
-// sine in fp32, as everything that follows.
-template <typename T, int VEC, int R>
+// sine in fp32, as everything that follows.  The result's rounding to the type is
+// the only one to fewer bits.
+//
+// Bound by its reads and writes: nine prompts of up to 2047 rows, 32 + 2 x 8 heads of
+// 128 bf16, 332 MB in 68 us (4.9 TB/s; a large copy reaches 4.7).  Trees of 25 rows of
+// 16 sequences take 4.7 us and three single rows 3.0, mostly the launch and two
+// waits in a row (the row's sequence, then its page).
+template <typename T, int VEC>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, int D) {
-  __shared__ float2 turn[R][kMaxPairs];
-  __shared__ int64_t s_at[R];  // element index of the row in its page, head 0; -1: not written
-  __shared__ int s_place[R];   // the row's position; INT_MIN: no sequence's row
-  const int tid = threadIdx.x, row0 = blockIdx.x * R;
-  const int wave = tid >> 6;
-  for (int i = wave; i < R; i += kAppendThreads / 64) {
-    const int row = row0 + i;
-    const int seq = row < a.r.rows ? seq_of_row(a.r, row) : -1;
-    if ((tid & 63) == 0) {
+  __shared__ float2 turn[kMaxPairs];
+  __shared__ int64_t s_at;  // element index of the row in its page, head 0; -1: not written
+  __shared__ int s_place;   // the row's position; INT_MIN: no sequence's row
+  const int tid = threadIdx.x, row = blockIdx.x;
+  if (tid < 64) {
+    const int seq = seq_of_row(a.r, row);
+    if (tid == 0) {
       int64_t at = -1;
       int pos = INT_MIN;
       if (seq >= 0) {
@@ -78,30 +82,26 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, in
         pos = a.position ? a.position[row] : place;
         if (pos == INT_MIN) pos = INT_MIN + 1;
       }
-      s_at[i] = at;
-      s_place[i] = pos;
+      s_at = at;
+      s_place = pos;
     }
   }
   __syncthreads();
+  if (s_place == INT_MIN) return;
   const int half = a.rot >> 1;
-  for (int i = tid; i < R * half; i += kAppendThreads) {
-    const int rr = i / half, p = i - rr * half;
+  for (int p = tid; p < half; p += kAppendThreads) {
     const double inv = exp2(-2.0 * p / a.rot * a.log2_theta) * 0.15915494309189533577;  // 1 / (2 pi)
-    double t = (double)s_place[rr] * inv;
+    double t = (double)s_place * inv;
     t -= rint(t);
     float sn, cs;
     sincospif((float)(2.0 * t), &sn, &cs);
-    turn[rr][p] = make_float2(cs, sn);
+    turn[p] = make_float2(cs, sn);
   }
   __syncthreads();
   const int per_head = D / (2 * VEC);
-  const int heads = a.q_heads + 2 * a.c.kv_heads;
-  const int items = R * heads * per_head;
+  const int items = (a.q_heads + 2 * a.c.kv_heads) * per_head;
   for (int it = blockIdx.y * kAppendThreads + tid; it < items; it += gridDim.y * kAppendThreads) {
-    const int u = it % per_head, rh = it / per_head;
-    const int h = rh % heads, rr = rh / heads;
-    if (s_place[rr] == INT_MIN) continue;
-    const int row = row0 + rr;
+    const int u = it % per_head, h = it / per_head;
     // the item's two vectors, and the pair index of its first element
     int e0, e1, pair0;
     const bool rotates = h < a.q_heads + a.c.kv_heads;
@@ -126,13 +126,13 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, in
       src = reinterpret_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
       dst = reinterpret_cast<T*>(a.q_out) + row * a.qo_row + h * a.qo_head;
     } else {
-      if (s_at[rr] < 0) continue;
+      if (s_at < 0) continue;
       const int kh = h - a.q_heads;
       const bool is_k = kh < a.c.kv_heads;
       const int hh = is_k ? kh : kh - a.c.kv_heads;
       src = is_k ? reinterpret_cast<const T*>(a.k) + row * a.k_row + hh * a.k_head
                  : reinterpret_cast<const T*>(a.v) + row * a.v_row + hh * a.v_head;
-      dst = reinterpret_cast<T*>(is_k ? a.c.k : a.c.v) + s_at[rr] + hh * a.c.head_stride(D);
+      dst = reinterpret_cast<T*>(is_k ? a.c.k : a.c.v) + s_at + hh * a.c.head_stride(D);
     }
     Vec<T, VEC> x = *reinterpret_cast<const Vec<T, VEC>*>(src + e0);
     Vec<T, VEC> y = *reinterpret_cast<const Vec<T, VEC>*>(src + e1);
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, in
           T& p = 2 * j < VEC ? x.v[(2 * j) % VEC] : y.v[(2 * j) % VEC];
           T& q = 2 * j + 1 < VEC ? x.v[(2 * j + 1) % VEC] : y.v[(2 * j + 1) % VEC];
           if (pair0 + j < half) {
-            const float2 cs = turn[rr][pair0 + j];
+            const float2 cs = turn[pair0 + j];
             const float fp = (float)p, fq = (float)q;
             p = (T)(fp * cs.x - fq * cs.y);
             q = (T)(fq * cs.x + fp * cs.y);
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, in
       } else {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float2 cs = turn[rr][pair0 + j];
+          const float2 cs = turn[pair0 + j];
           const float fp = (float)x.v[j], fq = (float)y.v[j];
           x.v[j] = (T)(fp * cs.x - fq * cs.y);
           y.v[j] = (T)(fq * cs.x + fp * cs.y);
@@ -165,13 +165,12 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, in
   }
 }
 
-template <typename T, int VEC, int R>
-void launch_append_rows(const AppendArgs& a, int D, hipStream_t s) {
-  const int bx = (a.r.rows + R - 1) / R;
-  const int items = R * (a.q_heads + 2 * a.c.kv_heads) * (D / (2 * VEC));
+template <typename T, int VEC>
+void launch_append_by(const AppendArgs& a, int D, hipStream_t s) {
+  const int items = (a.q_heads + 2 * a.c.kv_heads) * (D / (2 * VEC));
   // few rows: their heads over more blocks, down to one item a thread
-  const int by = std::max(1, std::min((items + kAppendThreads - 1) / kAppendThreads, 2048 / bx));
-  hipLaunchKernelGGL((append_kernel<T, VEC, R>), dim3(bx, by), dim3(kAppendThreads), 0, s, a, D);
+  const int by = std::max(1, std::min((items + kAppendThreads - 1) / kAppendThreads, 2048 / a.r.rows));
+  hipLaunchKernelGGL((append_kernel<T, VEC>), dim3(a.r.rows, by), dim3(kAppendThreads), 0, s, a, D);
   launched(hipGetLastError());
 }
 
@@ -182,33 +181,34 @@ void launch_append(const AppendArgs& a, int D, hipStream_t s) {
   const bool wide = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head) &&
                     (!a.q_heads || (fits(a.q, a.q_row, a.q_head) && fits(a.q_out, a.qo_row, a.qo_head))) &&
                     (a.interleaved || a.rot % (2 * V) == 0);
-  // Rows that fill the chip by themselves share a block's angles four at a time.
-  if (!wide)
-    launch_append_rows<T, 1, 1>(a, D, s);
-  else if (a.r.rows >= 2048)
-    launch_append_rows<T, V, 4>(a, D, s);
+  if (wide)
+    launch_append_by<T, V>(a, D, s);
   else
-    launch_append_rows<T, V, 1>(a, D, s);
+    launch_append_by<T, 1>(a, D, s);
 }
 
 // ------------------------------------------------------------------ attention
 constexpr int kBlocksWanted = 1024;   // four blocks of the small tiles a CU
 // Of the wide ones two fit a CU at 128 elements of 16 bits (by registers), else
 // three (by LDS).  More than those, as the last splits of shorter sequences are
-// short: trees of 63 over 4099 f16 keys take 78, 70, 92 us at 512, 640, 768, a
-// chain of 257 over 1201 f32 keys 54, 54, 50.
+// short: trees of 63 over 4099 f16 keys take 72, 65, 87 us at 512, 640, 768, a
+// chain of 257 over 1201 f32 keys 43 at each.
 constexpr int wide_wanted(int D, bool f32) { return D == 128 && !f32 ? 640 : 768; }
 constexpr int kMostSplits = 128;
 
 AttendPlan attend_plan(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
   const int group = (int)(q_heads / c.kv_heads), D = (int)c.head_dim;
   const bool f32 = c.dtype == MIT2CFM_DTYPE_F32;
-  // Query rows of a tile follow the average sequence: up to four matrix tiles a
-  // wave (at head sizes past 128 two: their accumulators fill the registers),
-  // past that the block kernel.
+  // Query rows of a tile follow the average sequence's.  Of 8 heads of 128 f16 in 8
+  // sequences of 4000 keys, 16 rows take 32, 43, 28 us with one tile, two, and the block
+  // kernel, 32 rows 49, 44, 32, 64 rows 82, 65, 37; 24 rows over 131001 bf16 keys 154,
+  // 119, 139; and one row of each of 64 sequences, the decoding step, 187, -, 193.
+  // Of heads of 64, and of fp32, the block kernel gains later: 20 heads of 64 f16 take 56,
+  // 43, 46 us at 32 rows, 77, 61, 50 at 48; fp32 111, 79, 111 and 164, 142, 146 (in 2
+  // sequences 34, 28, 35 and 47, 44, 39).  Four tiles a wave were slower than two.
   const uint64_t m = (uint64_t)r.rows * group / r.seqs;
   AttendPlan p;
-  p.form = wide_dim(D) && m > 64 ? kWide : m <= 16 ? 1 : m <= 32 || D > 128 ? 2 : 4;
+  p.form = wide_dim(D) && m > (D == 128 && !f32 ? 16 : 32) ? kWide : m <= 16 ? 1 : 2;
   const int mtile = p.form == kWide ? wide_rows(f32) : 16 * p.form;
   // sum over the sequences of ceil(rows * group / mtile): at most ...
   const uint64_t by_fill = ((uint64_t)r.rows * group + (uint64_t)std::min(r.seqs, r.rows) * (mtile - 1)) / mtile;
