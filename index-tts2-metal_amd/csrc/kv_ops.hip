@@ -59,9 +59,9 @@ struct AppendArgs {
 // the only one to fewer bits.
 //
 // Bound by its reads and writes: nine prompts of up to 2047 rows, 32 + 2 x 8 heads of
-// 128 bf16, 332 MB in 68 us (4.9 TB/s; a large copy reaches 4.7).  Trees of 25 rows of
-// 16 sequences take 4.7 us and three single rows 3.0, mostly the launch and two
-// waits in a row (the row's sequence, then its page).
+// 128 bf16, 332 MB in 64 us (5.2 TB/s; a large copy reaches 4.7), four rows a block in
+// 69.  Trees of 25 rows of 16 sequences take 4.5 us and three single rows 2.8, mostly
+// the launch and two waits in a row (the row's sequence, then its page).
 template <typename T, int VEC>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, int D) {
   __shared__ float2 turn[kMaxPairs];
