@@ -406,7 +406,7 @@ struct ReorderArgs {
   const int32_t* place;
 };
 
-constexpr int kReorderThreads = 256;
+constexpr int kReorderThreads = 512;
 
 // Block (new beam, part): part 0 writes the beam's table row and states, part 1
 // + l copies the part page's rows of layer l, for a beam that is not its
@@ -416,10 +416,12 @@ constexpr int kReorderThreads = 256;
 // before it, and there are as many beams without children.
 //
 // Bound by the part pages' copies: 32 searches of 8 beams, 24 layers of 8 heads of 64
-// bf16, 135 MB in 28 us when the last step left them in the caches, else in 42; three
-// beams of 20 fp32 heads take 3.7 us, most of it four waits in a row (parents,
-// length, table, rows).
-constexpr int kCopyBatch = 4;  // 16-byte loads of a thread in flight, of k and of v each
+// bf16, 135 MB in 30 us (4.5 TB/s).  Their stores go past the caches, whose lines the
+// pages' other bytes would come into first: 45 us with ordinary ones (and no loss to
+// the attention after, which reads far more than it finds there).  Three beams of 20
+// fp32 heads take 2.9 us, most of it four waits in a row (parents, length, table,
+// rows).  Several layers a block, 49 us and more.
+constexpr int kCopyBatch = 2;  // 16-byte loads of a thread in flight, of k and of v each
 __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(ReorderArgs a) {
   const int r = blockIdx.x, g = r / a.beams, b = r - g * a.beams;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -480,8 +482,8 @@ __global__ __launch_bounds__(kReorderThreads) void reorder_kernel(ReorderArgs a)
 #pragma unroll
     for (int u = 0; u < kCopyBatch; ++u)
       if (i0 + u * kReorderThreads < n) {
-        k[d + at[u]] = x[u];
-        v[d + at[u]] = y[u];
+        __builtin_nontemporal_store(x[u], k + d + at[u]);
+        __builtin_nontemporal_store(y[u], v + d + at[u]);
       }
   }
 }
