@@ -619,8 +619,10 @@ __device__ __forceinline__ void load_to_lds(const void* src, lds_ptr_t* lds) {
 // move into the operand of each score) and by the matrix cores behind them, which
 // two waves a SIMD overlap in part: trees of 63 rows, 32 query heads on 8 of 128,
 // over up to 4099 f16 keys take 57 us, 18 of vector and 8 of matrix instructions; a
-// ring of five buffers is 2.5% faster there and leaves no LDS.  A chain of 257 over
-// 1201 fp32 keys of 20 heads of 64 takes 40 us.  //
+// ring of five buffers is 2.5% faster there and leaves no LDS, two buffers of twice
+// the keys, with half the barriers, are as fast.  A chain of 257 over
+// 1201 fp32 keys of 20 heads of 64 takes 40 us.
+//
 // The ring's buffers are objects of their own, named by constants in the usual
 // path: a read that might alias any of them would wait for every load.
 template <typename T, int D>
