@@ -52,3 +52,15 @@ def test_a_workspace_that_covers_the_sizes(mit2):
     small = mit2.beam_select_workspace(s)
     s.groups = 4
     assert 0 < small < mit2.beam_select_workspace(s)
+
+
+def test_pages_and_places(mit2, tmp_path):
+    """kv_view.h's arithmetic compiled for the host alone."""
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not Path(hipcc).exists():
+        pytest.skip("hipcc not available")
+    exe = tmp_path / "kv_pages"
+    subprocess.run([hipcc, "-x", "hip", "--offload-host-only", "-std=c++17", "-O1", f"-I{mit2.PKG_DIR / 'csrc'}",
+                    str(Path(__file__).parent / "kv_pages.cpp"), "-o", str(exe)], check=True, capture_output=True, timeout=110)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and "0 wrong" in run.stdout, run.stdout + run.stderr
