@@ -372,15 +372,17 @@ __device__ __forceinline__ void add_values(const Piece<T, Dims<T, D>::DP> (&vv)[
 
 // New rows' values that are not finite must not meet a weight of 0 (0 x NaN
 // would reach rows that do not see them): they enter the products as 0 and join
-// at the end, for the rows that see them.
+// at the end, for the rows that see them.  Rows before the new ones, which every
+// row sees, stay in the products (new0: the tile's first key's place among the
+// new rows, negative before them).
 template <typename T, int NV, int DP>
-__device__ __forceinline__ bool take_out(Piece<T, DP> (&vv)[NV]) {
+__device__ __forceinline__ bool take_out(Piece<T, DP> (&vv)[NV], int new0, int grp) {
   bool odd = false;
 #pragma unroll
   for (int e = 0; e < NV; ++e)
 #pragma unroll
     for (int d = 0; d < DP; ++d) {
-      const bool bad = !finite(vv[e].v[d]);
+      const bool bad = new0 + key_of(e, grp) >= 0 && !finite(vv[e].v[d]);
       vv[e].v[d] = bad ? (T)0.f : vv[e].v[d];
       odd = odd | bad;
     }
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a, At
         for (int d = 0; d < DP; ++d) vv[e].v[d] = there >> e & 1u ? vv[e].v[d] : (T)0.f;
     }
     if (fresh) {
-      const bool odd = take_out(vv);
+      const bool odd = take_out(vv, j0 - p.first, grp);
       dirty = dirty || odd;
     }
     float s[MT][NV];
@@ -845,8 +847,10 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
       for (int e = 0; e < NV; ++e)
 #pragma unroll
         for (int d = 0; d < DP; ++d) vv[e].v[d] = there >> e & 1u ? vv[e].v[d] : (T)0.f;
-      const bool odd = take_out(vv);
-      dirty = dirty || odd;
+      if (j0 + KT > p.first) {
+        const bool odd = take_out(vv, j0 - p.first, grp);
+        dirty = dirty || odd;
+      }
       run[mt].weigh(s[0], a.scale2);
       add_values<T, D, 1>(vv, s, run + mt);
     }
