@@ -251,7 +251,7 @@ constexpr int kHeldCandidates = 4;  // of a thread, kept in registers
 // by one.  A group's block waits for the chip, not the chip for it: 6.5 us for 32
 // groups of 1664 candidates (10 with 256 threads, as much with 1024), 4.4 for 54.
 __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs a) {
-  __shared__ double s_off[kMaxBeams];   // a beam's score less its logits' log sum
+  __shared__ double s_log[kMaxBeams];   // a beam's logits' log sum; -inf: none is over -inf
   __shared__ float s_cum[kMaxBeams];    // its score
   __shared__ uint8_t s_kind[kMaxBeams]; // bit 0: finished, bit 1: does not exist
   __shared__ Scored list[kGroupList];
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs 
     const int r = g * a.beams + b;
     const float cum = a.scores[r];
     const int kind = (cum > -INFINITY ? 0 : 2) | (a.finished && a.finished[r] != 0 ? 1 : 0);
-    double off = -INFINITY;
+    double log_sum = -INFINITY;
     if (kind == 0) {
       const double* sums = a.sums + (size_t)r * a.splits;
       const float* tops = a.tops + (size_t)r * a.splits;
@@ -277,10 +277,10 @@ __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs 
         if (tops[s] > -INFINITY) sum += sums[s] * exp((double)tops[s] - (double)m);
 #pragma unroll
       for (int w = 1; w < 16; w *= 2) sum += __shfl_xor(sum, w, kWave);
-      if (m > -INFINITY) off = (double)cum - ((double)m + log(sum));
+      if (m > -INFINITY) log_sum = (double)m + log(sum);
     }
     if ((tid & 15) == 0) {
-      s_off[b] = off;
+      s_log[b] = log_sum;
       s_cum[b] = cum;
       s_kind[b] = (uint8_t)kind;
     }
@@ -305,8 +305,9 @@ __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs 
       return {score_key(kind == 1 && k == 0 ? (double)s_cum[b] : -INFINITY), first + (uint32_t)t};
     }
     if (stored == 0) return none;
+    // (the logit less the log sum first: beside a huge one, the beam's score would be lost)
     const float x = key_logit(stored);
-    return {score_key(x > -INFINITY ? (double)x + s_off[b] : -INFINITY), first + key_token(stored)};
+    return {score_key(x > -INFINITY ? (double)s_cum[b] + ((double)x - s_log[b]) : -INFINITY), first + key_token(stored)};
   };
   Scored held[kHeldCandidates];
 #pragma unroll
