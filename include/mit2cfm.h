@@ -644,8 +644,9 @@ mit2cfm_status mit2cfm_kv_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_ca
  * beam offers stop_token alone, at its unchanged score (its other candidates
  * count as -inf).  Candidates of -inf fill the list when others run out.
  * count = beams keeps a search going; 2 * beams leaves as many after stop
- * tokens are taken out.  Sums are fp64 of fp32 terms, candidates compared in
- * fp64 (where one beam's agree there, those of the larger logits are taken). */
+ * tokens are taken out.  Sums are fp64 of fp32 terms, scores formed as
+ * scores[b] + (logits[b][t] - log sum) and compared in fp64 (where one beam's
+ * agree there, the larger logit comes first). */
 typedef struct mit2cfm_beam_select {
   const void* logits; /* [groups * beams][vocab], rows logits_row elements apart */
   uint64_t logits_row;

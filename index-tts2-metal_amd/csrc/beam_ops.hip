@@ -226,12 +226,13 @@ __global__ __launch_bounds__(kSelectThreads) void select_rows_kernel(SelectArgs 
   }
 }
 
-// A candidate of a group: its score as a key that orders, its beam and token as
-// one number.
+// A candidate of a group: its score as a key that orders, and what orders equal
+// ones: the lower beam, its larger logit, the lower token (6, 32 and 24 bits).
 struct Scored {
-  uint64_t s;
-  uint32_t at;
+  uint64_t s, at;
   __device__ __forceinline__ bool over(const Scored& o) const { return s > o.s || (s == o.s && at < o.at); }
+  __device__ __forceinline__ int beam() const { return (int)(at >> 56); }
+  __device__ __forceinline__ int token() const { return (int)(at & 0xffffffu); }
 };
 __device__ __forceinline__ uint64_t score_key(double x) {
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
@@ -239,6 +240,9 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 }
 __device__ __forceinline__ double key_score(uint64_t k) {
   return __longlong_as_double((long long)((k >> 63) ? k & ~(1ull << 63) : ~k));
+}
+__device__ __forceinline__ Scored scored(double score, int beam, float logit, uint32_t token) {
+  return {score_key(score), (uint64_t)beam << 56 | (uint64_t)~float_key(logit) << 24 | token};
 }
 
 constexpr int kGroupList = 1024;
@@ -286,7 +290,7 @@ __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs 
     }
   }
   const int per = a.splits * a.count, n = a.beams * per;
-  const Scored none = {0, 0xffffffffu};
+  const Scored none = {0, ~0ull};
   const uint64_t* cand = a.cand + (size_t)g * n;
   // the stored keys of this thread's first candidates, asked for before the sums are known
   uint64_t key[kHeldCandidates];
@@ -298,16 +302,15 @@ __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs 
   __syncthreads();
   auto candidate = [&](int c, uint64_t stored) -> Scored {
     const int b = c / per, k = c - b * per, kind = s_kind[b];
-    const uint32_t first = (uint32_t)b * (uint32_t)a.vocab;
     if (kind != 0) {  // the lowest tokens at -inf; of a finished beam the stop token before them
       if (k >= a.count || k >= a.vocab) return none;
       const int t = kind & 2 ? k : k == 0 ? a.stop : k - 1 < a.stop ? k - 1 : k;
-      return {score_key(kind == 1 && k == 0 ? (double)s_cum[b] : -INFINITY), first + (uint32_t)t};
+      return scored(kind == 1 && k == 0 ? (double)s_cum[b] : -INFINITY, b, -INFINITY, (uint32_t)t);
     }
     if (stored == 0) return none;
     // (the logit less the log sum first: beside a huge one, the beam's score would be lost)
     const float x = key_logit(stored);
-    return {score_key(x > -INFINITY ? (double)s_cum[b] + ((double)x - s_log[b]) : -INFINITY), first + key_token(stored)};
+    return scored(x > -INFINITY ? (double)s_cum[b] + ((double)x - s_log[b]) : -INFINITY, b, x, key_token(stored));
   };
   Scored held[kHeldCandidates];
 #pragma unroll
@@ -322,7 +325,7 @@ __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs 
   };
   auto write = [&](const Scored& c, int rank) {
     const size_t at = (size_t)g * a.count + rank;
-    const int b = (int)(c.at / (uint32_t)a.vocab), t = (int)(c.at - (uint32_t)b * (uint32_t)a.vocab);
+    const int b = c.beam(), t = c.token();
     a.scores_out[at] = (float)key_score(c.s);
     a.parent_out[at] = b;
     a.token_out[at] = t;
@@ -365,7 +368,7 @@ __global__ __launch_bounds__(kGroupThreads) void select_group_kernel(SelectArgs 
     });
 #pragma unroll
     for (int off = 32; off; off >>= 1) {
-      const Scored o = {__shfl_xor((unsigned long long)next.s, off, kWave), (uint32_t)__shfl_xor((int)next.at, off, kWave)};
+      const Scored o = {__shfl_xor((unsigned long long)next.s, off, kWave), __shfl_xor((unsigned long long)next.at, off, kWave)};
       if (o.over(next)) next = o;
     }
     __syncthreads();

@@ -33,3 +33,15 @@ def test_a_beam_s_score_survives_infinite_and_huge_logits(mit2, ctx, dtype, voca
     got = _select(mit2, ctx, x.to(TORCH[dtype]), scores, 2, dtype=dtype)
     assert got[0][0].tolist() == [-0.5, -1.25] and got[1][0].tolist() == [2, 1] and got[2][0].tolist() == [7, 17]
     assert got[0][1].tolist() == [-0.125, -2.0] and got[1][1].tolist() == [0, 3] and got[2][1].tolist() == [3, 0]
+
+
+def test_equal_scores_of_one_beam_go_by_their_logits(mit2, ctx):  # noqa: F811
+    """Beside a logit of 1e30 all others of the beam score alike in 64 bits: the larger logits come first, of equal ones the lowest token, wherever
+    they lie in the row; and a beam's come before the next beam's."""
+    x = torch.zeros(1, 2, 12000)
+    x[0, :, 11999], x[0, :, 5000], x[0, :, 8500], x[0, :, 100] = 1e30, 2.0, 2.0, 1.0
+    for count in (2, 3, 4, 6, 9):
+        got = _select(mit2, ctx, x, np.array([[-1.0, -2.0]], np.float32), count)
+        assert got[2][0].tolist() == [11999, 11999, 5000, 8500, 100, 0, 1, 2, 3][:count], count
+        assert got[1][0].tolist() == [0, 1, 0, 0, 0, 0, 0, 0, 0][:count]
+        assert got[0][0].tolist() == [-1.0, -2.0] + [float(np.float32(-1e30))] * (count - 2)
