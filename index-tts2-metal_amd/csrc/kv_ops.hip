@@ -3,7 +3,6 @@
 #include "kv_ops.h"
 
 #include <algorithm>
-#include <climits>
 #include <cmath>
 #include <stdexcept>
 #include <string>
@@ -66,13 +65,14 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, int D) {
   __shared__ float2 turn[kMaxPairs];
   __shared__ int64_t s_at;  // element index of the row in its page, head 0; -1: not written
-  __shared__ int s_place;   // the row's position; INT_MIN: no sequence's row
+  __shared__ int s_place;   // the row's position
+  __shared__ int s_mine;    // the row is a sequence's
   const int tid = threadIdx.x, row = blockIdx.x;
   if (tid < 64) {
     const int seq = seq_of_row(a.r, row);
     if (tid == 0) {
       int64_t at = -1;
-      int pos = INT_MIN;
+      int pos = 0;
       if (seq >= 0) {
         const int place = a.r.length[seq] - (a.r.start[seq + 1] - row);
         if (place >= 0 && place < a.c.capacity()) {
@@ -80,14 +80,14 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a, in
           if (page >= 0) at = a.c.row_in(page, place, D);
         }
         pos = a.position ? a.position[row] : place;
-        if (pos == INT_MIN) pos = INT_MIN + 1;
       }
       s_at = at;
       s_place = pos;
+      s_mine = seq >= 0;
     }
   }
   __syncthreads();
-  if (s_place == INT_MIN) return;
+  if (!s_mine) return;
   const int half = a.rot >> 1;
   for (int p = tid; p < half; p += kAppendThreads) {
     const double inv = exp2(-2.0 * p / a.rot * a.log2_theta) * 0.15915494309189533577;  // 1 / (2 pi)
