@@ -592,7 +592,7 @@ typedef struct mit2cfm_kv_append {
   const void* v;
   uint64_t k_row, k_head, v_row, v_head;
   const void* q; /* [rows][q_heads][head_dim] by q_row, q_head; NULL: none */
-  void* q_out;   /* may be q itself, with its strides; no other overlap */
+  void* q_out;   /* may be q itself, with its strides; no other overlap with q, k or v, nor of its rows and heads */
   uint64_t q_row, q_head, q_out_row, q_out_head;
   uint32_t q_heads;        /* 0 .. 4096 */
   const int32_t* position; /* [rows]; NULL: a row's place in its sequence */
@@ -616,7 +616,7 @@ mit2cfm_status mit2cfm_kv_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache
  * with the probabilities rounded to the type. */
 typedef struct mit2cfm_kv_attention {
   const void* q; /* [rows][q_heads][head_dim] by q_row, q_head */
-  void* out;     /* the same by out_row, out_head; no overlap with q */
+  void* out;     /* the same by out_row, out_head; no overlap with q, nor of its rows and heads */
   uint64_t q_row, q_head, out_row, out_head;
   uint32_t q_heads; /* a multiple of kv_heads, <= 4096; rows * q_heads <= 2^28 */
   float scale;      /* finite */

@@ -11,6 +11,7 @@
 #include "device_common.h"
 #include "engine.h"
 #include "kv_ops.h"
+#include "overlap.h"
 
 namespace mit2hip {
 
@@ -508,8 +509,10 @@ void beam_select(const mit2cfm_beam_select& p, hipStream_t s) {
   need(p.logits && p.scores && p.scores_out && p.parent_out && p.token_out,
        "logits, scores, scores_out, parent_out and token_out must not be NULL");
   need(aligned(p.logits, (size_t)kv_elem_bytes(p.dtype)), "logits must be aligned to its type");
-  need(p.scores_out != p.scores && (!p.finished || p.finished_out != p.finished),
-       "scores_out must not be scores, nor finished_out finished");
+  const uint64_t in_bytes = (uint64_t)p.groups * p.beams * 4, out_bytes = (uint64_t)p.groups * p.count * 4;
+  need(!meet(p.scores, in_bytes, p.scores_out, out_bytes) &&
+           !(p.finished && p.finished_out && meet(p.finished, in_bytes, p.finished_out, out_bytes)),
+       "scores_out must not overlap scores, nor finished_out finished");
   need(aligned(p.scores, 4) && aligned(p.finished, 4) && aligned(p.scores_out, 4) && aligned(p.parent_out, 4) &&
            aligned(p.token_out, 4) && aligned(p.finished_out, 4),
        "scores, finished and the outputs must be 4-byte aligned");
@@ -555,9 +558,12 @@ void beam_reorder(const mit2cfm_kv_cache& c, const mit2cfm_beam_reorder& p, hipS
   need(p.parent_stride >= p.beams, "parent_stride must be >= beams");
   if (p.groups == 0) return;
   need(p.parent && p.length && p.table_out, "parent, length and table_out must not be NULL");
-  need(p.table_out != c.table, "table_out must not be the cache's table");
-  need(p.state == nullptr || (p.state_out && p.state_out != p.state && p.state_words >= 1 && p.state_words < (1u << 31)),
-       "state needs a state_out of its own and state_words in [1, 2^31)");
+  const uint64_t table_bytes = (uint64_t)p.groups * p.beams * c.table_stride * 4;
+  need(!meet(c.table, table_bytes, p.table_out, table_bytes), "table_out overlaps the cache's table");
+  need(p.state == nullptr || (p.state_out && p.state_words >= 1 && p.state_words < (1u << 31)),
+       "state needs a state_out and state_words in [1, 2^31)");
+  const uint64_t state_bytes = (uint64_t)p.groups * p.beams * p.state_words * 4;
+  need(p.state == nullptr || !meet(p.state, state_bytes, p.state_out, state_bytes), "state_out overlaps state");
   need(p.token == nullptr || (p.state && p.place), "token needs state and place");
   need(aligned(p.parent, 4) && aligned(p.length, 4) && aligned(p.table_out, 4) && aligned(p.state, 4) &&
            aligned(p.state_out, 4) && aligned(p.token, 4) && aligned(p.place, 4),

@@ -10,6 +10,7 @@
 #include "engine.h"
 #include "kv_attend.h"
 #include "kv_view.h"
+#include "overlap.h"
 
 namespace mit2hip {
 
@@ -237,11 +238,6 @@ bool attention_in_range(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uin
   return q_heads >= 1 && q_heads <= 4096 && q_heads % c.kv_heads == 0 && (uint64_t)r.rows * q_heads <= (1u << 28);
 }
 
-// An output's rows and heads must not lie on one another.
-void check_out(uint64_t row, uint64_t head, uint32_t rows, uint32_t heads, uint32_t D, const char* what) {
-  need((heads <= 1 || head >= D) && (rows <= 1 || row >= D), what);
-}
-
 }  // namespace
 
 void attend_launched(hipError_t e) { launched(e); }
@@ -285,9 +281,16 @@ void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cf
        "k, v, q and q_out must be aligned to their type");
   need(aligned(p.position, 4), "position must be 4-byte aligned");
   if (with_q) {
-    check_out(p.q_out_row, p.q_out_head, r.rows, p.q_heads, c.head_dim, "q_out's rows and heads overlap");
+    auto set = [&](const void* at, uint64_t row, uint64_t head, uint32_t heads) {
+      return pieces(at, row, head, r.rows, heads, c.head_dim, e);
+    };
+    const Pieces out = set(p.q_out, p.q_out_row, p.q_out_head, p.q_heads);
+    need(!meet_themselves(out), "q_out's rows and heads overlap");
     need(p.q != p.q_out || (p.q_row == p.q_out_row && p.q_head == p.q_out_head),
          "q_out may be q only with its strides");
+    need(p.q == p.q_out || !meet(set(p.q, p.q_row, p.q_head, p.q_heads), out), "q_out overlaps q");
+    need(!meet(set(p.k, p.k_row, p.k_head, c.kv_heads), out) && !meet(set(p.v, p.v_row, p.v_head, c.kv_heads), out),
+         "q_out overlaps k or v");
   }
   AppendArgs a;
   a.c = view(c);
@@ -340,7 +343,9 @@ void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit
   need(p.q && p.out && p.q != p.out, "q and out must not be NULL, nor the same");
   const size_t e = (size_t)kv_elem_bytes(c.dtype);
   need(aligned(p.q, e) && aligned(p.out, e), "q and out must be aligned to their type");
-  check_out(p.out_row, p.out_head, r.rows, p.q_heads, c.head_dim, "out's rows and heads overlap");
+  const Pieces out = pieces(p.out, p.out_row, p.out_head, r.rows, p.q_heads, c.head_dim, e);
+  need(!meet_themselves(out), "out's rows and heads overlap");
+  need(!meet(pieces(p.q, p.q_row, p.q_head, r.rows, p.q_heads, c.head_dim, e), out), "out overlaps q");
   const uint64_t bytes = kv_attention_workspace(c, r, p.q_heads);
   need(bytes == 0 || (p.workspace && p.workspace_bytes >= bytes), "workspace is NULL or too small");
   need(aligned(p.workspace, 16), "workspace must be 16-byte aligned");
