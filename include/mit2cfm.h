@@ -686,7 +686,7 @@ typedef struct mit2cfm_beam_reorder {
   uint32_t groups;        /* groups * beams <= 2^20 */
   uint32_t beams;         /* 1 .. 64 */
   uint32_t layers;        /* >= 1; the cache's k and v are the first's */
-  uint64_t layer_stride;  /* elements from a layer's k (v) to the next's: a multiple of 8 */
+  uint64_t layer_stride;  /* elements from a layer's k (v) to the next's: a multiple of 8, a layer's at least */
   const int32_t* parent;  /* [groups][beams], rows parent_stride apart */
   uint32_t parent_stride; /* >= beams */
   const int32_t* length;  /* [groups]: rows every beam of the group has cached */

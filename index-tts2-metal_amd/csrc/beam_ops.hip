@@ -555,6 +555,8 @@ void beam_reorder(const mit2cfm_kv_cache& c, const mit2cfm_beam_reorder& p, hipS
   need((uint64_t)p.groups * p.beams <= (1u << 20), "groups * beams must be <= 2^20");
   need(p.layers >= 1 && p.layers <= 16384, "layers must be in [1, 16384]");
   need(p.layers == 1 || p.layer_stride % 8 == 0, "layer_stride must be a multiple of 8");
+  need(p.layers == 1 || p.layer_stride >= (uint64_t)c.pages * c.kv_heads * c.page_rows * c.head_dim,
+       "layer_stride is smaller than a layer");
   need(p.parent_stride >= p.beams, "parent_stride must be >= beams");
   if (p.groups == 0) return;
   need(p.parent && p.length && p.table_out, "parent, length and table_out must not be NULL");

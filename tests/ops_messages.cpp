@@ -123,6 +123,7 @@ int main() {
   SELECT("finished_out finished", finished_out = at<int32_t>(10)) SELECT("finished_out finished", finished_out = at<int32_t>(10, 20))
   REORDER("table_out overlaps", table_out = at<int32_t>(0)) REORDER("table_out overlaps", table_out = at<int32_t>(0, 12))
   REORDER("state_out overlaps", state_out = at<uint32_t>(12)) REORDER("state_out overlaps", state = at<uint32_t>(13, 20))
+  REORDER("smaller than a layer", layer_stride = 504) REORDER("smaller than a layer", layer_stride = 8) REORDER("smaller than a layer", layer_stride = 0)
 
   // each other argument by itself
   CACHE("must not be NULL", k = nullptr) CACHE("must not be NULL", v = nullptr) CACHE("must not be NULL", table = nullptr)
