@@ -15,6 +15,7 @@
 #include <climits>
 #include <type_traits>
 
+#include "kv_plan.h"
 #include "kv_view.h"
 
 namespace mit2hip {
@@ -40,26 +41,10 @@ struct Parts {
   int32_t* n;
 };
 
-// How a launch is laid out (attend_plan, kv_ops.hip).
-struct AttendPlan {
-  int form;    // query tiles a wave (1, 2), kWide: the block kernel
-  int tiles;   // query tiles of the batch, an upper bound
-  int splits;  // of a sequence's keys, at most
-  int chunk;   // keys of a split, unless the sequence is longer than splits of them
-  int by_xcd;  // blocks of a key head and split on one XCD (see find_part)
-};
-constexpr int kWide = 0;
-// A split's keys are a multiple of this: a tile for each of a block's waves.
-constexpr int chunk_step(bool f32) { return f32 ? 64 : 128; }
-
 // Launches a plan's kernels; throws HipError.
 void launch_attend_f32(const AttendArgs& a, const AttendPlan& plan, int D, void* workspace, hipStream_t s);
 void launch_attend_f16(const AttendArgs& a, const AttendPlan& plan, int D, void* workspace, hipStream_t s);
 void launch_attend_bf16(const AttendArgs& a, const AttendPlan& plan, int D, void* workspace, hipStream_t s);
-
-// Query rows of the block kernel's tile, and the head sizes it is made for.
-constexpr int wide_rows(bool f32) { return f32 ? 64 : 128; }
-constexpr bool wide_dim(int D) { return D == 64 || D == 128; }
 
 #if defined(KV_ATTEND_KERNELS)
 
@@ -402,8 +387,6 @@ template <typename T>
 __device__ __forceinline__ float taken_out(T v) {
   return finite(v) ? 0.f : (float)v;
 }
-
-constexpr int kAttendWaves = 4, kAttendThreads = kAttendWaves * 64;
 
 // Few query rows: 16 MT of them a block, whose waves take every fourth tile of
 // the split's keys and join at the end.  Bound by the keys and values, which go
@@ -976,9 +959,8 @@ void launch_attend(const AttendArgs& a, const AttendPlan& plan, void* workspace,
   part.o = static_cast<float*>(workspace);
   part.ml = reinterpret_cast<float2*>(part.o + n * D);
   part.n = reinterpret_cast<int32_t*>(part.ml + n);
-  const int units = a.c.kv_heads * plan.splits;
-  const dim3 grid = plan.by_xcd ? dim3(8 * ((units + 7) / 8) * plan.tiles) : dim3(plan.tiles, units);
-  const dim3 block(kAttendThreads);
+  const AttendGrid g = attend_grid(plan, a.c.kv_heads);
+  const dim3 grid(g.x, g.y), block(kAttendThreads);
   const bool big = (1 << a.c.page_shift) >= Mat<T>::KT;
   auto tiles = [&](auto big_page) {
     constexpr bool BIG = decltype(big_page)::value;
