@@ -1670,15 +1670,14 @@ struct GptDecoder::Impl {
   // the step's buffers, all of it in two of what a selection reorders
   static constexpr int kBeamPage = 64;
   Arena bw;
-  int beam_cap[3] = {0, 0, 0};  // beams, cached rows, steps
-  int beam_entries = 0, beam_pages = 0, beams_held = 0, steps_held = 0;
+  int beam_entries = 0, beam_pages = 0;
   size_t beam_layer = 0;        // floats of a layer's keys (values)
-  BeamState* bst = nullptr;
+  BeamState* bst = nullptr;     // (these are laid out anew by each search)
   GptState* brow = nullptr;     // tells the row kernels how many rows there are
   float *bk = nullptr, *bv = nullptr, *bx, *bq, *batt, *bfc, *blogits, *new_k, *new_v, *bscore[2];
   int32_t *btable[2], *bdone[2];
   uint32_t* bhist[2];
-  void *battend = nullptr, *bselect = nullptr;
+  char *battend = nullptr, *bselect = nullptr;
   size_t battend_bytes = 0, bselect_bytes = 0;
 
   mit2cfm_kv_cache beam_cache(int l, int side) const {
@@ -1738,52 +1737,32 @@ struct GptDecoder::Impl {
     return a;
   }
 
+  // Lays the buffers out for a search of n beams, `rows` cached rows each and so many
+  // steps; what is held is enough if it has the bytes, whatever search it was for.
   void ensure_beams(int n, int rows, int steps) {
-    const int was[] = {beam_cap[0], beam_cap[1], beam_cap[2]};
-    beam_cap[0] = std::max(n, beam_cap[0]);
-    beam_cap[1] = std::max(rows, beam_cap[1]);
-    beam_cap[2] = std::max(steps, beam_cap[2]);
-    const int N = beam_cap[0], pages_before = beam_pages, entries = (beam_cap[1] + kBeamPage - 1) / kBeamPage;
-    // (what this call's plans need: the sizes' pointers do not matter)
-    BeamState none{};
-    BeamState* const held = bst;
-    bst = &none;
-    beam_entries = entries;
-    beam_pages = N * entries;
+    beam_entries = (rows + kBeamPage - 1) / kBeamPage;
+    beam_pages = n * beam_entries;
     beam_layer = (size_t)beam_pages * kBeamPage * kW;
-    const size_t attend_bytes = kv_attention_workspace(beam_cache(0, 0), beam_rows(n, rows), kHeads);
-    const size_t select_bytes = beam_select_workspace(beam_pick(n, 0));
-    bst = held;
-    const bool fits = held && beam_pages == pages_before && N == beams_held && beam_cap[2] == steps_held &&
-                      attend_bytes <= battend_bytes && select_bytes <= bselect_bytes;
-    if (fits) return;
-    beams_held = N;
-    steps_held = beam_cap[2];
-    battend_bytes = std::max(attend_bytes, battend_bytes);
-    bselect_bytes = std::max(select_bytes, bselect_bytes);
-    const size_t f = sizeof(float);
+    const size_t f = sizeof(float), N = (size_t)n, table = N * beam_entries * 4;
+    // (the sizes' pointers do not matter)
+    BeamState none{};
+    bst = &none;
+    battend_bytes = kv_attention_workspace(beam_cache(0, 0), beam_rows(n, rows), kHeads);
+    bselect_bytes = beam_select_workspace(beam_pick(n, 0));
+    bst = nullptr;
     const size_t sizes[] = {sizeof(BeamState), sizeof(GptState), (size_t)L * beam_layer * f, (size_t)L * beam_layer * f,
-                            (size_t)N * kW * f, (size_t)N * kW * f, (size_t)N * kW * f, (size_t)N * kMLP * f,
-                            (size_t)N * kVocab * f, (size_t)kPlainRows * kW * f, (size_t)kPlainRows * kW * f,
-                            (size_t)N * f, (size_t)N * f, (size_t)beam_pages * 4, (size_t)beam_pages * 4,
-                            (size_t)N * 4, (size_t)N * 4, (size_t)N * beam_cap[2] * 4, (size_t)N * beam_cap[2] * 4,
-                            battend_bytes, bselect_bytes};
+                            N * kW * f, N * kW * f, N * kW * f, N * kMLP * f, N * kVocab * f,
+                            (size_t)kPlainRows * kW * f, (size_t)kPlainRows * kW * f, N * f, N * f, table, table,
+                            N * 4, N * 4, N * steps * 4, N * steps * 4, battend_bytes, bselect_bytes};
     size_t total = 0;
     for (size_t b : sizes) total += align256(std::max<size_t>(b, 16));
-    bst = nullptr;  // (nothing is held should this fail)
-    try {
-      bw.reserve(total);
-    } catch (...) {
-      std::copy(was, was + 3, beam_cap);
-      throw;
-    }
+    if (total > bw.capacity()) bw.reserve(total);
+    bw.set_used(0);
     int i = 0;
     auto take = [&](auto*& p) { p = static_cast<std::remove_reference_t<decltype(p)>>(bw.take(std::max<size_t>(sizes[i++], 16))); };
     take(bst); take(brow); take(bk); take(bv); take(bx); take(bq); take(batt); take(bfc); take(blogits); take(new_k);
     take(new_v); take(bscore[0]); take(bscore[1]); take(btable[0]); take(btable[1]); take(bdone[0]); take(bdone[1]);
-    take(bhist[0]); take(bhist[1]);
-    battend = bw.take(std::max<size_t>(battend_bytes, 16));
-    bselect = bw.take(std::max<size_t>(bselect_bytes, 16));
+    take(bhist[0]); take(bhist[1]); take(battend); take(bselect);
   }
 
   // A step of n beams, whose tables, scores and histories are those of `side`;
