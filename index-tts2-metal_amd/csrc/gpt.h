@@ -85,7 +85,8 @@ class GptDecoder {
   // Beam search of up to `steps` tokens (no reference counterpart: its decoder
   // holds one sequence).  A hypothesis that takes the stop token stays in the
   // search with its score, the sum of its tokens' log probabilities; the search
-  // ends when all have.  The prefix is kept once, in pages that the beams share.
+  // ends when all have.  The prefix's rows are written once and its full pages read
+  // by all beams; memory is taken for beams x (prefix + steps) rows all the same.
   static constexpr int kMaxBeams = 8;
   struct Beams {
     std::vector<std::vector<uint32_t>> predicted;  // best first; the stop token included

@@ -1737,8 +1737,9 @@ struct GptDecoder::Impl {
     return a;
   }
 
-  // Lays the buffers out for a search of n beams, `rows` cached rows each and so many
-  // steps; what is held is enough if it has the bytes, whatever search it was for.
+  // Lays the buffers out for a search of n beams, pages for `rows` cached rows each (also
+  // of a prefix that they share) and so many steps; what is held is enough if it has the
+  // bytes, whatever search it was for.
   void ensure_beams(int n, int rows, int steps) {
     beam_entries = (rows + kBeamPage - 1) / kBeamPage;
     beam_pages = n * beam_entries;
