@@ -2127,6 +2127,30 @@ void GptDecoder::kv_beam(const float* prefix, int prefix_tokens, int steps, bool
   const int max_length = prefix_tokens + steps;
   d.ensure(prefix_tokens + 1, prefix_tokens + 1, 1);
   d.ensure_beams(beams, max_length, steps);
+  // Two steps, one from each side, replayed as a graph (made before the clock starts).
+  hipGraphExec_t pair = nullptr;
+  struct Drop {
+    hipGraphExec_t& g;
+    ~Drop() {
+      if (g) (void)hipGraphExecDestroy(g);
+    }
+  } drop{pair};
+  if (d.use_graph && steps >= kStepsPerCheck) {
+    hipGraph_t g = nullptr;
+    GPT_OK(hipStreamBeginCapture(d.s, hipStreamCaptureModeThreadLocal));
+    try {
+      d.enqueue_beams(beams, 0, hf, max_length, steps);
+      d.enqueue_beams(beams, 1, hf, max_length, steps);
+    } catch (...) {
+      (void)hipStreamEndCapture(d.s, &g);
+      if (g) (void)hipGraphDestroy(g);
+      throw;
+    }
+    GPT_OK(hipStreamEndCapture(d.s, &g));
+    const hipError_t err = hipGraphInstantiate(&pair, g, nullptr, nullptr, 0);
+    (void)hipGraphDestroy(g);
+    GPT_OK(err);
+  }
   GPT_OK(hipEventRecord(d.ev[0], d.s));
   if (prefix_tokens > 0) {  // the prefix through the layers, as generate() takes it
     GPT_OK(hipMemcpyAsync(d.rows, prefix, (size_t)prefix_tokens * kW * sizeof(float), hipMemcpyHostToDevice, d.s));
@@ -2190,30 +2214,6 @@ void GptDecoder::kv_beam(const float* prefix, int prefix_tokens, int steps, bool
   GPT_OK(hipEventRecord(d.ev[1], d.s));
   GPT_OK(hipStreamSynchronize(d.s));
 
-  // Two steps, one from each side, replayed as a graph.
-  hipGraphExec_t pair = nullptr;
-  struct Drop {
-    hipGraphExec_t& g;
-    ~Drop() {
-      if (g) (void)hipGraphExecDestroy(g);
-    }
-  } drop{pair};
-  if (d.use_graph && steps >= kStepsPerCheck) {
-    hipGraph_t g = nullptr;
-    GPT_OK(hipStreamBeginCapture(d.s, hipStreamCaptureModeThreadLocal));
-    try {
-      d.enqueue_beams(beams, 0, hf, max_length, steps);
-      d.enqueue_beams(beams, 1, hf, max_length, steps);
-    } catch (...) {
-      (void)hipStreamEndCapture(d.s, &g);
-      if (g) (void)hipGraphDestroy(g);
-      throw;
-    }
-    GPT_OK(hipStreamEndCapture(d.s, &g));
-    const hipError_t err = hipGraphInstantiate(&pair, g, nullptr, nullptr, 0);
-    (void)hipGraphDestroy(g);
-    GPT_OK(err);
-  }
   std::vector<int32_t> finished(beams);
   int done = 0;
   while (done < steps) {
