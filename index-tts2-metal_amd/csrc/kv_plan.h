@@ -27,12 +27,35 @@ constexpr int wide_rows(bool f32) { return f32 ? 64 : 128; }
 constexpr bool wide_dim(int D) { return D == 64 || D == 128; }
 
 constexpr int kBlocksWanted = 1024;   // four blocks of the small tiles a CU
-// Of the wide ones two fit a CU at 128 elements of 16 bits (by registers), else
-// three (by LDS).  More than those, as the last splits of shorter sequences are
-// short: trees of 63 over 4099 f16 keys take 72, 65, 87 us at 512, 640, 768, a
-// chain of 257 over 1201 f32 keys 43 at each.
-constexpr int wide_wanted(int D, bool f32) { return D == 128 && !f32 ? 640 : 768; }
+// Blocks of the wide form that run at once on 256 CUs: two a CU at 128 elements of
+// 16 bits (by registers), else three (by LDS).
+constexpr int wide_places(int D, bool f32) { return 256 * (D == 128 && !f32 ? 2 : 3); }
+// Keys of one of its buffers; a split's are a multiple of this.
+constexpr int wide_keys(int D, bool f32) { return 8192 / (D * (f32 ? 4 : 2)); }
 constexpr int kMostSplits = 128;
+
+// Splits of `len` keys for `blocks` wide blocks: those with which the rounds that the
+// blocks run in, times a block's keys, are least.  A block's begin and end (the
+// ring's fill, the last buffers' waits) count as four buffers, a join as four more.
+// (A fixed 640 for 512 places went in two rounds where the tiles' number is exact:
+// 63 rows of 32 heads on 8 of 128 f16 over 4099, 32768, 65536 keys took 41, 79, 128 us
+// so, 35, 67, 107 now; a prompt of 2047 in bf16 105, now 75; 30 sequences of 40 rows over
+// 2000 keys 108, now 92.  Of 8 ragged ones, whose shorter leave places free, it was
+// faster: 55, now 59.)
+inline uint64_t wide_splits(uint64_t blocks, uint64_t len, uint64_t places, uint64_t step, uint64_t most) {
+  uint64_t best = 1, least = ~uint64_t(0);
+  const uint64_t first = (blocks + places - 1) / places;  // rounds without a split
+  for (uint64_t r = first; r < first + 3; ++r) {
+    const uint64_t s = std::min(std::max<uint64_t>(1, r * places / blocks), most);
+    const uint64_t keys = ((len + s - 1) / s + step - 1) / step * step;
+    const uint64_t cost = (blocks * s + places - 1) / places * (keys + 4 * step) + (s > 1 ? 4 * step : 0);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
 
 inline AttendPlan attend_plan(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
   const int group = (int)(q_heads / c.kv_heads), D = (int)c.head_dim;
@@ -52,10 +75,19 @@ inline AttendPlan attend_plan(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& 
   const uint64_t by_fill = ((uint64_t)r.rows * group + (uint64_t)std::min(r.seqs, r.rows) * (mtile - 1)) / mtile;
   const uint64_t by_row = (uint64_t)r.rows * ((group + mtile - 1) / mtile);
   p.tiles = (int)std::min(by_fill, by_row);
-  const uint64_t blocks = (uint64_t)p.tiles * c.kv_heads, wanted = p.form == kWide ? wide_wanted(D, f32) : kBlocksWanted;
   const uint64_t len = std::max<uint64_t>(1, std::min<uint64_t>(r.max_length, (uint64_t)c.table_stride * c.page_rows));
-  const uint64_t step = chunk_step(f32), most = std::min<uint64_t>((len + step - 1) / step, kMostSplits);
-  const uint64_t splits = std::min<uint64_t>(most, (wanted + blocks - 1) / blocks);
+  const uint64_t step = p.form == kWide ? wide_keys(D, f32) : chunk_step(f32);
+  const uint64_t most = std::min<uint64_t>((len + chunk_step(f32) - 1) / chunk_step(f32), kMostSplits);
+  uint64_t splits;
+  if (p.form == kWide) {
+    // (as if the rows were spread evenly; of one sequence the number is exact)
+    const uint64_t each = ((uint64_t)r.rows + r.seqs - 1) / r.seqs;
+    const uint64_t even = std::min<uint64_t>(p.tiles, r.seqs * ((each * group + mtile - 1) / mtile));
+    splits = wide_splits(even * c.kv_heads, len, wide_places(D, f32), step, most);
+  } else {
+    const uint64_t blocks = (uint64_t)p.tiles * c.kv_heads;
+    splits = std::min<uint64_t>(most, (kBlocksWanted + blocks - 1) / blocks);
+  }
   p.chunk = (int)(((len + splits - 1) / splits + step - 1) / step * step);
   p.splits = (int)((len + p.chunk - 1) / p.chunk);
   const uint64_t units = (uint64_t)c.kv_heads * p.splits;

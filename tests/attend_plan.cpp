@@ -38,7 +38,31 @@ static void check(uint32_t dtype, uint32_t D, uint32_t kv_heads, uint32_t group,
   large += (uint64_t)p.tiles * units >= (uint64_t(1) << 24);
 }
 
+// One sequence's blocks, whose number is exact: how many rounds they run in, times a
+// block's keys, against the keys and tiles spread evenly over the chip.
+static void even(uint32_t dtype, uint32_t D, uint32_t kv_heads, uint32_t group, uint32_t rows, uint32_t length, uint64_t at_once, double most) {
+  mit2cfm_kv_cache c{};
+  c.dtype = (int32_t)dtype; c.head_dim = D; c.kv_heads = kv_heads; c.page_rows = 64; c.table_stride = length / 64 + 1; c.pages = 1;
+  mit2cfm_kv_rows r{};
+  r.seqs = 1; r.rows = rows; r.max_length = length;
+  const AttendPlan p = attend_plan(c, r, kv_heads * group);
+  const uint64_t mtile = dtype == MIT2CFM_DTYPE_F32 ? 64 : 128, tiles = ((uint64_t)rows * group + mtile - 1) / mtile;
+  const uint64_t blocks = tiles * kv_heads * p.splits, rounds = (blocks + at_once - 1) / at_once;
+  const double share = (double)tiles * kv_heads * length / at_once, longest = (double)rounds * p.chunk;
+  if (p.form != kWide || longest > most * share) {
+    std::printf("dtype %u D %u heads %u x %u rows %u length %u: %lu blocks of %d keys, %.2f of an even share\n", dtype, D, kv_heads, group, rows, length,
+                (unsigned long)blocks, p.chunk, longest / share);
+    ++bad;
+  }
+}
+
 int main() {
+  // long contexts of one sequence: within a tenth of an even share (two blocks of 128 elements of 16 bits a CU at once, else three)
+  even(MIT2CFM_DTYPE_F16, 128, 8, 4, 63, 32768, 512, 1.1);
+  even(MIT2CFM_DTYPE_BF16, 128, 8, 4, 63, 65536, 512, 1.1);
+  even(MIT2CFM_DTYPE_BF16, 128, 8, 4, 250, 65536, 512, 1.1);
+  even(MIT2CFM_DTYPE_F16, 64, 20, 1, 200, 65536, 768, 1.1);
+  even(MIT2CFM_DTYPE_F32, 64, 20, 1, 100, 40000, 768, 1.1);
   // as many blocks as the accepted sizes give: over 2^24, which one dimension of 256 threads each cannot hold
   check(MIT2CFM_DTYPE_F16, 128, 1024, 1, 15419, 262144, 16, 64, 1000);
   check(MIT2CFM_DTYPE_BF16, 128, 240, 1, 65535, 17 * 65535, 16, 64, 1000);
