@@ -612,8 +612,9 @@ mit2cfm_status mit2cfm_kv_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache
  * from the root); without a mask, when j <= i (one token, or a chain).  A row
  * that sees nothing, or only scores of -inf, gives 0.  What lies in places a
  * row does not see, NaN and infinities too, does not change it.  Sums and the
- * softmax are fp32; with 16-bit types the products run on the matrix cores,
- * with the probabilities rounded to the type. */
+ * softmax are fp32; with 16-bit types the products run on the matrix cores, the
+ * probabilities as a pair of that type where a sequence has up to 16 rows x query
+ * heads of a key head on average (tokens, short drafts), else rounded to it. */
 typedef struct mit2cfm_kv_attention {
   const void* q; /* [rows][q_heads][head_dim] by q_row, q_head */
   void* out;     /* the same by out_row, out_head; no overlap with q, nor of its rows and heads */

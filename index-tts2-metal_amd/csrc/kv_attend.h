@@ -257,8 +257,7 @@ __device__ __forceinline__ bool sees(const AttendArgs& a, const Query& x, int j,
 //
 // The maximum is raised only when a score passes it by kSlack (a wave-wide
 // vote): up to there the probabilities, at most 2^kSlack, stay exact in fp32 sums
-// and in range as 16-bit operands, where they round to the type, as the product
-// needs; the sum of the weights keeps fp32.
+// and in range as 16-bit operands (add_values); the sum of the weights keeps fp32.
 //
 // f16's weights are 2^7 times theirs throughout, the sum's too: with the slack up to
 // 2^15, in range, and normal down to 2^-21 of the largest.  (As they were, many
@@ -326,24 +325,41 @@ __device__ __forceinline__ void score_tile(const typename Mat<T>::op (&kv)[Dims<
     for (int e = 0; e < S::NV; ++e) s[e] = seen >> e & 1u ? s[e] : -INFINITY;
   }
 }
-// A tile's values, weighted, into the outputs of MT x 16 queries.
-template <typename T, int D, int MT>
+// A tile's values, weighted, into the outputs of MT x 16 queries.  16-bit operands
+// hold a weight rounded to the type; WHOLE: what that leaves off is a second product
+// (again rounded: 2^-16 of the weight in bf16, 2^-22 in f16), and errors against 64
+// bits are the result's rounding.  One query tile a wave waits for memory, and takes
+// it: 64 tokens over up to 8191 bf16 keys 297 us with it, 294 without, one over 131001
+// 103 and 102.  Two tiles do not (24 rows of 20 f16 heads of 64 over 3000 keys 39 us,
+// not 36), nor does the block form (trees of 63 rows over up to 4099 f16 keys 68, not
+// 59; a bf16 prompt of 2047 90, not 75).
+template <typename T, int D, int MT, bool WHOLE>
 __device__ __forceinline__ void add_values(const Piece<T, Dims<T, D>::DP> (&vv)[Dims<T, D>::NV],
                                            const float (&s)[MT][Dims<T, D>::NV], Running<T, D>* run) {
   typedef Dims<T, D> S;
   if constexpr (sizeof(T) == 2) {
-    typename Mat<T>::op p[MT];
+    typename Mat<T>::op p[MT], left[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[mt][e] = (T)s[mt][e];
+      for (int e = 0; e < 8; ++e) {
+        p[mt][e] = (T)s[mt][e];
+        if (WHOLE) left[mt][e] = (T)(s[mt][e] - (float)p[mt][e]);
+      }
 #pragma unroll
     for (int d = 0; d < S::DP; ++d) {
       typename Mat<T>::op v;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = vv[e].v[d];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) run[mt].o[d] = Mat<T>::mul(v, p[mt], run[mt].o[d]);
+      for (int mt = 0; mt < MT; ++mt) {
+        run[mt].o[d] = Mat<T>::mul(v, p[mt], run[mt].o[d]);
+        if (WHOLE) {  // (what is left, 0 or less, of an infinite value's weight is no part of it)
+          const floatx4 more = Mat<T>::mul(v, left[mt], run[mt].o[d]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) run[mt].o[d][r] = finite(more[r]) ? more[r] : run[mt].o[d][r];
+        }
+      }
     }
   } else {
 #pragma unroll
@@ -514,7 +530,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a, At
       score_tile<T, D>(kv, qv[mt], !all_there || fresh, seen, s[mt]);
       run[mt].weigh(s[mt], a.scale2);
     }
-    add_values<T, D, MT>(vv, s, run);
+    add_values<T, D, MT, MT == 1>(vv, s, run);
   }
 
   // the join: 16 rows at a time; thread -> row tid / 16, elements DP (tid % 16) ..
@@ -790,7 +806,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
           read_keys(bufK(B == 2 ? 0 : B + 1), kv);
         }
         __builtin_amdgcn_s_setprio(1);
-        add_values<T, D, WMT>(vv, s, run);
+        add_values<T, D, WMT, false>(vv, s, run);
       }
     };
     for (;;) {
@@ -835,7 +851,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
         dirty = dirty || odd;
       }
       run[mt].weigh(s[0], a.scale2);
-      add_values<T, D, 1>(vv, s, run + mt);
+      add_values<T, D, 1, false>(vv, s, run + mt);
     }
   };
   for (; b0 < p.end; buf = buf == 2 ? 0 : buf + 1) {
