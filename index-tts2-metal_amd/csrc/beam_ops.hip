@@ -421,7 +421,8 @@ constexpr int kReorderThreads = 512;
 // before it, and there are as many beams without children.
 //
 // Bound by the part pages' copies: 32 searches of 8 beams, 24 layers of 8 heads of 64
-// bf16, 135 MB in 30 us (4.5 TB/s).  Their stores go past the caches, whose lines the
+// bf16, 135 MB in 33 us a call (4.1 TB/s; the kernel 27 on pages that the last run
+// left in the caches).  Their stores go past the caches, whose lines the
 // pages' other bytes would come into first: 45 us with ordinary ones (and no loss to
 // the attention after, which reads far more than it finds there).  Three beams of 20
 // fp32 heads take 2.9 us, most of it four waits in a row (parents, length, table,

@@ -1768,7 +1768,7 @@ struct GptDecoder::Impl {
 
   // A step of n beams, whose tables, scores and histories are those of `side`;
   // the new ones go to the other.  Seven launches a layer, bound by them and by the
-  // weights: 1.27, 1.40, 1.81 ms with 1, 3, 8 beams behind a prefix of 150 rows (24
+  // weights: 1.26, 1.41, 1.80 ms with 1, 3, 8 beams behind a prefix of 150 rows (24
   // layers, as a graph).
   void enqueue_beams(int n, int side, bool hf, int max_length, int steps) {
     hipLaunchKernelGGL(beam_embed_kernel, dim3(n), dim3(320), 0, s, bst, hf ? 1 : 0, mel_emb, pos_emb, bx);

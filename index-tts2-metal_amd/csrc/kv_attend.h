@@ -410,7 +410,7 @@ __device__ __forceinline__ float taken_out(T v) {
 // BIG: a tile of keys lies in one page, whose entry is the same for all lanes.
 //
 // 64 tokens over up to 8191 bf16 keys of 8 heads of 128, in pages of 16: 1.52 GB in 288 us
-// (5.3 TB/s; a large copy reaches 4.7); one over 131001, 537 MB in 95 us (5.6).  Three
+// (5.3 TB/s; a large copy reaches 4.7); one over 131001, 537 MB in 96 us (5.6).  Three
 // tokens over 703 fp32 keys of 20 heads of 64 take 8.2 us, 5.6 of them the way to the
 // first key and from the last: sequence, page, keys, the join in LDS.
 template <typename T, int D, int MT, bool BIG>
@@ -616,13 +616,17 @@ __device__ __forceinline__ void load_to_lds(const void* src, lds_ptr_t* lds) {
 // waited for: about 2 us a buffer).  16-byte places of a row are exchanged by XOR
 // with the row's number, so that 16 rows' same place are read at once.
 //
-// Bound by its vector instructions (the weights: an exponential, a conversion and a
-// move into the operand of each score) and by the matrix cores behind them, which
-// two waves a SIMD overlap in part: trees of 63 rows, 32 query heads on 8 of 128,
-// over up to 4099 f16 keys take 57 us, 18 of vector and 8 of matrix instructions; a
-// ring of five buffers is 2.5% faster there and leaves no LDS, two buffers of twice
-// the keys, with half the barriers, are as fast.  A chain of 257 over
-// 1201 fp32 keys of 20 heads of 64 takes 40 us.
+// Where all blocks have as many keys it is bound by the SIMDs' issue: 63 rows of 32 query
+// heads on 8 of 128 over 65536 f16 keys take 102 us (665 TFLOP/s; 1.5 us a buffer of 32
+// keys of a CU's two blocks), of whose SIMD cycles 56% are vector instructions (the
+// weights: an exponential, a conversion and a move into the operand of each score) and
+// 38% matrix ones, which hardly overlap.  fp32, 100 rows of 20 heads of 64 over 8000
+// keys, 65 us: 24% and 72%.  Batches lose to their raggedness: blocks have the longest
+// sequence's keys, 33 buffers in 57 us for trees of up to 63 rows over up to 4099 f16
+// keys, where an even share is 22.8, and 23% of the tiles' rows are none; chains of 257
+// and 180 rows over 1201 and 841 fp32 keys 10 buffers in 41 us, an even share 6.6.  A ring
+// of five buffers was 2.5% faster on the trees and leaves no LDS, two buffers of
+// twice the keys, with half the barriers, as fast.
 //
 // The ring's buffers are objects of their own, named by constants in the usual
 // path: a read that might alias any of them would wait for every load.

@@ -19,7 +19,8 @@ struct AttendPlan {
 };
 constexpr int kWide = 0;
 constexpr int kAttendWaves = 4, kAttendThreads = kAttendWaves * 64;
-// A split's keys are a multiple of this: a tile for each of a block's waves.
+// A split of the small tiles is a multiple of this, a tile for each of a block's
+// waves; one of the block form has as many keys at least.
 constexpr int chunk_step(bool f32) { return f32 ? 64 : 128; }
 
 // Query rows of the block kernel's tile, and the head sizes it is made for.
