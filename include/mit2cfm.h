@@ -634,6 +634,23 @@ mit2cfm_status mit2cfm_kv_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_ca
                                            const mit2cfm_kv_rows* rows, const mit2cfm_kv_attention* attention,
                                            uint32_t flags);
 
+/* mit2cfm_kv_append with each query and key head normalised before it is rotated:
+ *   y = (x - c) / sqrt(mean((x - c)^2) + eps) * weight,  c = mean(x) when centered, else 0,
+ * over the head's head_dim elements, all in fp32; the result is rounded to the type
+ * once, after the rotation.  Squares that leave fp32's range do not matter.  Values
+ * go to their pages as they are. */
+typedef struct mit2cfm_kv_norm {
+  const void* q_weight; /* [q_heads][head_dim], heads q_weight_head elements apart (0: one for all); NULL: 1 */
+  const void* k_weight; /* [kv_heads][head_dim] by k_weight_head; no overlap of either with q_out */
+  uint64_t q_weight_head, k_weight_head;
+  int32_t weight_dtype; /* MIT2CFM_DTYPE_F32, or the cache's */
+  int32_t centered;
+  float eps;            /* 1e-20 .. 1e20 */
+} mit2cfm_kv_norm;
+mit2cfm_status mit2cfm_kv_norm_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                             const mit2cfm_kv_rows* rows, const mit2cfm_kv_append* append,
+                                             const mit2cfm_kv_norm* norm, uint32_t flags);
+
 /* ---- beam search --------------------------------------------------------------
  * (See the paged cache above for what holds of every call.)  groups searches
  * of `beams` hypotheses each. */

@@ -672,6 +672,13 @@ mit2cfm_status mit2cfm_kv_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache
                    [&](hipStream_t s) { mit2hip::kv_append(*cache, *rows, *append, s); });
 }
 
+mit2cfm_status mit2cfm_kv_norm_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                             const mit2cfm_kv_rows* rows, const mit2cfm_kv_append* append,
+                                             const mit2cfm_kv_norm* norm, uint32_t flags) {
+  return on_stream(ctx, flags, cache && rows && append && norm, "cache, rows, append and norm must not be NULL",
+                   [&](hipStream_t s) { mit2hip::kv_norm_append(*cache, *rows, *append, *norm, s); });
+}
+
 mit2cfm_status mit2cfm_kv_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
                                            const mit2cfm_kv_rows* rows, const mit2cfm_kv_attention* attention,
                                            uint32_t flags) {

@@ -9,9 +9,12 @@
 
 namespace mit2hip {
 
-// Both check their arguments (std::invalid_argument) and enqueue on s without
+// All check their arguments (std::invalid_argument) and enqueue on s without
 // waiting or allocating.
 void kv_append(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const mit2cfm_kv_append& a, hipStream_t s);
+// The same with normalised queries and keys (kv_norm.hip).
+void kv_norm_append(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const mit2cfm_kv_append& a,
+                    const mit2cfm_kv_norm& n, hipStream_t s);
 void kv_attention(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const mit2cfm_kv_attention& a,
                   hipStream_t s);
 // Bytes of kv_attention's workspace; 0: none needed, or an argument out of range.

@@ -5,9 +5,8 @@
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>
-#include <string>
 
-#include "engine.h"
+#include "kv_args.h"
 #include "kv_attend.h"
 #include "kv_view.h"
 #include "overlap.h"
@@ -16,39 +15,8 @@ namespace mit2hip {
 
 namespace {
 
-void need(bool ok, const char* what) {
-  if (!ok) throw std::invalid_argument(what);
-}
-void launched(hipError_t e) {
-  if (e != hipSuccess) throw HipError(std::string("kv operator launch: ") + hipGetErrorString(e));
-}
-bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-CacheView view(const mit2cfm_kv_cache& c) {
-  return {static_cast<char*>(c.k), static_cast<char*>(c.v), c.table, (int)c.pages,
-          __builtin_ctz(c.page_rows), (int)c.kv_heads, (int)c.table_stride};
-}
-RowView view(const mit2cfm_kv_rows& r) { return {r.start, r.length, (int)r.seqs, (int)r.rows}; }
-
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Vec {
-  T v[N];
-};
-
 // ------------------------------------------------------------------ append
 constexpr int kAppendThreads = 256;
-constexpr int kMaxPairs = 128;  // rotated pairs of a head
-
-struct AppendArgs {
-  CacheView c;
-  RowView r;
-  const char *k, *v, *q;
-  char* q_out;
-  int64_t k_row, k_head, v_row, v_head, q_row, q_head, qo_row, qo_head;
-  const int32_t* position;
-  int q_heads, rot, interleaved;
-  double log2_theta;
-};
 
 // A block takes a row's items (blockIdx.y: its share of them).  An item is two
 // vectors of VEC elements of a head, chosen so that a rotated pair's two
@@ -172,30 +140,19 @@ void launch_append_by(const AppendArgs& a, int D, hipStream_t s) {
   // few rows: their heads over more blocks, down to one item a thread
   const int by = std::max(1, std::min((items + kAppendThreads - 1) / kAppendThreads, 2048 / a.r.rows));
   hipLaunchKernelGGL((append_kernel<T, VEC>), dim3(a.r.rows, by), dim3(kAppendThreads), 0, s, a, D);
-  launched(hipGetLastError());
+  kv_launched(hipGetLastError());
 }
 
 template <typename T>
 void launch_append(const AppendArgs& a, int D, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  auto fits = [&](const void* p, int64_t row, int64_t head) { return aligned(p, 16) && row % V == 0 && head % V == 0; };
-  const bool wide = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head) &&
-                    (!a.q_heads || (fits(a.q, a.q_row, a.q_head) && fits(a.q_out, a.qo_row, a.qo_head))) &&
-                    (a.interleaved || a.rot % (2 * V) == 0);
-  if (wide)
+  if (append_wide(a, V))
     launch_append_by<T, V>(a, D, s);
   else
     launch_append_by<T, 1>(a, D, s);
 }
 
 // ------------------------------------------------------------------ attention
-void check_rows(const mit2cfm_kv_rows& r) {
-  need(r.seqs <= 65535, "seqs must be <= 65535");
-  need(r.rows < (1u << 24), "rows must be below 2^24");
-  need(r.seqs == 0 || r.rows == 0 || (r.start && r.length), "start and length must not be NULL");
-  need(aligned(r.start, 4) && aligned(r.length, 4), "start and length must be 4-byte aligned");
-}
-
 // What attend_plan's numbers, and the kernels' 32-bit ones of query rows, are made for.
 bool attention_in_range(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
   return q_heads >= 1 && q_heads <= 4096 && q_heads % c.kv_heads == 0 && (uint64_t)r.rows * q_heads <= (1u << 28);
@@ -203,7 +160,7 @@ bool attention_in_range(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uin
 
 }  // namespace
 
-void attend_launched(hipError_t e) { launched(e); }
+void attend_launched(hipError_t e) { kv_launched(e); }
 
 int kv_elem_bytes(int32_t dtype) { return dtype == MIT2CFM_DTYPE_F32 ? 4 : 2; }
 
@@ -229,13 +186,13 @@ void check_kv_cache(const mit2cfm_kv_cache& c) {
        "the cache's k and v must be 16-byte aligned, its table 4-byte aligned");
 }
 
-void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_append& p, hipStream_t s) {
+bool append_args(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_append& p, AppendArgs& a) {
   check_kv_cache(c);
-  check_rows(r);
+  check_kv_rows(r);
   need(p.q_heads <= 4096, "q_heads must be <= 4096");
   need(p.rotary_dim <= c.head_dim && p.rotary_dim % 2 == 0, "rotary_dim must be even and <= head_dim");
   need(p.rotary_dim == 0 || (p.theta > 0.0 && std::isfinite(p.theta)), "theta must be positive and finite");
-  if (r.seqs == 0 || r.rows == 0) return;
+  if (r.seqs == 0 || r.rows == 0) return false;
   const bool with_q = p.q != nullptr;
   need(p.k && p.v, "k and v must not be NULL");
   need(!with_q || (p.q_out && p.q_heads > 0), "q needs q_out and q_heads");
@@ -255,7 +212,6 @@ void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cf
     need(!meet(set(p.k, p.k_row, p.k_head, c.kv_heads), out) && !meet(set(p.v, p.v_row, p.v_head, c.kv_heads), out),
          "q_out overlaps k or v");
   }
-  AppendArgs a;
   a.c = view(c);
   a.r = view(r);
   a.k = static_cast<const char*>(p.k);
@@ -271,6 +227,12 @@ void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cf
   a.rot = (int)p.rotary_dim;
   a.interleaved = p.interleaved != 0;
   a.log2_theta = p.rotary_dim ? std::log2(p.theta) : 0.0;
+  return true;
+}
+
+void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_append& p, hipStream_t s) {
+  AppendArgs a;
+  if (!append_args(c, r, p, a)) return;
   const int D = (int)c.head_dim;
   if (c.dtype == MIT2CFM_DTYPE_F32)
     launch_append<float>(a, D, s);
@@ -283,7 +245,7 @@ void kv_append(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cf
 uint64_t kv_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
   try {
     check_kv_sizes(c);
-    check_rows(r);
+    check_kv_rows(r);
   } catch (const std::invalid_argument&) {
     return 0;
   }
@@ -295,7 +257,7 @@ uint64_t kv_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows
 
 void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, hipStream_t s) {
   check_kv_cache(c);
-  check_rows(r);
+  check_kv_rows(r);
   need(attention_in_range(c, r, p.q_heads),
        "q_heads must be a multiple of kv_heads, <= 4096, rows * q_heads <= 2^28");
   need(std::isfinite(p.scale), "scale must be finite");

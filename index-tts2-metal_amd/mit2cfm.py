@@ -138,6 +138,8 @@ def lib() -> ctypes.CDLL:
         "mit2cfm_kv_attention_workspace": (u64, [ctypes.POINTER(KvCache), ctypes.POINTER(KvRows), u32]),
         "mit2cfm_kv_append_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
                                           ctypes.POINTER(KvAppend), u32]),
+        "mit2cfm_kv_norm_append_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
+                                               ctypes.POINTER(KvAppend), ctypes.POINTER(KvNorm), u32]),
         "mit2cfm_kv_attention_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
                                              ctypes.POINTER(KvAttention), u32]),
         "mit2cfm_beam_select_workspace": (u64, [ctypes.POINTER(BeamSelect)]),
@@ -185,6 +187,13 @@ class KvAppend(ctypes.Structure):
                 ("q_out_row", ctypes.c_uint64), ("q_out_head", ctypes.c_uint64), ("q_heads", ctypes.c_uint32),
                 ("position", ctypes.c_void_p), ("rotary_dim", ctypes.c_uint32), ("interleaved", ctypes.c_int32),
                 ("theta", ctypes.c_double)]
+
+
+class KvNorm(ctypes.Structure):
+    """mit2cfm_kv_norm."""
+    _fields_ = [("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("q_weight_head", ctypes.c_uint64),
+                ("k_weight_head", ctypes.c_uint64), ("weight_dtype", ctypes.c_int32), ("centered", ctypes.c_int32),
+                ("eps", ctypes.c_float)]
 
 
 class KvAttention(ctypes.Structure):
@@ -824,6 +833,10 @@ class Context:
     def kv_append_device(self, cache: KvCache, rows: KvRows, append: KvAppend, sync: bool = False) -> None:
         """Appends new rows' keys (rotated) and values to a paged cache and rotates their queries."""
         self._c(lib().mit2cfm_kv_append_device(self._h, cache, rows, append, FLAG_SYNC if sync else 0))
+
+    def kv_norm_append_device(self, cache: KvCache, rows: KvRows, append: KvAppend, norm: KvNorm, sync: bool = False) -> None:
+        """kv_append_device with each query and key head normalised before its rotation."""
+        self._c(lib().mit2cfm_kv_norm_append_device(self._h, cache, rows, append, norm, FLAG_SYNC if sync else 0))
 
     def kv_attention_device(self, cache: KvCache, rows: KvRows, attention: KvAttention, sync: bool = False) -> None:
         """Attention of new rows (tokens, chains, trees) over their sequences' paged caches."""
