@@ -651,6 +651,34 @@ mit2cfm_status mit2cfm_kv_norm_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_
                                              const mit2cfm_kv_rows* rows, const mit2cfm_kv_append* append,
                                              const mit2cfm_kv_norm* norm, uint32_t flags);
 
+/* The attention weight that cached rows get, added up: for key head h of every sequence s that
+ * has new rows, and each of its cached rows j,
+ *   weights_out[s][h][j] = decay * weights[s][h][j] + sum exp(scale * q . k_j - lse)
+ * over the new rows (the last last_rows of them) that see j and the query heads of h; where j
+ * is new itself, and had no weight, without the first term.  Who sees what: as for
+ * mit2cfm_kv_attention.  lse is mit2cfm_kv_prefix_attention's; a row of -inf adds nothing.
+ * Places without a page get the first term alone; places from a sequence's length on, and
+ * sequences without new rows, are left alone.  Sums are fp32, in the same order each time. */
+typedef struct mit2cfm_kv_weigh {
+  const void* q; /* [rows][q_heads][head_dim] by q_row, q_head */
+  uint64_t q_row, q_head;
+  uint32_t q_heads; /* a multiple of kv_heads, <= 4096; rows * q_heads <= 2^28 */
+  float scale;      /* finite */
+  const uint32_t* mask;
+  uint32_t mask_words;
+  uint32_t last_rows;       /* 0: all */
+  const float* lse;         /* [rows][q_heads] */
+  const float* weights;     /* [seqs][kv_heads][weight_stride] */
+  float* weights_out;       /* may be weights itself; no other overlap with weights, q, lse or mask */
+  uint32_t weight_stride;   /* places that are counted: what lies past them is not.  1 .. 2^30 */
+  float decay;              /* finite */
+  const int32_t* position;  /* [rows]; NULL: a row's place.  Used with born alone */
+  int32_t* born;            /* [seqs][kv_heads][weight_stride]: new rows' places get their positions; NULL: none.
+                             * No overlap with the other buffers */
+} mit2cfm_kv_weigh;
+mit2cfm_status mit2cfm_kv_weigh_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache, const mit2cfm_kv_rows* rows,
+                                       const mit2cfm_kv_weigh* weigh, uint32_t flags);
+
 /* ---- beam search --------------------------------------------------------------
  * (See the paged cache above for what holds of every call.)  groups searches
  * of `beams` hypotheses each. */

@@ -686,6 +686,12 @@ mit2cfm_status mit2cfm_kv_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_ca
                    [&](hipStream_t s) { mit2hip::kv_attention(*cache, *rows, *attention, s); });
 }
 
+mit2cfm_status mit2cfm_kv_weigh_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache, const mit2cfm_kv_rows* rows,
+                                       const mit2cfm_kv_weigh* weigh, uint32_t flags) {
+  return on_stream(ctx, flags, cache && rows && weigh, "cache, rows and weigh must not be NULL",
+                   [&](hipStream_t s) { mit2hip::kv_weigh(*cache, *rows, *weigh, s); });
+}
+
 uint64_t mit2cfm_beam_select_workspace(const mit2cfm_beam_select* select) {
   return select ? mit2hip::beam_select_workspace(*select) : 0;
 }

@@ -2,10 +2,13 @@
 // the host: refusals, the kernels' views of a cache and its rows, launch errors.
 #pragma once
 
+#include <algorithm>
+#include <cmath>
 #include <stdexcept>
 #include <string>
 
 #include "engine.h"
+#include "kv_attend.h"
 #include "kv_ops.h"
 #include "kv_view.h"
 #include "overlap.h"
@@ -32,6 +35,17 @@ inline void check_kv_rows(const mit2cfm_kv_rows& r) {
   need(r.seqs == 0 || r.rows == 0 || (r.start && r.length), "start and length must not be NULL");
   need(aligned(r.start, 4) && aligned(r.length, 4), "start and length must be 4-byte aligned");
 }
+
+// What the attention's plans, and the kernels' 32-bit numbers of query rows, are made for.
+inline bool query_rows_in_range(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
+  return q_heads >= 1 && q_heads <= 4096 && q_heads % c.kv_heads == 0 && (uint64_t)r.rows * q_heads <= (1u << 28);
+}
+inline void set_scale(AttendArgs& a, float scale) {
+  a.flip = scale < 0.f;
+  a.scale2 = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-37f);  // (0: masked scores stay -inf)
+}
+// A plain range among sets of pieces.
+inline Pieces whole(const void* at, uint64_t bytes) { return {at, 0, 0, 1, 1, bytes}; }
 
 // What an append's kernels take (kv_ops.hip, kv_norm.hip).
 struct AppendArgs {

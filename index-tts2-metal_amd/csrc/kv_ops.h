@@ -17,6 +17,8 @@ void kv_norm_append(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, 
                     const mit2cfm_kv_norm& n, hipStream_t s);
 void kv_attention(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const mit2cfm_kv_attention& a,
                   hipStream_t s);
+// Adds up the attention weight that cached rows get (kv_weigh.hip).
+void kv_weigh(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const mit2cfm_kv_weigh& w, hipStream_t s);
 // Bytes of kv_attention's workspace; 0: none needed, or an argument out of range.
 uint64_t kv_attention_workspace(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, uint32_t q_heads);
 

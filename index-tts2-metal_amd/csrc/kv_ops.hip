@@ -152,12 +152,6 @@ void launch_append(const AppendArgs& a, int D, hipStream_t s) {
     launch_append_by<T, 1>(a, D, s);
 }
 
-// ------------------------------------------------------------------ attention
-// What attend_plan's numbers, and the kernels' 32-bit ones of query rows, are made for.
-bool attention_in_range(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
-  return q_heads >= 1 && q_heads <= 4096 && q_heads % c.kv_heads == 0 && (uint64_t)r.rows * q_heads <= (1u << 28);
-}
-
 }  // namespace
 
 void attend_launched(hipError_t e) { kv_launched(e); }
@@ -249,7 +243,7 @@ uint64_t kv_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows
   } catch (const std::invalid_argument&) {
     return 0;
   }
-  if (r.seqs == 0 || r.rows == 0 || !attention_in_range(c, r, q_heads)) return 0;
+  if (r.seqs == 0 || r.rows == 0 || !query_rows_in_range(c, r, q_heads)) return 0;
   const AttendPlan plan = attend_plan(c, r, q_heads);
   if (plan.splits == 1) return 0;
   return (uint64_t)r.rows * q_heads * (plan.splits * (uint64_t)(c.head_dim + 2) + 1) * sizeof(float);
@@ -258,7 +252,7 @@ uint64_t kv_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows
 void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, hipStream_t s) {
   check_kv_cache(c);
   check_kv_rows(r);
-  need(attention_in_range(c, r, p.q_heads),
+  need(query_rows_in_range(c, r, p.q_heads),
        "q_heads must be a multiple of kv_heads, <= 4096, rows * q_heads <= 2^28");
   need(std::isfinite(p.scale), "scale must be finite");
   need(p.mask == nullptr || p.mask_words >= 1, "mask_words must be >= 1 with a mask");
@@ -285,8 +279,7 @@ void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit
   a.mask_words = p.mask ? (int)p.mask_words : 0;
   a.q_heads = (int)p.q_heads;
   a.group = (int)(p.q_heads / c.kv_heads);
-  a.flip = p.scale < 0.f;
-  a.scale2 = std::max(std::fabs(p.scale) * 1.4426950408889634f, 1e-37f);  // (0: masked scores stay -inf)
+  set_scale(a, p.scale);
   a.q_wide = aligned(p.q, 16) && p.q_row % 8 == 0 && p.q_head % 8 == 0;
   a.o_wide = aligned(p.out, 16) && p.out_row % 8 == 0 && p.out_head % 8 == 0;
   const int D = (int)c.head_dim;

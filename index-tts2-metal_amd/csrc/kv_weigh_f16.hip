@@ -1,0 +1,11 @@
+// kv_weigh_f16.hip -- the added-up attention weights' kernels for f16 caches (kv_weigh.h).
+#define KV_ATTEND_KERNELS
+#include "kv_weigh.h"
+
+namespace mit2hip {
+
+void launch_weigh_f16(const WeighArgs& w, const WeighPlan& plan, int D, hipStream_t s) {
+  launch_weigh_dim<half_t>(w, plan, D, s);
+}
+
+}  // namespace mit2hip

@@ -142,6 +142,7 @@ def lib() -> ctypes.CDLL:
                                                ctypes.POINTER(KvAppend), ctypes.POINTER(KvNorm), u32]),
         "mit2cfm_kv_attention_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
                                              ctypes.POINTER(KvAttention), u32]),
+        "mit2cfm_kv_weigh_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows), ctypes.POINTER(KvWeigh), u32]),
         "mit2cfm_beam_select_workspace": (u64, [ctypes.POINTER(BeamSelect)]),
         "mit2cfm_beam_select_device": (st, [vp, ctypes.POINTER(BeamSelect), u32]),
         "mit2cfm_beam_reorder_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(BeamReorder), u32]),
@@ -202,6 +203,15 @@ class KvAttention(ctypes.Structure):
                 ("out_row", ctypes.c_uint64), ("out_head", ctypes.c_uint64), ("q_heads", ctypes.c_uint32),
                 ("scale", ctypes.c_float), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_uint32),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class KvWeigh(ctypes.Structure):
+    """mit2cfm_kv_weigh."""
+    _fields_ = [("q", ctypes.c_void_p), ("q_row", ctypes.c_uint64), ("q_head", ctypes.c_uint64), ("q_heads", ctypes.c_uint32),
+                ("scale", ctypes.c_float), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_uint32),
+                ("last_rows", ctypes.c_uint32), ("lse", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+                ("weights_out", ctypes.c_void_p), ("weight_stride", ctypes.c_uint32), ("decay", ctypes.c_float),
+                ("position", ctypes.c_void_p), ("born", ctypes.c_void_p)]
 
 
 class BeamSelect(ctypes.Structure):
@@ -841,6 +851,10 @@ class Context:
     def kv_attention_device(self, cache: KvCache, rows: KvRows, attention: KvAttention, sync: bool = False) -> None:
         """Attention of new rows (tokens, chains, trees) over their sequences' paged caches."""
         self._c(lib().mit2cfm_kv_attention_device(self._h, cache, rows, attention, FLAG_SYNC if sync else 0))
+
+    def kv_weigh_device(self, cache: KvCache, rows: KvRows, weigh: KvWeigh, sync: bool = False) -> None:
+        """Adds the attention weight that new rows give to cached ones."""
+        self._c(lib().mit2cfm_kv_weigh_device(self._h, cache, rows, weigh, FLAG_SYNC if sync else 0))
 
     def beam_select_device(self, select: BeamSelect, sync: bool = False) -> None:
         """The best continuations of every group's beams."""

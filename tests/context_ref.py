@@ -104,3 +104,68 @@ def norm_append64(b, q_weight, k_weight, eps, centered, position, rot, interleav
             k[page, :, at], kt[page, :, at] = one(b.new_k[row], k_weight)
             v[page, :, at] = b.new_v[row].double()
     return q, qt, k, kt, v
+
+
+# ------------------------------------------------------------------ attention weights
+def seen(b, row, s, i, before, mask):
+    """Cached places that a new row sees: [(place, page, slot)]."""
+    at = []
+    for j in range(max(0, b.length[s])):
+        n = j - before
+        if n >= 0 and (n > i if mask is None else not (n < 32 * mask.shape[1] and mask[row, n // 32] >> np.uint32(n % 32) & 1)):
+            continue
+        page = b.page_of(s, j)
+        if page >= 0:
+            at.append((j, page, j % b.page))
+    return at
+
+
+def lse64(b, scale, mask=None):
+    """log sum exp of each row's scores [rows][q_heads] in float64: -inf where it sees nothing, NaN for rows of no sequence."""
+    out = torch.full(b.q.shape[:2], math.nan, dtype=torch.float64)
+    group = b.q_heads // b.kv_heads
+    for row, s, i, before in b.each_row():
+        at = seen(b, row, s, i, before, mask)
+        if not at:
+            out[row] = -math.inf
+            continue
+        _, pages, slots = (torch.tensor(x) for x in zip(*at))
+        for h in range(b.kv_heads):
+            z = b.q[row, h * group: (h + 1) * group].double() @ b.k[pages, h, slots].double().t() * scale
+            out[row, h * group: (h + 1) * group] = torch.logsumexp(z, -1)
+    return out
+
+
+def weigh64(b, lse, weights, scale, mask=None, decay=1.0, last=0):
+    """(weights_out, its tolerance) in float64; lse [rows][q_heads] and weights [seqs][kv_heads][stride] fp32.
+
+    An exponential's argument is off by the score's error (dim products and sums, the scale) and by the roundings of it and of lse
+    in powers of two; its value by one more.  Then the fp32 sums over rows and query heads, and the product and sum with the old."""
+    out, tol = weights.double().clone(), torch.zeros(weights.shape, dtype=torch.float64)
+    stride, group = weights.shape[2], b.q_heads // b.kv_heads
+    decay = float(np.float32(decay))
+    for s, n in enumerate(b.new):
+        if n == 0:
+            continue
+        first = b.length[s] - n
+        places = min(b.length[s], stride, b.table.shape[1] * b.page)
+        for j in range(max(0, places)):
+            out[s, :, j] = out[s, :, j] * decay if j < first else 0.0
+        tol[s] = 3 * U * out[s].abs()
+        tol[s, :, max(0, places):] = 0.0
+    for row, s, i, before in b.each_row():
+        if last and i < b.new[s] - last:
+            continue
+        at = [x for x in seen(b, row, s, i, before, mask) if x[0] < stride]
+        if not at:
+            continue
+        places, pages, slots = (torch.tensor(x) for x in zip(*at))
+        for h in range(b.kv_heads):
+            k = b.k[pages, h, slots].double()
+            q = b.q[row, h * group: (h + 1) * group].double()
+            z, l = q @ k.t() * scale, lse[row, h * group: (h + 1) * group].double()[:, None]
+            p = torch.where(l == -math.inf, 0.0, torch.exp(z - l))
+            rel = (b.dim + 4) * U * abs(scale) * (q.abs() @ k.abs().t()) + 4 * U * (z.abs() + l.abs().nan_to_num(posinf=0.0)) + 8 * U
+            out[s, h, places] += p.sum(0)
+            tol[s, h, places] += (p * 1.01 * (rel + (b.new[s] * group + 8) * U)).sum(0) + group * 2.0 ** -120
+    return out, tol
