@@ -679,6 +679,40 @@ typedef struct mit2cfm_kv_weigh {
 mit2cfm_status mit2cfm_kv_weigh_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache, const mit2cfm_kv_rows* rows,
                                        const mit2cfm_kv_weigh* weigh, uint32_t flags);
 
+/* Rows of least weight leave the caches of all layers, each key head choosing its own.
+ * Of a sequence's n = length[s] rows, min(n, keep[s]) stay: the first first_rows places
+ * before all, and with them the youngest (with born: those of born >= now[s] - last_rows,
+ * else the last last_rows places), then the others by weight, the largest first, of equal
+ * ones the lowest place first (a NaN counts as less than all, and so does a place without a
+ * page; a row that moves to one is lost).  The rows that stay from place keep[s] on move down: the i-th of them in order goes to the
+ * i-th place below keep[s] that a row left.  Everything else stays where it is, so places
+ * tell ages no more: give born where a cache is cut again and again.  Keys keep the
+ * rotation they were appended with; new rows are appended at positions of the caller's.
+ * Pages that sequences share must lie below first_rows (others are written to). */
+typedef struct mit2cfm_kv_evict {
+  uint32_t seqs;           /* 0 .. 65535 */
+  uint32_t layers;         /* >= 1; the cache's k and v are the first's; layers * seqs * kv_heads <= 2^24 */
+  uint64_t layer_stride;   /* elements from a layer's k (v) to the next's: a multiple of 8, a layer's at least */
+  const int32_t* length;   /* [seqs] */
+  const int32_t* keep;     /* [seqs]; negative counts as 0 */
+  uint32_t first_rows;
+  uint32_t last_rows;
+  uint32_t max_length;     /* about the largest length: the work is split by it (any value is right) */
+  const float* weights;    /* [layers][seqs][kv_heads][weight_stride] */
+  float* weights_out;      /* places below the new length; may be weights itself, no other overlap */
+  uint32_t weight_stride;  /* 1 .. 2^30; a length past it (or the table) counts as it */
+  const int32_t* born;     /* as weights; NULL: none */
+  int32_t* born_out;       /* as weights_out, with born */
+  const int32_t* now;      /* [seqs], with born: the position that the sequence's next row will have */
+  int32_t* length_out;     /* [seqs]: min(n, keep); may be length itself, no other overlap */
+  void* workspace;         /* 16-byte aligned, of mit2cfm_kv_evict_workspace bytes; calls that may run at
+                            * the same time need one each */
+  uint64_t workspace_bytes;
+} mit2cfm_kv_evict;
+uint64_t mit2cfm_kv_evict_workspace(const mit2cfm_kv_cache* cache, const mit2cfm_kv_evict* evict); /* 0: an argument out of range */
+mit2cfm_status mit2cfm_kv_evict_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache, const mit2cfm_kv_evict* evict,
+                                       uint32_t flags);
+
 /* ---- beam search --------------------------------------------------------------
  * (See the paged cache above for what holds of every call.)  groups searches
  * of `beams` hypotheses each. */

@@ -692,6 +692,16 @@ mit2cfm_status mit2cfm_kv_weigh_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache*
                    [&](hipStream_t s) { mit2hip::kv_weigh(*cache, *rows, *weigh, s); });
 }
 
+uint64_t mit2cfm_kv_evict_workspace(const mit2cfm_kv_cache* cache, const mit2cfm_kv_evict* evict) {
+  return cache && evict ? mit2hip::kv_evict_workspace(*cache, *evict) : 0;
+}
+
+mit2cfm_status mit2cfm_kv_evict_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache, const mit2cfm_kv_evict* evict,
+                                       uint32_t flags) {
+  return on_stream(ctx, flags, cache && evict, "cache and evict must not be NULL",
+                   [&](hipStream_t s) { mit2hip::kv_evict(*cache, *evict, s); });
+}
+
 uint64_t mit2cfm_beam_select_workspace(const mit2cfm_beam_select* select) {
   return select ? mit2hip::beam_select_workspace(*select) : 0;
 }

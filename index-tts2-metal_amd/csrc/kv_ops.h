@@ -22,8 +22,14 @@ void kv_weigh(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const 
 // Bytes of kv_attention's workspace; 0: none needed, or an argument out of range.
 uint64_t kv_attention_workspace(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, uint32_t q_heads);
 
-// Whether a cache's sizes, type and pointers are within their ranges (throws
-// std::invalid_argument otherwise); bytes of an element.
+// Rows of least weight leave the caches of all layers (kv_evict.hip); the bytes of its
+// workspace, 0: an argument out of range.
+void kv_evict(const mit2cfm_kv_cache& cache, const mit2cfm_kv_evict& e, hipStream_t s);
+uint64_t kv_evict_workspace(const mit2cfm_kv_cache& cache, const mit2cfm_kv_evict& e);
+
+// Whether a cache's sizes and type, and its pointers too, are within their ranges
+// (throw std::invalid_argument otherwise); bytes of an element.
+void check_kv_sizes(const mit2cfm_kv_cache& c);
 void check_kv_cache(const mit2cfm_kv_cache& cache);
 int kv_elem_bytes(int32_t dtype);
 

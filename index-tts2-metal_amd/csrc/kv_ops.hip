@@ -158,7 +158,6 @@ void attend_launched(hipError_t e) { kv_launched(e); }
 
 int kv_elem_bytes(int32_t dtype) { return dtype == MIT2CFM_DTYPE_F32 ? 4 : 2; }
 
-namespace {
 void check_kv_sizes(const mit2cfm_kv_cache& c) {
   need(c.dtype >= MIT2CFM_DTYPE_F32 && c.dtype <= MIT2CFM_DTYPE_BF16, "the cache's dtype must be f32, f16 or bf16");
   need(c.page_rows >= 1 && c.page_rows <= 1024 && (c.page_rows & (c.page_rows - 1)) == 0,
@@ -171,7 +170,6 @@ void check_kv_sizes(const mit2cfm_kv_cache& c) {
   need(c.table_stride >= 1 && (uint64_t)c.table_stride * c.page_rows <= (1u << 30),
        "table_stride must be >= 1, page_rows * table_stride <= 2^30");
 }
-}  // namespace
 
 void check_kv_cache(const mit2cfm_kv_cache& c) {
   check_kv_sizes(c);

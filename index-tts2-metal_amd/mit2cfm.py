@@ -143,6 +143,8 @@ def lib() -> ctypes.CDLL:
         "mit2cfm_kv_attention_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
                                              ctypes.POINTER(KvAttention), u32]),
         "mit2cfm_kv_weigh_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows), ctypes.POINTER(KvWeigh), u32]),
+        "mit2cfm_kv_evict_workspace": (u64, [ctypes.POINTER(KvCache), ctypes.POINTER(KvEvict)]),
+        "mit2cfm_kv_evict_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvEvict), u32]),
         "mit2cfm_beam_select_workspace": (u64, [ctypes.POINTER(BeamSelect)]),
         "mit2cfm_beam_select_device": (st, [vp, ctypes.POINTER(BeamSelect), u32]),
         "mit2cfm_beam_reorder_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(BeamReorder), u32]),
@@ -214,6 +216,16 @@ class KvWeigh(ctypes.Structure):
                 ("position", ctypes.c_void_p), ("born", ctypes.c_void_p)]
 
 
+class KvEvict(ctypes.Structure):
+    """mit2cfm_kv_evict."""
+    _fields_ = [("seqs", ctypes.c_uint32), ("layers", ctypes.c_uint32), ("layer_stride", ctypes.c_uint64),
+                ("length", ctypes.c_void_p), ("keep", ctypes.c_void_p), ("first_rows", ctypes.c_uint32),
+                ("last_rows", ctypes.c_uint32), ("max_length", ctypes.c_uint32), ("weights", ctypes.c_void_p),
+                ("weights_out", ctypes.c_void_p), ("weight_stride", ctypes.c_uint32), ("born", ctypes.c_void_p),
+                ("born_out", ctypes.c_void_p), ("now", ctypes.c_void_p), ("length_out", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
 class BeamSelect(ctypes.Structure):
     """mit2cfm_beam_select."""
     _fields_ = [("logits", ctypes.c_void_p), ("logits_row", ctypes.c_uint64), ("dtype", ctypes.c_int32),
@@ -236,6 +248,11 @@ class BeamReorder(ctypes.Structure):
 def kv_attention_workspace(cache: KvCache, rows: KvRows, q_heads: int) -> int:
     """Bytes of workspace that Context.kv_attention_device needs for these sizes."""
     return int(lib().mit2cfm_kv_attention_workspace(ctypes.byref(cache), ctypes.byref(rows), q_heads))
+
+
+def kv_evict_workspace(cache: KvCache, evict: KvEvict) -> int:
+    """Bytes of workspace that Context.kv_evict_device needs for these sizes."""
+    return int(lib().mit2cfm_kv_evict_workspace(ctypes.byref(cache), ctypes.byref(evict)))
 
 
 def beam_select_workspace(select: BeamSelect) -> int:
@@ -855,6 +872,10 @@ class Context:
     def kv_weigh_device(self, cache: KvCache, rows: KvRows, weigh: KvWeigh, sync: bool = False) -> None:
         """Adds the attention weight that new rows give to cached ones."""
         self._c(lib().mit2cfm_kv_weigh_device(self._h, cache, rows, weigh, FLAG_SYNC if sync else 0))
+
+    def kv_evict_device(self, cache: KvCache, evict: KvEvict, sync: bool = False) -> None:
+        """Rows of least weight leave the caches of all layers."""
+        self._c(lib().mit2cfm_kv_evict_device(self._h, cache, evict, FLAG_SYNC if sync else 0))
 
     def beam_select_device(self, select: BeamSelect, sync: bool = False) -> None:
         """The best continuations of every group's beams."""

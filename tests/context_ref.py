@@ -169,3 +169,39 @@ def weigh64(b, lse, weights, scale, mask=None, decay=1.0, last=0):
             out[s, h, places] += p.sum(0)
             tol[s, h, places] += (p * 1.01 * (rel + (b.new[s] * group + 8) * U)).sum(0) + group * 2.0 ** -120
     return out, tol
+
+
+# ------------------------------------------------------------------ eviction
+def evict(k, v, table, page, length, keep, weights, first, last, born=None, now=None):
+    """kv_evict on numpy arrays: k, v [layers][pages][heads][page][dim], table [seqs][entries], weights and born
+    [layers][seqs][heads][stride].  Returns (k, v, weights, born, length): places past the new lengths are NaN (-1) in the copies."""
+    old_k, old_v, k, v = k, v, k.copy(), v.copy()
+    pages = k.shape[1]
+    new_w = np.full(weights.shape, np.nan, np.float32)
+    new_b = None if born is None else np.full(born.shape, -1, np.int32)
+    out = []
+    for s in range(table.shape[0]):
+        n = max(0, min(length[s], table.shape[1] * page, weights.shape[3]))
+        m = min(n, max(0, keep[s]))
+        out.append(m)
+        for layer in range(weights.shape[0]):
+            for h in range(weights.shape[2]):
+                w = weights[layer, s, h, :n]
+                rank = []
+                for j in range(n):
+                    stays = j < first or (j >= n - last if born is None else int(born[layer, s, h, j]) >= int(now[s]) - last)
+                    least = np.isnan(w[j]) or not 0 <= table[s, j // page] < pages
+                    rank.append((-2 if stays else 0 if least else -1, 0.0 if stays or least else -float(w[j]), j))
+                kept = sorted(x[2] for x in sorted(rank)[:m])
+                place = {j: j for j in kept if j < m}
+                free = [j for j in range(m) if j not in place]
+                for dst, src in zip(free, [j for j in kept if j >= m]):
+                    place[dst] = src
+                    a, b = int(table[s, src // page]), int(table[s, dst // page])
+                    if 0 <= a < pages and 0 <= b < pages:
+                        k[layer, b, h, dst % page], v[layer, b, h, dst % page] = old_k[layer, a, h, src % page], old_v[layer, a, h, src % page]
+                for dst, src in place.items():
+                    new_w[layer, s, h, dst] = w[src]
+                    if born is not None:
+                        new_b[layer, s, h, dst] = born[layer, s, h, src]
+    return k, v, new_w, new_b, np.array(out, np.int32)
