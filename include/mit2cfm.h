@@ -651,6 +651,28 @@ mit2cfm_status mit2cfm_kv_norm_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_
                                              const mit2cfm_kv_rows* rows, const mit2cfm_kv_append* append,
                                              const mit2cfm_kv_norm* norm, uint32_t flags);
 
+/* mit2cfm_kv_attention of sequences that share their first rows, which are then read
+ * once for all of a group's new rows.  The sequences group[g] .. group[g + 1] - 1 share
+ * their first shared[g] rows: those have the same contents for each of them, the same
+ * pages or copies, and which of them are read is not said.  New rows are never taken as
+ * shared, whatever shared[g] says: no more are than every sequence of the group that has
+ * new rows has before them.  group does not decrease; sequences in no group share nothing. */
+typedef struct mit2cfm_kv_prefix {
+  const int32_t* group;  /* [groups + 1] */
+  const int32_t* shared; /* [groups] */
+  uint32_t groups;       /* 0 .. 65535 */
+  uint32_t max_shared;   /* about the largest of shared: the work is split by it (any value is right) */
+  float* lse;            /* [rows][q_heads]: log(sum_j exp(scale q . k_j)) over the keys a row sees, -inf where
+                          * there are none; NULL: not asked for.  No overlap with q or out */
+} mit2cfm_kv_prefix;
+/* 0 where an argument is out of its range; the workspace of mit2cfm_kv_attention has these bytes here. */
+uint64_t mit2cfm_kv_prefix_attention_workspace(const mit2cfm_kv_cache* cache, const mit2cfm_kv_rows* rows,
+                                               uint32_t q_heads, const mit2cfm_kv_prefix* prefix);
+mit2cfm_status mit2cfm_kv_prefix_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                                  const mit2cfm_kv_rows* rows,
+                                                  const mit2cfm_kv_attention* attention,
+                                                  const mit2cfm_kv_prefix* prefix, uint32_t flags);
+
 /* The attention weight that cached rows get, added up: for key head h of every sequence s that
  * has new rows, and each of its cached rows j,
  *   weights_out[s][h][j] = decay * weights[s][h][j] + sum exp(scale * q . k_j - lse)

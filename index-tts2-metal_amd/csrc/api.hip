@@ -686,6 +686,19 @@ mit2cfm_status mit2cfm_kv_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_ca
                    [&](hipStream_t s) { mit2hip::kv_attention(*cache, *rows, *attention, s); });
 }
 
+uint64_t mit2cfm_kv_prefix_attention_workspace(const mit2cfm_kv_cache* cache, const mit2cfm_kv_rows* rows,
+                                               uint32_t q_heads, const mit2cfm_kv_prefix* prefix) {
+  return cache && rows && prefix ? mit2hip::kv_prefix_attention_workspace(*cache, *rows, q_heads, *prefix) : 0;
+}
+
+mit2cfm_status mit2cfm_kv_prefix_attention_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache,
+                                                  const mit2cfm_kv_rows* rows,
+                                                  const mit2cfm_kv_attention* attention,
+                                                  const mit2cfm_kv_prefix* prefix, uint32_t flags) {
+  return on_stream(ctx, flags, cache && rows && attention && prefix, "cache, rows, attention and prefix must not be NULL",
+                   [&](hipStream_t s) { mit2hip::kv_prefix_attention(*cache, *rows, *attention, *prefix, s); });
+}
+
 mit2cfm_status mit2cfm_kv_weigh_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache* cache, const mit2cfm_kv_rows* rows,
                                        const mit2cfm_kv_weigh* weigh, uint32_t flags) {
   return on_stream(ctx, flags, cache && rows && weigh, "cache, rows and weigh must not be NULL",

@@ -69,6 +69,9 @@ inline bool append_wide(const AppendArgs& a, int V) {
          (a.interleaved || a.rot % (2 * V) == 0);
 }
 
+// Checks an attention's arguments but for its workspace's size; false: there are no rows.
+bool attention_args(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, AttendArgs& a);
+
 // N elements that are read or written at once.
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec {

@@ -33,6 +33,17 @@ struct AttendArgs {
   float scale2;        // |scale| log2(e): scores in powers of two
 };
 
+// Either half of the attention of sequences that share their first rows (kv_prefix.h):
+// the shared rows, for all new rows of a group of sequences at once, or what each
+// sequence has of its own.  Both leave parts, for one join.
+struct PrefixArgs : AttendArgs {
+  const int32_t* bounds;  // [groups + 1] first sequences of the groups
+  const int32_t* shared;  // [groups] rows that a group's sequences share
+  int groups;
+  int own;                // the second half
+  int slots, slot0;       // parts of a query row, and this half's first
+};
+
 // What splits leave for their join: [row][query head][split] outputs, maxima and
 // weights' sums, [row][query head] the number of splits.
 struct Parts {
@@ -187,6 +198,121 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, const AttendPlan&
   p.parts = p.whole ? 1 : (p.len + chunk - 1) / chunk;
   return p.split == 0 || p.begin < p.len;
 }
+
+// Where a split's part goes, and whether the block says how many there are.
+__device__ __forceinline__ size_t slot_of(const AttendArgs&, const AttendPlan& plan, const Part& p, size_t pair) {
+  return pair * plan.splits + p.split;
+}
+__device__ __forceinline__ bool tells_parts(const AttendArgs&, const AttendPlan& plan, const Part& p) {
+  return p.split == 0 && plan.splits > 1;
+}
+
+// Rows that the sequences lo .. hi - 1 may share: as many as said, of those before any
+// of their new rows, in whole runs of kSharedStep.  (The same for all lanes.)
+constexpr int kSharedStep = 64;
+__device__ __forceinline__ int shared_rows(const RowView& r, int lo, int hi, int said, int capacity) {
+  const int lane = threadIdx.x & 63;
+  int least = min(said, capacity);
+  for (int base = lo; base < hi; base += 64) {
+    const int s = base + lane;
+    if (s < hi) {
+      const int s0 = r.start[s], s1 = r.start[s + 1];
+      if (s1 > s0) least = min(least, r.length[s] - (s1 - s0));
+    }
+  }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) least = min(least, __shfl_xor(least, off, kWave));
+  return __builtin_amdgcn_readfirstlane(max(least, 0) / kSharedStep * kSharedStep);
+}
+// A block's part of either half (see Part).  Shared rows: a group's new rows as if they
+// were one sequence's, all of which see all keys.
+__device__ __forceinline__ bool find_part(const PrefixArgs& a, const AttendPlan& plan, int mtile, Part& p) {
+  int tile = blockIdx.x, unit = blockIdx.y;
+  if (plan.by_xcd) {
+    const int slot = blockIdx.x >> 3;
+    unit = slot / plan.tiles * 8 + (blockIdx.x & 7);
+    tile = slot % plan.tiles;
+    if (unit >= a.c.kv_heads * plan.splits) return false;
+  }
+  const int lane = threadIdx.x & 63;
+  p.kvh = unit % a.c.kv_heads;
+  p.split = unit / a.c.kv_heads;
+  p.whole = false;
+  if (a.own) {
+    Found f;
+    if (!find_tile(a.r, a.group, mtile, tile, f)) return false;
+    p.seq = f.seq;
+    p.raw_start = f.start;
+    p.start = max(f.start, 0);
+    p.mrows = (min(f.stop, a.r.rows) - p.start) * a.group;
+    p.m0 = f.in_seq * mtile;
+    p.first = f.length - (f.stop - f.start);
+    p.len = min(f.length, a.c.capacity());
+    int from = 0;  // the group's shared rows
+    for (int base = 0; base < a.groups; base += 64) {
+      int lo = 0, hi = 0, said = 0;
+      if (base + lane < a.groups) {
+        lo = a.bounds[base + lane];
+        hi = a.bounds[base + lane + 1];
+        said = a.shared[base + lane];
+      }
+      const uint64_t mine = __ballot(lo <= f.seq && f.seq < hi);
+      if (!mine) continue;
+      const int l = __ffsll((unsigned long long)mine) - 1;
+      from = shared_rows(a.r, max(__builtin_amdgcn_readlane(lo, l), 0), min(__builtin_amdgcn_readlane(hi, l), a.r.seqs),
+                         __builtin_amdgcn_readlane(said, l), a.c.capacity());
+      break;
+    }
+    const int chunk = chunk_of(p.len - from, plan.chunk, plan.splits);
+    p.begin = min(from + p.split * chunk, max(p.len, from));
+    p.end = min(p.begin + chunk, p.len);
+    // (bit 16: there are shared rows)
+    p.parts = max(1, (p.len - from + chunk - 1) / chunk) | (from > 0 ? 1 << 16 : 0);
+    return p.split == 0 || p.begin < p.len;
+  }
+  int before = 0;
+  for (int base = 0; base < a.groups; base += 64) {
+    int n = 0, s0 = 0, lo = 0, hi = 0, said = 0;
+    if (base + lane < a.groups) {
+      lo = max(a.bounds[base + lane], 0);
+      hi = min(a.bounds[base + lane + 1], a.r.seqs);
+      said = a.shared[base + lane];
+      if (lo < hi && said >= kSharedStep) {
+        s0 = a.r.start[lo];
+        const int rows = min(a.r.start[hi], a.r.rows) - max(s0, 0);
+        n = rows > 0 ? (int)(((int64_t)rows * a.group + mtile - 1) / mtile) : 0;
+        p.mrows = rows * a.group;
+      }
+    }
+    int incl = n;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(incl, off, kWave);
+      if (lane >= off) incl += o;
+    }
+    const uint64_t past = __ballot(before + incl > tile);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      p.seq = __builtin_amdgcn_readlane(lo, l);
+      p.raw_start = __builtin_amdgcn_readlane(s0, l);
+      p.start = max(p.raw_start, 0);
+      p.mrows = __builtin_amdgcn_readlane(p.mrows, l);
+      p.m0 = (tile - before - __builtin_amdgcn_readlane(incl - n, l)) * mtile;
+      p.len = p.first = shared_rows(a.r, p.seq, __builtin_amdgcn_readlane(hi, l), __builtin_amdgcn_readlane(said, l), a.c.capacity());
+      const int chunk = chunk_of(p.len, plan.chunk, plan.splits);
+      p.begin = p.split * chunk;
+      p.end = min(p.begin + chunk, p.len);
+      p.parts = (p.len + chunk - 1) / chunk;
+      return p.begin < p.len;
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+__device__ __forceinline__ size_t slot_of(const PrefixArgs& a, const AttendPlan&, const Part& p, size_t pair) {
+  return pair * a.slots + a.slot0 + p.split;
+}
+__device__ __forceinline__ bool tells_parts(const PrefixArgs&, const AttendPlan&, const Part& p) { return p.split == 0; }
 
 // A lane's query: its row in the buffers, its place among the sequence's new
 // rows (as given), its head.
@@ -413,8 +539,8 @@ __device__ __forceinline__ float taken_out(T v) {
 // (5.3 TB/s; a large copy reaches 4.7); one over 131001, 537 MB in 96 us (5.6).  Three
 // tokens over 703 fp32 keys of 20 heads of 64 take 8.2 us, 5.6 of them the way to the
 // first key and from the last: sequence, page, keys, the join in LDS.
-template <typename T, int D, int MT, bool BIG>
-__global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a, AttendPlan plan, Parts part) {
+template <typename T, int D, int MT, bool BIG, typename A>
+__global__ __launch_bounds__(kAttendThreads) void attend_kernel(A a, AttendPlan plan, Parts part) {
   typedef Dims<T, D> S;
   typedef typename Mat<T>::op Op;
   constexpr int KT = S::KT, NT = S::NT, DP = S::DP, DC = S::DC, NV = S::NV;
@@ -578,12 +704,12 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a, At
           for (int d = 0; d < DP; ++d) out[d] = r.v[d];
         }
       } else {
-        const size_t at = ((size_t)x.row * a.q_heads + x.h) * plan.splits + p.split;
+        const size_t at = slot_of(a, plan, p, (size_t)x.row * a.q_heads + x.h);
 #pragma unroll
         for (int d = 0; d < DP; ++d) part.o[at * D + d0 + d] = O[d];
         if ((tid & 15) == 0) part.ml[at] = make_float2(mm, L);
       }
-      if (p.split == 0 && plan.splits > 1 && (tid & 15) == 0) part.n[(size_t)x.row * a.q_heads + x.h] = p.parts;
+      if (tells_parts(a, plan, p) && (tid & 15) == 0) part.n[(size_t)x.row * a.q_heads + x.h] = p.parts;
     }
   }
 }
@@ -630,8 +756,8 @@ __device__ __forceinline__ void load_to_lds(const void* src, lds_ptr_t* lds) {
 //
 // The ring's buffers are objects of their own, named by constants in the usual
 // path: a read that might alias any of them would wait for every load.
-template <typename T, int D>
-__global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendArgs a, AttendPlan plan, Parts part) {
+template <typename T, int D, typename A>
+__global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(A a, AttendPlan plan, Parts part) {
   typedef Dims<T, D> S;
   typedef typename Mat<T>::op Op;
   constexpr int KT = S::KT, NT = S::NT, DP = S::DP, DC = S::DC, NV = S::NV;
@@ -895,7 +1021,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
         }
       }
     } else {
-      const size_t at = ((size_t)x.row * a.q_heads + x.h) * plan.splits + p.split;
+      const size_t at = slot_of(a, plan, p, (size_t)x.row * a.q_heads + x.h);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -904,7 +1030,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(AttendAr
               floatx4{run[mt].o[d][r], run[mt].o[d + 1][r], run[mt].o[d + 2][r], run[mt].o[d + 3][r]};
       if (grp == 0) part.ml[at] = make_float2(run[mt].mx, L);
     }
-    if (p.split == 0 && plan.splits > 1 && grp == 0) part.n[(size_t)x.row * a.q_heads + x.h] = p.parts;
+    if (tells_parts(a, plan, p) && grp == 0) part.n[(size_t)x.row * a.q_heads + x.h] = p.parts;
   }
 }
 
@@ -972,6 +1098,29 @@ __global__ __launch_bounds__(WAVES * 64) void combine_kernel(AttendArgs a, Atten
 
 void attend_launched(hipError_t e);  // throws HipError (kv_ops.hip)
 
+// The launch of a plan's blocks.
+template <typename T, int D, typename A>
+void launch_tiles(const A& a, const AttendPlan& plan, const Parts& part, hipStream_t s) {
+  const AttendGrid g = attend_grid(plan, a.c.kv_heads);
+  const dim3 grid(g.x, g.y), block(kAttendThreads);
+  const bool big = (1 << a.c.page_shift) >= Mat<T>::KT;
+  auto tiles = [&](auto big_page) {
+    constexpr bool BIG = decltype(big_page)::value;
+    if (plan.form == 1)
+      hipLaunchKernelGGL((attend_kernel<T, D, 1, BIG, A>), grid, block, 0, s, a, plan, part);
+    else
+      hipLaunchKernelGGL((attend_kernel<T, D, 2, BIG, A>), grid, block, 0, s, a, plan, part);
+  };
+  if (plan.form == kWide) {
+    if constexpr (wide_dim(D)) hipLaunchKernelGGL((attend_wide_kernel<T, D, A>), grid, block, 0, s, a, plan, part);
+  } else if (big) {
+    tiles(std::true_type{});
+  } else {
+    tiles(std::false_type{});
+  }
+  attend_launched(hipGetLastError());
+}
+
 template <typename T, int D>
 void launch_attend(const AttendArgs& a, const AttendPlan& plan, void* workspace, hipStream_t s) {
   const size_t pairs = (size_t)a.r.rows * a.q_heads, n = pairs * plan.splits;
@@ -979,24 +1128,7 @@ void launch_attend(const AttendArgs& a, const AttendPlan& plan, void* workspace,
   part.o = static_cast<float*>(workspace);
   part.ml = reinterpret_cast<float2*>(part.o + n * D);
   part.n = reinterpret_cast<int32_t*>(part.ml + n);
-  const AttendGrid g = attend_grid(plan, a.c.kv_heads);
-  const dim3 grid(g.x, g.y), block(kAttendThreads);
-  const bool big = (1 << a.c.page_shift) >= Mat<T>::KT;
-  auto tiles = [&](auto big_page) {
-    constexpr bool BIG = decltype(big_page)::value;
-    if (plan.form == 1)
-      hipLaunchKernelGGL((attend_kernel<T, D, 1, BIG>), grid, block, 0, s, a, plan, part);
-    else
-      hipLaunchKernelGGL((attend_kernel<T, D, 2, BIG>), grid, block, 0, s, a, plan, part);
-  };
-  if (plan.form == kWide) {
-    if constexpr (wide_dim(D)) hipLaunchKernelGGL((attend_wide_kernel<T, D>), grid, block, 0, s, a, plan, part);
-  } else if (big) {
-    tiles(std::true_type{});
-  } else {
-    tiles(std::false_type{});
-  }
-  attend_launched(hipGetLastError());
+  launch_tiles<T, D>(a, plan, part, s);
   if (plan.splits == 1) return;
   if (plan.splits <= kFewSplits)
     hipLaunchKernelGGL((combine_kernel<T, D, 1>), dim3(a.r.rows, a.q_heads), dim3(64), 0, s, a, plan, part);

@@ -17,6 +17,12 @@ void kv_norm_append(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, 
                     const mit2cfm_kv_norm& n, hipStream_t s);
 void kv_attention(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const mit2cfm_kv_attention& a,
                   hipStream_t s);
+// Attention of sequences that share their first rows (kv_prefix.hip), and its
+// workspace's bytes, 0: an argument out of range.
+void kv_prefix_attention(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const mit2cfm_kv_attention& a,
+                         const mit2cfm_kv_prefix& x, hipStream_t s);
+uint64_t kv_prefix_attention_workspace(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, uint32_t q_heads,
+                                       const mit2cfm_kv_prefix& x);
 // Adds up the attention weight that cached rows get (kv_weigh.hip).
 void kv_weigh(const mit2cfm_kv_cache& cache, const mit2cfm_kv_rows& rows, const mit2cfm_kv_weigh& w, hipStream_t s);
 // Bytes of kv_attention's workspace; 0: none needed, or an argument out of range.

@@ -247,7 +247,8 @@ uint64_t kv_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows
   return (uint64_t)r.rows * q_heads * (plan.splits * (uint64_t)(c.head_dim + 2) + 1) * sizeof(float);
 }
 
-void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, hipStream_t s) {
+// Checks an attention's arguments but for its workspace; false: there are no rows.
+bool attention_args(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, AttendArgs& a) {
   check_kv_cache(c);
   check_kv_rows(r);
   need(query_rows_in_range(c, r, p.q_heads),
@@ -256,17 +257,14 @@ void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit
   need(p.mask == nullptr || p.mask_words >= 1, "mask_words must be >= 1 with a mask");
   need(p.mask_words < (1u << 24), "mask_words must be below 2^24");
   need(aligned(p.mask, 4), "mask must be 4-byte aligned");
-  if (r.seqs == 0 || r.rows == 0) return;
+  if (r.seqs == 0 || r.rows == 0) return false;
   need(p.q && p.out && p.q != p.out, "q and out must not be NULL, nor the same");
   const size_t e = (size_t)kv_elem_bytes(c.dtype);
   need(aligned(p.q, e) && aligned(p.out, e), "q and out must be aligned to their type");
   const Pieces out = pieces(p.out, p.out_row, p.out_head, r.rows, p.q_heads, c.head_dim, e);
   need(!meet_themselves(out), "out's rows and heads overlap");
   need(!meet(pieces(p.q, p.q_row, p.q_head, r.rows, p.q_heads, c.head_dim, e), out), "out overlaps q");
-  const uint64_t bytes = kv_attention_workspace(c, r, p.q_heads);
-  need(bytes == 0 || (p.workspace && p.workspace_bytes >= bytes), "workspace is NULL or too small");
   need(aligned(p.workspace, 16), "workspace must be 16-byte aligned");
-  AttendArgs a;
   a.c = view(c);
   a.r = view(r);
   a.q = static_cast<const char*>(p.q);
@@ -280,6 +278,14 @@ void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit
   set_scale(a, p.scale);
   a.q_wide = aligned(p.q, 16) && p.q_row % 8 == 0 && p.q_head % 8 == 0;
   a.o_wide = aligned(p.out, 16) && p.out_row % 8 == 0 && p.out_head % 8 == 0;
+  return true;
+}
+
+void kv_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p, hipStream_t s) {
+  AttendArgs a;
+  if (!attention_args(c, r, p, a)) return;
+  const uint64_t bytes = kv_attention_workspace(c, r, p.q_heads);
+  need(bytes == 0 || (p.workspace && p.workspace_bytes >= bytes), "workspace is NULL or too small");
   const int D = (int)c.head_dim;
   const AttendPlan plan = attend_plan(c, r, p.q_heads);
   if (c.dtype == MIT2CFM_DTYPE_F32)

@@ -142,6 +142,10 @@ def lib() -> ctypes.CDLL:
                                                ctypes.POINTER(KvAppend), ctypes.POINTER(KvNorm), u32]),
         "mit2cfm_kv_attention_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
                                              ctypes.POINTER(KvAttention), u32]),
+        "mit2cfm_kv_prefix_attention_workspace": (u64, [ctypes.POINTER(KvCache), ctypes.POINTER(KvRows), u32,
+                                                        ctypes.POINTER(KvPrefix)]),
+        "mit2cfm_kv_prefix_attention_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows),
+                                                    ctypes.POINTER(KvAttention), ctypes.POINTER(KvPrefix), u32]),
         "mit2cfm_kv_weigh_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvRows), ctypes.POINTER(KvWeigh), u32]),
         "mit2cfm_kv_evict_workspace": (u64, [ctypes.POINTER(KvCache), ctypes.POINTER(KvEvict)]),
         "mit2cfm_kv_evict_device": (st, [vp, ctypes.POINTER(KvCache), ctypes.POINTER(KvEvict), u32]),
@@ -207,6 +211,12 @@ class KvAttention(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
+class KvPrefix(ctypes.Structure):
+    """mit2cfm_kv_prefix."""
+    _fields_ = [("group", ctypes.c_void_p), ("shared", ctypes.c_void_p), ("groups", ctypes.c_uint32),
+                ("max_shared", ctypes.c_uint32), ("lse", ctypes.c_void_p)]
+
+
 class KvWeigh(ctypes.Structure):
     """mit2cfm_kv_weigh."""
     _fields_ = [("q", ctypes.c_void_p), ("q_row", ctypes.c_uint64), ("q_head", ctypes.c_uint64), ("q_heads", ctypes.c_uint32),
@@ -248,6 +258,11 @@ class BeamReorder(ctypes.Structure):
 def kv_attention_workspace(cache: KvCache, rows: KvRows, q_heads: int) -> int:
     """Bytes of workspace that Context.kv_attention_device needs for these sizes."""
     return int(lib().mit2cfm_kv_attention_workspace(ctypes.byref(cache), ctypes.byref(rows), q_heads))
+
+
+def kv_prefix_attention_workspace(cache: KvCache, rows: KvRows, q_heads: int, prefix: KvPrefix) -> int:
+    """Bytes of workspace that Context.kv_prefix_attention_device needs for these sizes."""
+    return int(lib().mit2cfm_kv_prefix_attention_workspace(ctypes.byref(cache), ctypes.byref(rows), q_heads, ctypes.byref(prefix)))
 
 
 def kv_evict_workspace(cache: KvCache, evict: KvEvict) -> int:
@@ -868,6 +883,10 @@ class Context:
     def kv_attention_device(self, cache: KvCache, rows: KvRows, attention: KvAttention, sync: bool = False) -> None:
         """Attention of new rows (tokens, chains, trees) over their sequences' paged caches."""
         self._c(lib().mit2cfm_kv_attention_device(self._h, cache, rows, attention, FLAG_SYNC if sync else 0))
+
+    def kv_prefix_attention_device(self, cache: KvCache, rows: KvRows, attention: KvAttention, prefix: KvPrefix, sync: bool = False) -> None:
+        """kv_attention_device of sequences that share their first rows, which are read once for all of a group's."""
+        self._c(lib().mit2cfm_kv_prefix_attention_device(self._h, cache, rows, attention, prefix, FLAG_SYNC if sync else 0))
 
     def kv_weigh_device(self, cache: KvCache, rows: KvRows, weigh: KvWeigh, sync: bool = False) -> None:
         """Adds the attention weight that new rows give to cached ones."""

@@ -205,3 +205,38 @@ def evict(k, v, table, page, length, keep, weights, first, last, born=None, now=
                     if born is not None:
                         new_b[layer, s, h, dst] = born[layer, s, h, src]
     return k, v, new_w, new_b, np.array(out, np.int32)
+
+
+# ------------------------------------------------------------------ shared prefixes
+def share(b, bounds, shared, alias):
+    """Makes the first shared[g] rows of the sequences bounds[g] .. bounds[g + 1] - 1 of a batch alike: full pages by name when
+    `alias`, else (and the last part page) by copies."""
+    for g, n in enumerate(shared):
+        lo, hi = bounds[g], bounds[g + 1]
+        for s in range(lo + 1, hi):
+            for j in range(min(n, b.length[s], b.length[lo])):
+                if alias and (j // b.page + 1) * b.page <= n:
+                    b.table[s, j // b.page] = b.table[lo, j // b.page]
+                    continue
+                frm, to, at = b.page_of(lo, j), b.page_of(s, j), j % b.page
+                for x in (b.k, b.v):
+                    x[to, :, at] = x[frm, :, at]
+
+
+def lse_tolerance(b, scale, mask=None):
+    """How far a log sum may be off: its scores' errors, weighted (dim products and sums, the scale, the exponentials), the sum's,
+    and the maximum's and logarithm's roundings in powers of two."""
+    tol = torch.zeros(b.q.shape[:2], dtype=torch.float64)
+    group = b.q_heads // b.kv_heads
+    for row, s, i, before in b.each_row():
+        at = seen(b, row, s, i, before, mask)
+        if not at:
+            continue
+        _, pages, slots = (torch.tensor(x) for x in zip(*at))
+        for h in range(b.kv_heads):
+            k, q = b.k[pages, h, slots].double(), b.q[row, h * group: (h + 1) * group].double()
+            z = q @ k.t() * scale
+            score = (b.dim + 4) * U * abs(scale) * (q.abs() @ k.abs().t()) + 4 * U * z.abs() + 4 * U
+            lse = torch.logsumexp(z, -1)
+            tol[row, h * group: (h + 1) * group] = 1.01 * (torch.softmax(z, -1) * score).sum(-1) + (len(at) + 16) * U + 6 * U * lse.abs()
+    return tol
