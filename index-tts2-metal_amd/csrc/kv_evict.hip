@@ -284,7 +284,8 @@ void kv_evict(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p, hipStream_t 
          "weights, born, now and their outputs overlap");
   }
   auto clear = [&](const void* out, uint64_t n) {
-    return !meet(p.keep, seq_bytes, out, n) && (out == p.length || !meet(p.length, seq_bytes, out, n));
+    const bool length = out == p.length_out && p.length == p.length_out;  // (may be itself)
+    return !meet(p.keep, seq_bytes, out, n) && (length || !meet(p.length, seq_bytes, out, n));
   };
   need(clear(p.weights_out, bytes) && clear(p.length_out, seq_bytes) && (!p.born || clear(p.born_out, bytes)) &&
            !meet(p.weights, bytes, p.length_out, seq_bytes) && !meet(p.weights_out, bytes, p.length_out, seq_bytes) &&
