@@ -1,6 +1,7 @@
 // kv_evict.hip -- rows of least weight leave a paged cache (see kv_ops.h and
 // mit2cfm.h for what it computes).
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_args.h"
 
@@ -10,8 +11,12 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
+constexpr int kKeys = 16;                         // a thread's keys at a time
+constexpr int kWaveKeys = 64 * kKeys;             // a wave's
+constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64;
+constexpr int kSplitKeys = kSplitWaves * kWaveKeys;  // a segment's, where the length is as said
 constexpr int kBins = 2048;
+constexpr int kMaxSegments = 64;
 constexpr int kMoveThreads = 256;
 
 struct EvictArgs {
@@ -30,6 +35,11 @@ struct EvictArgs {
   // from: list_stride of each), their number, a sequence's new length
   int32_t *to, *from, *moves, *stay;
   int64_t list_stride;
+  // long lines: histograms [line][segment][kBins] of three rounds, and what they tell
+  uint32_t* hist[3];
+  uint2* found[2];  // [line] the bits so far, rows that stay among the keys that have them
+  uint32_t* larger;  // [line][segment] keys above those that agree in the first two rounds' bits
+  int segments;
 };
 
 __device__ __forceinline__ int64_t line_of(const EvictArgs& a, int layer, int seq, int head) {
@@ -47,66 +57,325 @@ struct Ranks {
   const int32_t* born;
   const int32_t* table;
   int n, first, tail, pages, page_shift;  // tail: the first of the youngest places, without births
-  int64_t oldest;                         // with births: rows from this one on
-  __device__ __forceinline__ uint32_t key(int j) const {
-    const bool stays = j < first || (born ? (int64_t)born[j] >= oldest : j >= tail);
-    uint32_t u = __float_as_uint(weights[j]);
-    if (u == 0x80000000u) u = 0;
-    const bool least = (u & 0x7fffffffu) > 0x7f800000u || (unsigned)table[j >> page_shift] >= (unsigned)pages;
+  int oldest;                             // with births: rows from this one on
+  __device__ __forceinline__ uint32_t key_of(int j, float weight, int birth, int page) const {
+    const bool stays = (j < first) | (born ? birth >= oldest : j >= tail);
+    uint32_t u = __float_as_uint(weight);
+    u = u == 0x80000000u ? 0u : u;
+    const bool least = ((u & 0x7fffffffu) > 0x7f800000u) | ((unsigned)page >= (unsigned)pages);
     u ^= u >> 31 ? 0xffffffffu : 0x80000000u;
     return stays ? 0xffffffffu : least ? 0u : u;
   }
+  // The keys of a wave's places j0 .. j1 - 1 (at most kWaveKeys) to LDS, one after
+  // the other, 0 past the end.  Read through resources that end where the places do.
+  __device__ __forceinline__ void load(int j0, int j1, uint32_t* to) const {
+    constexpr int B = 8;  // of a lane at once
+    const int lane = threadIdx.x & 63, size = max(j1 - j0, 0);
+    const int e0 = j0 >> page_shift, entries = size ? ((j1 - 1) >> page_shift) - e0 + 1 : 0;
+    const buffer_rsrc_t rw = make_buffer_rsrc(weights + j0, 4 * size), rt = make_buffer_rsrc(table + e0, 4 * entries);
+    const buffer_rsrc_t rb = make_buffer_rsrc(born ? born + j0 : nullptr, born ? 4 * size : 0);
+#pragma unroll 1
+    for (int i0 = 0; i0 < kWaveKeys; i0 += 64 * B) {
+      float w[B];
+      int birth[B], page[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const int i = i0 + 64 * u + lane;
+        w[u] = buffer_load_f32(rw, 4 * i);
+        birth[u] = __float_as_int(buffer_load_f32(rb, 4 * i));
+        page[u] = __float_as_int(buffer_load_f32(rt, 4 * (((j0 + i) >> page_shift) - e0)));
+      }
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const int i = i0 + 64 * u + lane;
+        to[i] = i < size ? key_of(j0 + i, w[u], birth[u], page[u]) : 0u;
+      }
+    }
+  }
 };
 
-// A block ranks a line: the key of the last row that stays is found by three
-// histograms of its bits (11, 11, 10), among the keys that agree so far; then each
-// wave walks its share of the places in order.  A place p that stays has
-// before(p) = #(larger keys before p) + min(#(equal keys before p), ties) rows before
-// it that stay, which gives a freed place and a row that moves their numbers in the
-// lists: p - before(p), before(p) - before(keep).
-__global__ __launch_bounds__(kChooseThreads) void choose_kernel(EvictArgs a) {
-  __shared__ uint32_t bins[kBins];
-  __shared__ uint32_t s_wave[kChooseWaves], s_gt[kChooseWaves], s_eq[kChooseWaves], s_gt_below[kChooseWaves], s_eq_below[kChooseWaves];
-  __shared__ uint32_t s_bin, s_left;
-  const int head = blockIdx.x, seq = blockIdx.y, layer = blockIdx.z;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
-  const int64_t line = line_of(a, layer, seq, head);
+// base + #(voting lanes before this one)
+__device__ __forceinline__ uint32_t lanes_below(uint64_t vote, uint32_t base) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(vote >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote, base));
+}
+// An element at a 32-bit distance in bytes.
+template <typename T>
+__device__ __forceinline__ T& near(T* base, uint32_t i) {
+  return *reinterpret_cast<T*>(reinterpret_cast<std::conditional_t<std::is_const<T>::value, const char, char>*>(base) + (uint32_t)(4u * i));
+}
+
+// A line as its block sees it.
+struct Line {
+  int head, seq, layer;
+  int64_t at;
+  int m;  // rows that stay
+  bool apart, apart_born;
+  float* weights_out;
+  int32_t* born_out;
   Ranks r;
-  r.n = places_of(a, seq);
-  const int m = min(r.n, max(a.keep[seq], 0));
-  const bool apart = a.weights_out != a.weights, apart_born = a.born && a.born_out != a.born;
-  r.weights = a.weights + line * a.stride;
-  r.born = a.born ? a.born + line * a.stride : nullptr;
-  r.table = a.c.table + (size_t)seq * a.c.table_stride;
-  r.first = (int)min(a.first_rows, (int64_t)r.n);
-  r.tail = (int)max(r.n - a.last_rows, (int64_t)0);
-  r.pages = a.c.pages;
-  r.page_shift = a.c.page_shift;
-  r.oldest = a.born ? (int64_t)a.now[seq] - a.last_rows : 0;
-  float* weights_out = a.weights_out + line * a.stride;
-  int32_t* born_out = a.born_out ? a.born_out + line * a.stride : nullptr;
-  if (tid == 0 && head == 0 && layer == 0) a.stay[seq] = m;
-  if (m == r.n || m == 0) {
-    if (tid == 0) a.moves[line] = 0;
-    for (int j = tid; j < m; j += blockDim.x) {
-      if (apart) weights_out[j] = r.weights[j];
-      if (apart_born) born_out[j] = r.born[j];
+  __device__ __forceinline__ Line(const EvictArgs& a, int head_) : head(head_), seq(blockIdx.y), layer(blockIdx.z) {
+    at = line_of(a, layer, seq, head);
+    r.n = places_of(a, seq);
+    m = min(r.n, max(a.keep[seq], 0));
+    apart = a.weights_out != a.weights;
+    apart_born = a.born && a.born_out != a.born;
+    r.weights = a.weights + at * a.stride;
+    r.born = a.born ? a.born + at * a.stride : nullptr;
+    r.table = a.c.table + (size_t)seq * a.c.table_stride;
+    r.first = (int)min(a.first_rows, (int64_t)r.n);
+    r.tail = (int)max(r.n - a.last_rows, (int64_t)0);
+    r.pages = a.c.pages;
+    r.page_shift = a.c.page_shift;
+    r.oldest = a.born ? (int)max((int64_t)a.now[seq] - a.last_rows, (int64_t)INT32_MIN) : 0;
+    weights_out = a.weights_out + at * a.stride;
+    born_out = a.born_out ? a.born_out + at * a.stride : nullptr;
+  }
+  // Weights and births to where they are wanted, of the places j0 .. j1 - 1 below m, by
+  // `by` threads.  (Those of places that rows left are written again by the moves.)
+  __device__ __forceinline__ void copy(int j0, int j1, int mine, int by) const {
+    if (!apart && !apart_born) return;
+    constexpr int B = 8;  // of a thread in flight
+    j1 = min(j1, m);
+#pragma unroll 1
+    for (int j = j0 + mine; j < j1; j += B * by) {
+      float w[B];
+      int birth[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const int at = min(j + u * by, j1 - 1);
+        if (apart) w[u] = near(r.weights, at);
+        if (apart_born) birth[u] = near(r.born, at);
+      }
+#pragma unroll
+      for (int u = 0; u < B; ++u)
+        if (j + u * by < j1) {
+          if (apart) near(weights_out, j + u * by) = w[u];
+          if (apart_born) near(born_out, j + u * by) = birth[u];
+        }
     }
+  }
+};
+
+// A wave's places j0 .. j1 - 1 in order, 64 at a time: f(place, key, whether it is one of
+// them).  held: `keys` has them; else it is filled as they come.
+template <typename F>
+__device__ __forceinline__ void sweep(const Ranks& r, int j0, int j1, bool held, uint32_t* keys, F&& f) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int base = j0; base < j1; base += kWaveKeys) {
+    const int size = min(j1 - base, kWaveKeys);
+    if (!held) r.load(base, base + size, keys);
+#pragma unroll 1
+    for (int i = 0; i < size; i += 64) f(base + i + lane, keys[i + lane], i + lane < size);
+  }
+}
+
+// Writes the lists' share of a wave's places.  Keys above `least` stay, and the first
+// `ties` that equal it.  A place p that stays has before(p) = #(larger keys before p) +
+// min(#(equal keys before p), ties) rows before it that stay, which gives a freed place
+// and a row that moves their numbers in the lists: p - before(p), before(p) - stay_below.
+// gt, eq: larger and equal keys of the places before the wave's.
+__device__ __forceinline__ void list_moves(const EvictArgs& a, const Line& x, int j0, int j1, bool held, uint32_t* keys,
+                                           uint32_t least, uint32_t ties, uint32_t gt, uint32_t eq, uint32_t stay_below) {
+  int32_t *to = a.to + x.at * a.list_stride, *from = a.from + x.at * a.list_stride;
+  sweep(x.r, j0, j1, held, keys, [&](int j, uint32_t k, bool in) {
+    const bool more = in && k > least, equal = in && k == least;
+    const uint64_t vote_gt = __ballot(more), vote_eq = __ballot(equal);
+    const uint32_t gt_before = lanes_below(vote_gt, gt), eq_before = lanes_below(vote_eq, eq);
+    const uint32_t before = gt_before + min(eq_before, ties);
+    const bool stays = more || (equal && eq_before < ties);
+    if (j < x.m) {
+      if (in && !stays) near(to, j - before) = j;
+    } else if (stays) {
+      near(from, before - stay_below) = j;
+    }
+    gt += __popcll(vote_gt);
+    eq += __popcll(vote_eq);
+  });
+}
+
+// A block of W waves ranks a line whose keys lie in registers (longer lines than were
+// said are read again each time).  The key of the last row that stays, the m-th
+// largest, is found bit by bit from the top: votes count the keys from a candidate on,
+// and end the search once these are m.  No histogram, so no addition waits for another,
+// and of one wave no barrier.
+template <int W>
+__global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
+  __shared__ uint32_t s_keys[W][kWaveKeys];
+  __shared__ uint32_t s_count[2][W], s_gt[W], s_eq[W], s_gt_below[W], s_eq_below[W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Line x(a, blockIdx.x);
+  const int n = x.r.n, m = x.m;
+  if (tid == 0 && x.head == 0 && x.layer == 0) a.stay[x.seq] = m;
+  if (m == n || m == 0) {
+    if (tid == 0) a.moves[x.at] = 0;
+    x.copy(0, m, tid, 64 * W);
     return;
   }
+  const bool held = n <= W * kWaveKeys;
+  const int share = held ? kWaveKeys : ((n + W - 1) / W + 63) / 64 * 64;  // a wave's places
+  const int j0 = min(wave * share, n), j1 = min(j0 + share, n);
+  uint32_t* const keys = s_keys[wave];
+  uint32_t key[kKeys];
+  if (held) {
+    x.r.load(j0, j1, keys);
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) key[i] = keys[64 * i + lane];
+  }
 
-  uint32_t agreed = 0, left = m;  // the bits so far; rows that stay among the keys that have them
-#pragma unroll 1
-  for (int round = 0; round < 3; ++round) {
-    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, above = round == 0 ? 32 : round == 1 ? 21 : 10;
-    const uint32_t mask = round == 2 ? 1023u : 2047u;
-    for (int b = tid; b < kBins; b += blockDim.x) bins[b] = 0;
+  int turn = 0;
+  auto whole = [&](uint32_t count) {  // over the block
+    if (W == 1) return count;
+    if (lane == 0) s_count[turn][wave] = count;
     __syncthreads();
-    for (int j = tid; j < r.n; j += blockDim.x) {
-      const uint32_t k = r.key(j);
-      const bool in = round == 0 || k >> above == agreed >> above;
-      if (!in) continue;
-      const uint32_t bin = k >> shift & mask;
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += s_count[turn][w];
+    turn ^= 1;
+    return (uint32_t)__builtin_amdgcn_readfirstlane(sum);
+  };
+  auto from_on = [&](uint32_t c) {  // keys >= c; c > 0, so none past the end
+    uint32_t count = 0;
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) count += __popcll(__ballot(key[i] >= c));
+    } else {
+      sweep(x.r, j0, j1, false, keys, [&](int, uint32_t k, bool) { count += __popcll(__ballot(k >= c)); });
+    }
+    return whole(count);
+  };
+  uint32_t least = 0, ties = 0;
+  bool exact = false;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = least | 1u << bit, count = from_on(c);
+    if (count >= (uint32_t)m) least = c;
+    if (count == (uint32_t)m) {
+      exact = true;
+      break;
+    }
+  }
+  if (exact)
+    least -= 1;  // all from the candidate on stay
+  else
+    ties = m - (least == 0xffffffffu ? 0u : from_on(least + 1));
+
+  uint32_t gt = 0, eq = 0, gt_below = 0, eq_below = 0;
+  sweep(x.r, j0, j1, held, keys, [&](int j, uint32_t k, bool in) {
+    const uint64_t more = __ballot(in && k > least), equal = __ballot(in && k == least), low = __ballot(j < m);
+    gt += __popcll(more);
+    eq += __popcll(equal);
+    gt_below += __popcll(more & low);
+    eq_below += __popcll(equal & low);
+  });
+  if (W > 1) {
+    if (lane == 0) {
+      s_gt[wave] = gt;
+      s_eq[wave] = eq;
+      s_gt_below[wave] = gt_below;
+      s_eq_below[wave] = eq_below;
+    }
+    __syncthreads();
+    gt = eq = gt_below = eq_below = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      gt += w < wave ? s_gt[w] : 0;
+      eq += w < wave ? s_eq[w] : 0;
+      gt_below += s_gt_below[w];
+      eq_below += s_eq_below[w];
+    }
+  } else {
+    gt = eq = 0;
+  }
+  const uint32_t stay_below = gt_below + min(eq_below, ties);  // of the places below m
+  if (tid == 0) a.moves[x.at] = m - stay_below;
+  list_moves(a, x, j0, j1, held, keys, least, ties, gt, eq, stay_below);
+  x.copy(j0, j1, lane, 64);
+}
+
+// Long lines in segments, a block each: those of the first m places, then those of
+// the others, so that no segment has places on both sides.
+struct Segment {
+  int lower;   // segments below m
+  int j0, j1;  // this one's places
+  __device__ __forceinline__ Segment(const Line& x, int segments, int seg) {
+    const int n = x.r.n, m = x.m;
+    lower = min(max((int)((int64_t)segments * m / n), 1), segments - 1);
+    const bool low = seg < lower;
+    const int base = low ? 0 : m, size = low ? m : n - m, parts = low ? lower : segments - lower, i = low ? seg : seg - lower;
+    const int each = ((size + parts - 1) / parts + 63) / 64 * 64;
+    j0 = __builtin_amdgcn_readfirstlane(base + (int)min((int64_t)i * each, (int64_t)size));
+    j1 = __builtin_amdgcn_readfirstlane(base + (int)min((int64_t)(i + 1) * each, (int64_t)size));
+  }
+};
+constexpr int bits_from(int round) { return round == 0 ? 21 : round == 1 ? 10 : 0; }
+constexpr uint32_t bits_mask(int round) { return round == 2 ? 1023u : 2047u; }
+
+// The bin of a round's histogram (of all segments) in which the last row that stays lies:
+// its bits join those known, and of the rows that stay those among the keys with them.
+template <int ROUND>
+__device__ __forceinline__ uint2 find_bin(const EvictArgs& a, const Line& x) {
+  __shared__ uint32_t s_wave[kSplitWaves];
+  __shared__ uint2 s_found;
+  constexpr int PER = kBins / kSplitThreads;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint2 known = ROUND == 0 ? make_uint2(0u, (uint32_t)x.m) : a.found[ROUND > 0 ? ROUND - 1 : 0][x.at];
+  const uint4* hist = reinterpret_cast<const uint4*>(a.hist[ROUND] + x.at * a.segments * kBins);
+  static_assert(PER == 4, "a thread's bins are a vector");
+  const int mine = kSplitThreads - 1 - tid;  // from the top
+  uint4 n = make_uint4(0, 0, 0, 0);
+#pragma unroll 8
+  for (int s = 0; s < a.segments; ++s) {
+    const uint4 o = hist[s * (kBins / 4) + mine];
+    n.x += o.x; n.y += o.y; n.z += o.z; n.w += o.w;
+  }
+  const uint32_t sum = n.x + n.y + n.z + n.w;
+  uint32_t incl = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t o = __shfl_up(incl, off, kWave);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 63) s_wave[wave] = incl;
+  __syncthreads();
+  uint32_t before = incl - sum;
+  for (int w = 0; w < wave; ++w) before += s_wave[w];
+  if (before < known.y && before + sum >= known.y) {
+    uint32_t bin = 4 * mine + 3, left = known.y - before;
+    if (left > n.w) { left -= n.w; --bin;
+      if (left > n.z) { left -= n.z; --bin;
+        if (left > n.y) { left -= n.y; --bin; } } }
+    s_found = make_uint2(known.x | bin << bits_from(ROUND), left);
+  }
+  __syncthreads();
+  return s_found;
+}
+
+// A round's histogram of a segment's keys, of those that have the bits known so far.
+template <int ROUND>
+__global__ __launch_bounds__(kSplitThreads) void split_count_kernel(EvictArgs a) {
+  __shared__ uint32_t s_keys[kSplitWaves][kWaveKeys];
+  __shared__ uint32_t bins[kBins], s_larger[kSplitWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = blockIdx.x / a.segments, seg = blockIdx.x - head * a.segments;
+  const Line x(a, head);
+  if (x.m == x.r.n || x.m == 0) return;
+  const Segment g(x, a.segments, seg);
+  uint32_t known = 0;
+  if constexpr (ROUND > 0) {
+    const uint2 found = find_bin<ROUND - 1>(a, x);
+    known = found.x;
+    if (seg == 0 && tid == 0) a.found[ROUND - 1][x.at] = found;
+  }
+  uint32_t larger = 0;
+  for (int b = tid; b < kBins; b += kSplitThreads) bins[b] = 0;
+  __syncthreads();
+  const int size = g.j1 - g.j0, share = ((size + kSplitWaves - 1) / kSplitWaves + 63) / 64 * 64;
+  const int j0 = min(g.j0 + wave * share, g.j1), j1 = min(j0 + share, g.j1);
+  sweep(x.r, j0, j1, false, s_keys[wave], [&](int, uint32_t k, bool there) {
+    constexpr int above = ROUND == 0 ? 0 : bits_from(ROUND - 1);
+    if (ROUND == 2) larger += __popcll(__ballot(there && k >> above > known >> above));
+    if (there && (ROUND == 0 || k >> above == known >> above)) {
+      const uint32_t bin = k >> bits_from(ROUND) & bits_mask(ROUND);
       // lanes with the first one's bin add at once
       const uint32_t first = __builtin_amdgcn_readfirstlane(bin);
       const uint64_t same = __ballot(bin == first);
@@ -115,98 +384,93 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(EvictArgs a) {
       else if (lane == __ffsll((unsigned long long)same) - 1)
         atomicAdd(&bins[bin], (uint32_t)__popcll(same));
     }
-    __syncthreads();
-    // from the top: the bin in which the last row that stays lies
-    const int per = kBins / blockDim.x;  // a thread's bins, neighbours
-    const int top = kBins - 1 - tid * per;
-    uint32_t mine = 0;
-    for (int b = 0; b < per; ++b) mine += bins[top - b];
-    uint32_t incl = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t o = __shfl_up(incl, off, kWave);
-      if (lane >= off) incl += o;
-    }
-    if (lane == 63) s_wave[wave] = incl;
-    __syncthreads();
-    uint32_t before = incl - mine;
-    for (int w = 0; w < wave; ++w) before += s_wave[w];
-    if (before < left && before + mine >= left) {
-      for (int b = 0; b < per; ++b) {
-        const uint32_t n = bins[top - b];
-        if (before + n >= left) {
-          s_bin = top - b;
-          s_left = left - before;
-          break;
-        }
-        before += n;
-      }
-    }
-    __syncthreads();
-    agreed |= s_bin << shift;
-    left = s_left;
-    __syncthreads();
+  });
+  if (ROUND == 2 && lane == 0) s_larger[wave] = larger;
+  __syncthreads();
+  if (ROUND == 2 && tid == 0) {
+    for (int w = 1; w < kSplitWaves; ++w) larger += s_larger[w];
+    a.larger[x.at * a.segments + seg] = larger;
   }
-  const uint32_t least = agreed, ties = left;  // keys above `least` stay, and the first `ties` that equal it
+  uint32_t* hist = a.hist[ROUND] + (x.at * a.segments + seg) * kBins;
+  for (int b = tid; b < kBins; b += kSplitThreads) hist[b] = bins[b];
+}
 
-  // each wave's places, a multiple of 64
-  const int share = ((r.n + waves - 1) / waves + 63) / 64 * 64;
-  const int j0 = min(wave * share, r.n), j1 = min(j0 + share, r.n);
-  uint32_t gt = 0, eq = 0, gt_below = 0, eq_below = 0;
-  for (int j = j0 + lane; j < j1; j += 64) {
-    const uint32_t k = r.key(j);
-    gt += k > least;
-    eq += k == least;
-    gt_below += k > least && j < m;
-    eq_below += k == least && j < m;
+// The lists' share of a segment.  What lies above and at the last row's key in each
+// segment, its histograms tell.
+__global__ __launch_bounds__(kSplitThreads) void split_list_kernel(EvictArgs a) {
+  __shared__ uint32_t s_keys[kSplitWaves][kWaveKeys];
+  __shared__ uint32_t s_gt[kMaxSegments], s_eq[kMaxSegments], s_wgt[kSplitWaves], s_weq[kSplitWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = blockIdx.x / a.segments, seg = blockIdx.x - head * a.segments;
+  const Line x(a, head);
+  const int n = x.r.n, m = x.m;
+  if (tid == 0 && blockIdx.x == 0 && x.layer == 0) a.stay[x.seq] = m;
+  if (m == n || m == 0) {
+    if (tid == 0 && seg == 0) a.moves[x.at] = 0;
+    x.copy(0, m, seg * kSplitThreads + tid, a.segments * kSplitThreads);
+    return;
   }
+  const Segment g(x, a.segments, seg);
+  const uint2 found = find_bin<2>(a, x);
+  const uint32_t least = found.x, ties = found.y;
+  // larger and equal keys of each segment, a wave each
+  const int last = least & bits_mask(2);
+  for (int s = wave; s < a.segments; s += kSplitWaves) {
+    const uint4* hist = reinterpret_cast<const uint4*>(a.hist[2] + (x.at * a.segments + s) * kBins);
+    uint32_t above = 0, equal = 0;
 #pragma unroll
-  for (int off = 32; off; off >>= 1) {
-    gt += __shfl_xor(gt, off, kWave);
-    eq += __shfl_xor(eq, off, kWave);
-    gt_below += __shfl_xor(gt_below, off, kWave);
-    eq_below += __shfl_xor(eq_below, off, kWave);
-  }
-  if (lane == 0) {
-    s_gt[wave] = gt;
-    s_eq[wave] = eq;
-    s_gt_below[wave] = gt_below;
-    s_eq_below[wave] = eq_below;
+    for (int u = 0; u < 4; ++u) {
+      const int b = 4 * (64 * u + lane);
+      const uint4 n = hist[64 * u + lane];
+      above += (b > last ? n.x : 0) + (b + 1 > last ? n.y : 0) + (b + 2 > last ? n.z : 0) + (b + 3 > last ? n.w : 0);
+      equal += (b == last ? n.x : 0) + (b + 1 == last ? n.y : 0) + (b + 2 == last ? n.z : 0) + (b + 3 == last ? n.w : 0);
+    }
+#pragma unroll
+    for (int off = 32; off; off >>= 1) {
+      above += __shfl_xor(above, off, kWave);
+      equal += __shfl_xor(equal, off, kWave);
+    }
+    if (lane == 0) {
+      s_gt[s] = above + a.larger[x.at * a.segments + s];
+      s_eq[s] = equal;
+    }
   }
   __syncthreads();
-  gt = eq = gt_below = eq_below = 0;
-  for (int w = 0; w < waves; ++w) {
-    if (w < wave) {
-      gt += s_gt[w];
-      eq += s_eq[w];
+  uint32_t gt = 0, eq = 0, gt_below = 0, eq_below = 0;
+  for (int s = 0; s < a.segments; ++s) {
+    if (s < seg) {
+      gt += s_gt[s];
+      eq += s_eq[s];
     }
-    gt_below += s_gt_below[w];
-    eq_below += s_eq_below[w];
+    if (s < g.lower) {
+      gt_below += s_gt[s];
+      eq_below += s_eq[s];
+    }
   }
   const uint32_t stay_below = gt_below + min(eq_below, ties);  // of the places below m
-  if (tid == 0) a.moves[line] = m - stay_below;
-  int32_t *to = a.to + line * a.list_stride, *from = a.from + line * a.list_stride;
-  for (int j = j0 + lane; j - lane < j1; j += 64) {
-    const bool in = j < j1;
-    const uint32_t k = in ? r.key(j) : 0;
-    const bool more = in && k > least, equal = in && k == least;
-    const uint64_t below = (1ull << lane) - 1, vote_gt = __ballot(more), vote_eq = __ballot(equal);
-    const uint32_t gt_before = gt + __popcll(vote_gt & below), eq_before = eq + __popcll(vote_eq & below);
-    const uint32_t before = gt_before + min(eq_before, ties);
-    const bool stays = more || (equal && eq_before < ties);
-    if (in && j < m) {
-      if (!stays) {
-        to[j - before] = j;
-      } else {
-        if (apart) weights_out[j] = r.weights[j];
-        if (apart_born) born_out[j] = r.born[j];
-      }
-    } else if (stays) {
-      from[before - stay_below] = j;
-    }
-    gt += __popcll(vote_gt);
-    eq += __popcll(vote_eq);
+  if (tid == 0 && seg == 0) a.moves[x.at] = m - stay_below;
+  // its waves' shares in turn
+  const int size = g.j1 - g.j0, share = ((size + kSplitWaves - 1) / kSplitWaves + 63) / 64 * 64;
+  const int j0 = min(g.j0 + wave * share, g.j1), j1 = min(j0 + share, g.j1);
+  const bool held = share <= kWaveKeys;
+  uint32_t* const keys = s_keys[wave];
+  if (held) x.r.load(j0, j1, keys);
+  uint32_t wgt = 0, weq = 0;
+  sweep(x.r, j0, j1, held, keys, [&](int, uint32_t k, bool in) {
+    wgt += __popcll(__ballot(in && k > least));
+    weq += __popcll(__ballot(in && k == least));
+  });
+  if (lane == 0) {
+    s_wgt[wave] = wgt;
+    s_weq[wave] = weq;
   }
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) {
+    gt += s_wgt[w];
+    eq += s_weq[w];
+  }
+  list_moves(a, x, j0, j1, held, keys, least, ties, gt, eq, stay_below);
+  x.copy(j0, j1, lane, 64);
 }
 
 // Moves the rows of a line's list, 16 bytes of a key and of a value a lane at a time.
@@ -242,6 +506,13 @@ uint64_t align16(uint64_t n) { return (n + 15) / 16 * 16; }
 uint64_t most_moves(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p) {
   return std::min<uint64_t>(p.weight_stride, (uint64_t)c.table_stride * c.page_rows) / 2 + 1;
 }
+// Segments of a line; 1: its block's registers hold it, or lines enough fill the chip.
+int segments_of(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p) {
+  const uint64_t len = std::min<uint64_t>({p.max_length, p.weight_stride, (uint64_t)c.table_stride * c.page_rows});
+  const uint64_t lines = (uint64_t)p.layers * p.seqs * c.kv_heads;
+  if (len <= 16 * kWaveKeys) return 1;
+  return (int)std::min<uint64_t>({(len + kSplitKeys - 1) / kSplitKeys, (uint64_t)kMaxSegments, std::max<uint64_t>(2, 4096 / lines)});
+}
 bool evict_in_range(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p) {
   return p.seqs <= 65535 && p.layers >= 1 && p.layers <= 16384 && (uint64_t)p.layers * p.seqs * c.kv_heads <= (1u << 24) &&
          p.weight_stride >= 1 && p.weight_stride <= (1u << 30);
@@ -257,7 +528,9 @@ uint64_t kv_evict_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p
   }
   if (p.seqs == 0 || !evict_in_range(c, p)) return 0;
   const uint64_t lines = (uint64_t)p.layers * p.seqs * c.kv_heads;
-  return 2 * align16(lines * most_moves(c, p) * 4) + align16(lines * 4) + align16(p.seqs * 4);
+  const uint64_t segments = (uint64_t)segments_of(c, p);
+  return 2 * align16(lines * most_moves(c, p) * 4) + align16(lines * 4) + align16(p.seqs * 4) +
+         (segments > 1 ? 3 * lines * segments * kBins * 4 + 2 * align16(lines * 8) + align16(lines * segments * 4) : 0);
 }
 
 void kv_evict(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p, hipStream_t s) {
@@ -315,10 +588,34 @@ void kv_evict(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p, hipStream_t 
   a.moves = reinterpret_cast<int32_t*>(w);
   w += align16(lines * 4);
   a.stay = reinterpret_cast<int32_t*>(w);
+  w += align16(p.seqs * 4);
   const uint64_t len = std::min<uint64_t>({p.max_length, p.weight_stride, (uint64_t)c.table_stride * c.page_rows});
-  // as many threads as a thread has about eight places each
-  const int threads = len <= 2048 ? 256 : len <= 4096 ? 512 : kChooseThreads;
-  hipLaunchKernelGGL(choose_kernel, dim3(c.kv_heads, p.seqs, p.layers), dim3(threads), 0, s, a);
+  a.segments = segments_of(c, p);
+  const dim3 grid(c.kv_heads * a.segments, p.seqs, p.layers);
+  if (a.segments > 1) {
+    for (int round = 0; round < 3; ++round) {
+      a.hist[round] = reinterpret_cast<uint32_t*>(w);
+      w += lines * a.segments * kBins * 4;
+    }
+    for (int round = 0; round < 2; ++round) {
+      a.found[round] = reinterpret_cast<uint2*>(w);
+      w += align16(lines * 8);
+    }
+    a.larger = reinterpret_cast<uint32_t*>(w);
+    hipLaunchKernelGGL((split_count_kernel<0>), grid, dim3(kSplitThreads), 0, s, a);
+    kv_launched(hipGetLastError());
+    hipLaunchKernelGGL((split_count_kernel<1>), grid, dim3(kSplitThreads), 0, s, a);
+    kv_launched(hipGetLastError());
+    hipLaunchKernelGGL((split_count_kernel<2>), grid, dim3(kSplitThreads), 0, s, a);
+    kv_launched(hipGetLastError());
+    hipLaunchKernelGGL(split_list_kernel, grid, dim3(kSplitThreads), 0, s, a);
+  } else if (len <= kWaveKeys) {
+    hipLaunchKernelGGL((choose_kernel<1>), grid, dim3(64), 0, s, a);
+  } else if (len <= 4 * kWaveKeys) {
+    hipLaunchKernelGGL((choose_kernel<4>), grid, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((choose_kernel<16>), grid, dim3(1024), 0, s, a);
+  }
   kv_launched(hipGetLastError());
   const uint64_t per = kMoveThreads / a.row16;
   const uint64_t wanted = std::max<uint64_t>(1, 8192 / lines);  // blocks of a line, for as many moves as half its places at most

@@ -258,3 +258,21 @@ def test_offsets_past_32_bits(mit2, ctx):
     finally:
         del big, far
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("length,hint", [(16500, 16500), (40000, 40000), (20000, 100000), (3000, 100000), (100, 1 << 30), (20000, 500), (20000, 3000)])
+@pytest.mark.parametrize("born", [False, True])
+def test_lines_in_segments_and_hints_that_are_off(mit2, ctx, length, hint, born):
+    """Lines longer than a block holds, in segments; and shorter and longer ones than their launch was laid out for."""
+    Cut(mit2, [length, length - 77, 5], [length // 2 + 3, length - 78, 2], layers=1, heads=1, page=128, first=5, last=60, born=born, hint=hint, seed=length,
+        capacity=[max(length, hint) if hint < 1 << 20 else length]).check(ctx)
+
+
+@pytest.mark.parametrize("kind", ["equal", "few", "wild"])
+@pytest.mark.parametrize("part", [0.001, 0.5, 0.999])
+def test_equal_and_wild_weights_in_segments(mit2, ctx, kind, part):
+    rng = np.random.default_rng(5)
+    shape = (1, 1, 2, 33000)
+    w = {"equal": np.full(shape, 0.25), "few": rng.integers(0, 3, shape) * 0.5,
+         "wild": rng.choice([np.nan, np.inf, -np.inf, 1e-45, -1e-45, 0.0, -0.0, 3e38, 1.0, 1.0000001, -1.0], shape)}[kind].astype(np.float32)
+    Cut(mit2, [32900], [int(32900 * part)], layers=1, page=128, weights=w, seed=1).check(ctx)
