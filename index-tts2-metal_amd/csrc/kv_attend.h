@@ -33,16 +33,21 @@ struct AttendArgs {
   float scale2;        // |scale| log2(e): scores in powers of two
 };
 
-// Either half of the attention of sequences that share their first rows (kv_prefix.h):
-// the shared rows, for all new rows of a group of sequences at once, or what each
-// sequence has of its own.  Both leave parts, for one join.
+// Attention of sequences that share their first rows (kv_prefix.h), in one launch: first
+// the blocks of the shared rows, each for new rows of all a group's sequences, then
+// those of what each sequence has of its own.  Both leave parts, for one join.
 struct PrefixArgs : AttendArgs {
   const int32_t* bounds;  // [groups + 1] first sequences of the groups
   const int32_t* shared;  // [groups] rows that a group's sequences share
   int groups;
-  int own;                // the second half
-  int slots, slot0;       // parts of a query row, and this half's first
+  int step;               // shared rows are taken in whole runs of this
+  AttendPlan own;         // (the kernels' plan is the shared rows')
+  uint32_t shared_blocks, blocks;
+  size_t pairs;           // query rows x heads
 };
+
+template <typename A>
+constexpr int wide_blocks = std::is_same<A, PrefixArgs>::value ? 3 : 2;  // of a CU
 
 // What splits leave for their join: [row][query head][split] outputs, maxima and
 // weights' sums, [row][query head] the number of splits.
@@ -170,6 +175,7 @@ struct Part {
   int begin, end;        // the split's keys
   int parts;             // splits that hold keys
   bool whole;            // one split holds all keys: results are final
+  bool own;              // (of shared prefixes) a sequence's own rows
 };
 __device__ __forceinline__ bool find_part(const AttendArgs& a, const AttendPlan& plan, int mtile, Part& p) {
   int tile = blockIdx.x, unit = blockIdx.y;
@@ -199,120 +205,200 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, const AttendPlan&
   return p.split == 0 || p.begin < p.len;
 }
 
-// Where a split's part goes, and whether the block says how many there are.
+// Where a split's part goes, and how many of them there are.
 __device__ __forceinline__ size_t slot_of(const AttendArgs&, const AttendPlan& plan, const Part& p, size_t pair) {
   return pair * plan.splits + p.split;
 }
-__device__ __forceinline__ bool tells_parts(const AttendArgs&, const AttendPlan& plan, const Part& p) {
-  return p.split == 0 && plan.splits > 1;
+__device__ __forceinline__ void tell_parts(const AttendArgs&, const AttendPlan& plan, const Part& p, const Parts& part, size_t pair) {
+  if (p.split == 0 && plan.splits > 1) part.n[pair] = p.parts;
 }
 
-// Rows that the sequences lo .. hi - 1 may share: as many as said, of those before any
-// of their new rows, in whole runs of kSharedStep.  (The same for all lanes.)
-constexpr int kSharedStep = 64;
-__device__ __forceinline__ int shared_rows(const RowView& r, int lo, int hi, int said, int capacity) {
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int off = 32; off; off >>= 1) x = min(x, __shfl_xor(x, off, kWave));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+// Of 64 (or fewer) runs of n tiles, lane by lane: the one that holds tile t, and the
+// tiles before it; -1: none does, `before` then counts them all.
+__device__ __forceinline__ int run_of(int n, int t, int& before) {
   const int lane = threadIdx.x & 63;
-  int least = min(said, capacity);
-  for (int base = lo; base < hi; base += 64) {
-    const int s = base + lane;
-    if (s < hi) {
-      const int s0 = r.start[s], s1 = r.start[s + 1];
-      if (s1 > s0) least = min(least, r.length[s] - (s1 - s0));
+  int incl = n;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(incl, off, kWave);
+    if (lane >= off) incl += o;
+  }
+  const uint64_t past = __ballot(before + incl > t);
+  if (!past) {
+    before += __builtin_amdgcn_readlane(incl, 63);
+    return -1;
+  }
+  const int l = __ffsll((unsigned long long)past) - 1;
+  before += __builtin_amdgcn_readlane(incl - n, l);
+  return l;
+}
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, int start, int stop, int mtile) {
+  const int rows = min(stop, a.r.rows) - max(start, 0);
+  return rows > 0 ? (int)(((int64_t)rows * a.group + mtile - 1) / mtile) : 0;
+}
+
+// What a wave's lanes hold of the sequences and groups where neither are more than 64:
+// asked for at once (looked up one from the other, they are three waits in a row).
+struct Few {
+  bool all;                 // they are no more
+  int start, stop, length;  // sequence `lane`'s
+  int lo, hi, said;         // group `lane`'s
+  __device__ __forceinline__ Few(const PrefixArgs& a) {
+    const int lane = threadIdx.x & 63;
+    all = a.r.seqs <= 64 && a.groups <= 64;
+    start = stop = length = lo = hi = said = 0;
+    if (!all) return;
+    const int s = min(lane, a.r.seqs - 1);
+    start = a.r.start[s];
+    stop = a.r.start[s + 1];
+    length = a.r.length[s];
+    if (a.groups > 0) {
+      const int g = min(lane, a.groups - 1);
+      lo = a.bounds[g];
+      hi = a.bounds[g + 1];
+      said = a.shared[g];
+    }
+    if (lane >= a.r.seqs) start = stop = 0;
+    if (lane >= a.groups) lo = hi = 0;
+  }
+};
+
+// Rows that the sequences lo .. hi - 1 may share: as many as said, of those before any
+// of their new rows, in whole runs of `step`.  (The same for all lanes.)
+__device__ __forceinline__ int shared_rows(const PrefixArgs& a, const Few& few, int lo, int hi, int said) {
+  const int lane = threadIdx.x & 63;
+  int least = min(said, a.c.capacity());
+  if (few.all) {
+    if (lane >= lo && lane < hi && few.stop > few.start) least = min(least, few.length - (few.stop - few.start));
+  } else {
+    for (int base = lo; base < hi; base += 64) {
+      const int s = base + lane;
+      if (s < hi) {
+        const int s0 = a.r.start[s], s1 = a.r.start[s + 1];
+        if (s1 > s0) least = min(least, a.r.length[s] - (s1 - s0));
+      }
     }
   }
-#pragma unroll
-  for (int off = 32; off; off >>= 1) least = min(least, __shfl_xor(least, off, kWave));
-  return __builtin_amdgcn_readfirstlane(max(least, 0) / kSharedStep * kSharedStep);
+  return max(wave_min(least), 0) & -a.step;
 }
-// A block's part of either half (see Part).  Shared rows: a group's new rows as if they
-// were one sequence's, all of which see all keys.
-__device__ __forceinline__ bool find_part(const PrefixArgs& a, const AttendPlan& plan, int mtile, Part& p) {
-  int tile = blockIdx.x, unit = blockIdx.y;
-  if (plan.by_xcd) {
-    const int slot = blockIdx.x >> 3;
-    unit = slot / plan.tiles * 8 + (blockIdx.x & 7);
-    tile = slot % plan.tiles;
-    if (unit >= a.c.kv_heads * plan.splits) return false;
-  }
+// A sequence's own rows (see Part).
+__device__ __forceinline__ bool find_own(const PrefixArgs& a, const Few& few, int mtile, int tile, Part& p) {
   const int lane = threadIdx.x & 63;
-  p.kvh = unit % a.c.kv_heads;
-  p.split = unit / a.c.kv_heads;
-  p.whole = false;
-  if (a.own) {
-    Found f;
-    if (!find_tile(a.r, a.group, mtile, tile, f)) return false;
-    p.seq = f.seq;
-    p.raw_start = f.start;
-    p.start = max(f.start, 0);
-    p.mrows = (min(f.stop, a.r.rows) - p.start) * a.group;
-    p.m0 = f.in_seq * mtile;
-    p.first = f.length - (f.stop - f.start);
-    p.len = min(f.length, a.c.capacity());
-    int from = 0;  // the group's shared rows
-    for (int base = 0; base < a.groups; base += 64) {
-      int lo = 0, hi = 0, said = 0;
+  Found f;
+  if (few.all) {
+    int before = 0;
+    const int l = run_of(tiles_of(a, few.start, few.stop, mtile), tile, before);
+    if (l < 0) return false;
+    f.seq = l;
+    f.in_seq = tile - before;
+    f.start = __builtin_amdgcn_readlane(few.start, l);
+    f.stop = __builtin_amdgcn_readlane(few.stop, l);
+    f.length = __builtin_amdgcn_readlane(few.length, l);
+  } else if (!find_tile(a.r, a.group, mtile, tile, f)) {
+    return false;
+  }
+  p.seq = f.seq;
+  p.raw_start = f.start;
+  p.start = max(f.start, 0);
+  p.mrows = (min(f.stop, a.r.rows) - p.start) * a.group;
+  p.m0 = f.in_seq * mtile;
+  p.first = f.length - (f.stop - f.start);
+  p.len = min(f.length, a.c.capacity());
+  int from = 0;  // the group's shared rows
+  for (int base = 0; base < a.groups; base += 64) {
+    int lo = few.lo, hi = few.hi, said = few.said;
+    if (!few.all) {
+      lo = hi = 0;
       if (base + lane < a.groups) {
         lo = a.bounds[base + lane];
         hi = a.bounds[base + lane + 1];
         said = a.shared[base + lane];
       }
-      const uint64_t mine = __ballot(lo <= f.seq && f.seq < hi);
-      if (!mine) continue;
-      const int l = __ffsll((unsigned long long)mine) - 1;
-      from = shared_rows(a.r, max(__builtin_amdgcn_readlane(lo, l), 0), min(__builtin_amdgcn_readlane(hi, l), a.r.seqs),
-                         __builtin_amdgcn_readlane(said, l), a.c.capacity());
-      break;
     }
-    const int chunk = chunk_of(p.len - from, plan.chunk, plan.splits);
-    p.begin = min(from + p.split * chunk, max(p.len, from));
-    p.end = min(p.begin + chunk, p.len);
-    // (bit 16: there are shared rows)
-    p.parts = max(1, (p.len - from + chunk - 1) / chunk) | (from > 0 ? 1 << 16 : 0);
-    return p.split == 0 || p.begin < p.len;
+    const uint64_t mine = __ballot(lo <= f.seq && f.seq < hi);
+    if (!mine) continue;
+    const int l = __ffsll((unsigned long long)mine) - 1;
+    from = shared_rows(a, few, max(__builtin_amdgcn_readlane(lo, l), 0), min(__builtin_amdgcn_readlane(hi, l), a.r.seqs),
+                       __builtin_amdgcn_readlane(said, l));
+    break;
   }
+  const int chunk = chunk_of(p.len - from, a.own.chunk, a.own.splits);
+  p.begin = min(from + p.split * chunk, max(p.len, from));
+  p.end = min(p.begin + chunk, p.len);
+  // (bit 16: there are shared rows)
+  p.parts = max(1, (p.len - from + chunk - 1) / chunk) | (from > 0 ? 1 << 16 : 0);
+  return p.split == 0 || p.begin < p.len;
+}
+// A group's shared rows: its new rows are as one sequence's, and see all of them.
+__device__ __forceinline__ bool find_shared(const PrefixArgs& a, const AttendPlan& plan, const Few& few, int mtile, int tile, Part& p) {
+  const int lane = threadIdx.x & 63;
   int before = 0;
   for (int base = 0; base < a.groups; base += 64) {
-    int n = 0, s0 = 0, lo = 0, hi = 0, said = 0;
-    if (base + lane < a.groups) {
-      lo = max(a.bounds[base + lane], 0);
-      hi = min(a.bounds[base + lane + 1], a.r.seqs);
-      said = a.shared[base + lane];
-      if (lo < hi && said >= kSharedStep) {
-        s0 = a.r.start[lo];
-        const int rows = min(a.r.start[hi], a.r.rows) - max(s0, 0);
-        n = rows > 0 ? (int)(((int64_t)rows * a.group + mtile - 1) / mtile) : 0;
-        p.mrows = rows * a.group;
+    int lo = few.lo, hi = few.hi, said = few.said, start = 0, stop = 0;
+    if (!few.all) {
+      lo = hi = 0;
+      if (base + lane < a.groups) {
+        lo = a.bounds[base + lane];
+        hi = a.bounds[base + lane + 1];
+        said = a.shared[base + lane];
       }
     }
-    int incl = n;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(incl, off, kWave);
-      if (lane >= off) incl += o;
+    lo = max(lo, 0);
+    hi = min(hi, a.r.seqs);
+    const bool some = lo < hi && said >= a.step;
+    if (few.all) {
+      start = __shfl(few.start, lo & 63, kWave);
+      stop = __shfl(few.stop, (hi - 1) & 63, kWave);
+    } else if (some) {
+      start = a.r.start[lo];
+      stop = a.r.start[hi];
     }
-    const uint64_t past = __ballot(before + incl > tile);
-    if (past) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      p.seq = __builtin_amdgcn_readlane(lo, l);
-      p.raw_start = __builtin_amdgcn_readlane(s0, l);
-      p.start = max(p.raw_start, 0);
-      p.mrows = __builtin_amdgcn_readlane(p.mrows, l);
-      p.m0 = (tile - before - __builtin_amdgcn_readlane(incl - n, l)) * mtile;
-      p.len = p.first = shared_rows(a.r, p.seq, __builtin_amdgcn_readlane(hi, l), __builtin_amdgcn_readlane(said, l), a.c.capacity());
-      const int chunk = chunk_of(p.len, plan.chunk, plan.splits);
-      p.begin = p.split * chunk;
-      p.end = min(p.begin + chunk, p.len);
-      p.parts = (p.len + chunk - 1) / chunk;
-      return p.begin < p.len;
-    }
-    before += __builtin_amdgcn_readlane(incl, 63);
+    const int l = run_of(some ? tiles_of(a, start, stop, mtile) : 0, tile, before);
+    if (l < 0) continue;
+    p.seq = __builtin_amdgcn_readlane(lo, l);
+    p.raw_start = __builtin_amdgcn_readlane(start, l);
+    p.start = max(p.raw_start, 0);
+    p.mrows = (min(__builtin_amdgcn_readlane(stop, l), a.r.rows) - p.start) * a.group;
+    p.m0 = (tile - before) * mtile;
+    p.len = p.first = shared_rows(a, few, p.seq, __builtin_amdgcn_readlane(hi, l), __builtin_amdgcn_readlane(said, l));
+    const int chunk = chunk_of(p.len, plan.chunk, plan.splits);
+    p.begin = p.split * chunk;
+    p.end = min(p.begin + chunk, p.len);
+    p.parts = (p.len + chunk - 1) / chunk;
+    return p.begin < p.len;
   }
   return false;
 }
-__device__ __forceinline__ size_t slot_of(const PrefixArgs& a, const AttendPlan&, const Part& p, size_t pair) {
-  return pair * a.slots + a.slot0 + p.split;
+__device__ __forceinline__ bool find_part(const PrefixArgs& a, const AttendPlan& shared, int mtile, Part& p) {
+  uint32_t id = blockIdx.y * gridDim.x + blockIdx.x;
+  if (id >= a.blocks) return false;
+  const Few few(a);
+  p.own = id >= a.shared_blocks;
+  if (p.own) id -= a.shared_blocks;
+  const AttendPlan& plan = p.own ? a.own : shared;
+  int tile = id % plan.tiles, unit = id / plan.tiles;
+  if (plan.by_xcd) {
+    const int slot = id >> 3;
+    unit = slot / plan.tiles * 8 + (id & 7);
+    tile = slot % plan.tiles;
+    if (unit >= a.c.kv_heads * plan.splits) return false;
+  }
+  p.kvh = unit % a.c.kv_heads;
+  p.split = unit / a.c.kv_heads;
+  p.whole = false;
+  return p.own ? find_own(a, few, mtile, tile, p) : find_shared(a, shared, few, mtile, tile, p);
 }
-__device__ __forceinline__ bool tells_parts(const PrefixArgs&, const AttendPlan&, const Part& p) { return p.split == 0; }
+__device__ __forceinline__ size_t slot_of(const PrefixArgs& a, const AttendPlan& shared, const Part& p, size_t pair) {
+  return pair * (shared.splits + a.own.splits) + (p.own ? shared.splits : 0) + p.split;
+}
+__device__ __forceinline__ void tell_parts(const PrefixArgs& a, const AttendPlan&, const Part& p, const Parts& part, size_t pair) {
+  if (p.split == 0) part.n[pair + (p.own ? a.pairs : 0)] = p.parts;
+}
 
 // A lane's query: its row in the buffers, its place among the sequence's new
 // rows (as given), its head.
@@ -709,7 +795,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(A a, AttendPlan 
         for (int d = 0; d < DP; ++d) part.o[at * D + d0 + d] = O[d];
         if ((tid & 15) == 0) part.ml[at] = make_float2(mm, L);
       }
-      if (tells_parts(a, plan, p) && (tid & 15) == 0) part.n[(size_t)x.row * a.q_heads + x.h] = p.parts;
+      if ((tid & 15) == 0) tell_parts(a, plan, p, part, (size_t)x.row * a.q_heads + x.h);
     }
   }
 }
@@ -756,8 +842,9 @@ __device__ __forceinline__ void load_to_lds(const void* src, lds_ptr_t* lds) {
 //
 // The ring's buffers are objects of their own, named by constants in the usual
 // path: a read that might alias any of them would wait for every load.
-template <typename T, int D, typename A>
-__global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(A a, AttendPlan plan, Parts part) {
+template <typename T, int D, int WMT, typename A>
+__device__ __forceinline__ void attend_wide(const A& a, const AttendPlan& plan, const Parts& part, Part p, u32x4* sK0, u32x4* sK1,
+                                            u32x4* sK2, u32x4* sV0, u32x4* sV1, u32x4* sV2) {
   typedef Dims<T, D> S;
   typedef typename Mat<T>::op Op;
   constexpr int KT = S::KT, NT = S::NT, DP = S::DP, DC = S::DC, NV = S::NV;
@@ -766,15 +853,10 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(A a, Att
   constexpr int KEYS = 512 / CPR;                 // keys of a buffer: 8 KB each of keys and values
   constexpr int STEP = kAttendThreads / CPR;      // rows a pass of the block loads
   constexpr int PASSES = KEYS / STEP;             // 2
-  constexpr int WMT = wide_rows(sizeof(T) == 4) / (16 * kAttendWaves);
   constexpr int XM = CPR < 16 ? CPR - 1 : 15;
-  __shared__ __attribute__((aligned(1024))) u32x4 sK0[KEYS * CPR], sK1[KEYS * CPR], sK2[KEYS * CPR];
-  __shared__ __attribute__((aligned(1024))) u32x4 sV0[KEYS * CPR], sV1[KEYS * CPR], sV2[KEYS * CPR];
   auto bufK = [&](int b) -> u32x4* { return b == 0 ? sK0 : b == 1 ? sK1 : sK2; };
   auto bufV = [&](int b) -> u32x4* { return b == 0 ? sV0 : b == 1 ? sV1 : sV2; };
 
-  Part p;
-  if (!find_part(a, plan, 16 * WMT * kAttendWaves, p)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lq = lane & 15, grp = lane >> 4;
   const int wm0 = p.m0 + 16 * WMT * wave;
@@ -1030,8 +1112,19 @@ __global__ __launch_bounds__(kAttendThreads, 2) void attend_wide_kernel(A a, Att
               floatx4{run[mt].o[d][r], run[mt].o[d + 1][r], run[mt].o[d + 2][r], run[mt].o[d + 3][r]};
       if (grp == 0) part.ml[at] = make_float2(run[mt].mx, L);
     }
-    if (tells_parts(a, plan, p) && grp == 0) part.n[(size_t)x.row * a.q_heads + x.h] = p.parts;
+    if (grp == 0) tell_parts(a, plan, p, part, (size_t)x.row * a.q_heads + x.h);
   }
+}
+
+template <typename T, int D, typename A>
+__global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_kernel(A a, AttendPlan plan, Parts part) {
+  constexpr int PLACES = 512;  // of 16 bytes
+  constexpr int WMT = (std::is_same<A, PrefixArgs>::value ? kPrefixRows : wide_rows(sizeof(T) == 4)) / (16 * kAttendWaves);
+  __shared__ __attribute__((aligned(1024))) u32x4 sK0[PLACES], sK1[PLACES], sK2[PLACES];
+  __shared__ __attribute__((aligned(1024))) u32x4 sV0[PLACES], sV1[PLACES], sV2[PLACES];
+  Part p;
+  if (!find_part(a, plan, 16 * WMT * kAttendWaves, p)) return;
+  attend_wide<T, D, WMT>(a, plan, part, p, sK0, sK1, sK2, sV0, sV1, sV2);
 }
 
 // Joins a row and query head's splits, WAVES waves for each: lane groups of D/4
@@ -1100,8 +1193,7 @@ void attend_launched(hipError_t e);  // throws HipError (kv_ops.hip)
 
 // The launch of a plan's blocks.
 template <typename T, int D, typename A>
-void launch_tiles(const A& a, const AttendPlan& plan, const Parts& part, hipStream_t s) {
-  const AttendGrid g = attend_grid(plan, a.c.kv_heads);
+void launch_tiles(const A& a, const AttendPlan& plan, const Parts& part, AttendGrid g, hipStream_t s) {
   const dim3 grid(g.x, g.y), block(kAttendThreads);
   const bool big = (1 << a.c.page_shift) >= Mat<T>::KT;
   auto tiles = [&](auto big_page) {
@@ -1128,7 +1220,7 @@ void launch_attend(const AttendArgs& a, const AttendPlan& plan, void* workspace,
   part.o = static_cast<float*>(workspace);
   part.ml = reinterpret_cast<float2*>(part.o + n * D);
   part.n = reinterpret_cast<int32_t*>(part.ml + n);
-  launch_tiles<T, D>(a, plan, part, s);
+  launch_tiles<T, D>(a, plan, part, attend_grid(plan, a.c.kv_heads), s);
   if (plan.splits == 1) return;
   if (plan.splits <= kFewSplits)
     hipLaunchKernelGGL((combine_kernel<T, D, 1>), dim3(a.r.rows, a.q_heads), dim3(64), 0, s, a, plan, part);

@@ -7,27 +7,6 @@
 
 namespace mit2hip {
 
-// How the two halves are laid out.
-struct PrefixPlan {
-  AttendPlan shared, own;
-  bool shares;  // there may be shared rows
-  int slots() const { return (shares ? shared.splits : 0) + own.splits; }
-};
-inline PrefixPlan prefix_plan(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads, const mit2cfm_kv_prefix& x) {
-  PrefixPlan p{};
-  p.shares = x.groups > 0;
-  mit2cfm_kv_rows some = r;
-  if (p.shares) {
-    some.seqs = x.groups;
-    some.max_length = x.max_shared;
-    p.shared = attend_plan(c, some, q_heads);
-  }
-  some.seqs = r.seqs;
-  some.max_length = !p.shares ? r.max_length : r.max_length > x.max_shared ? r.max_length - x.max_shared + 63 : 64;
-  p.own = attend_plan(c, some, q_heads);
-  return p;
-}
-
 // Launches both halves and their join; throws HipError.  lse may be NULL.
 void launch_prefix_f32(const PrefixArgs& a, const PrefixPlan& plan, int D, void* workspace, float* lse, hipStream_t s);
 void launch_prefix_f16(const PrefixArgs& a, const PrefixPlan& plan, int D, void* workspace, float* lse, hipStream_t s);
@@ -35,37 +14,58 @@ void launch_prefix_bf16(const PrefixArgs& a, const PrefixPlan& plan, int D, void
 
 #if defined(KV_ATTEND_KERNELS)
 
-// Joins the parts of a row and query head, a wave each: those of the shared rows, then
-// its sequence's own.  Lane groups of D/4 take every so manyth part, four elements a lane.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void join_kernel(PrefixArgs a, Parts part, const int32_t* shared_parts, float* lse) {
-  constexpr int L4 = D / 4, G = 64 / L4;
+// Joins the parts of a row and query head: those of the shared rows, then its
+// sequence's own.  Lane groups of D/4 take every so manyth part, four elements a lane,
+// AHEAD of them at once; WAVES of them for more parts than those.
+constexpr int kJoinFew = 16;
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void join_kernel(PrefixArgs a, int shared_splits, Parts part, float* lse) {
+  constexpr int L4 = D / 4, G = WAVES * 64 / L4, AHEAD = 8;
   __shared__ floatx4 sO[G][L4];
-  __shared__ float sF[2 * kMostSplits];
+  __shared__ float sF[2 * kMostSplits], sM[WAVES], sL[WAVES];
   const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  if (row < a.r.start[0] || row >= a.r.start[a.r.seqs]) return;  // nobody's row
-  const size_t pair = (size_t)row * a.q_heads + h, at = pair * a.slots;
-  const int told = part.n[pair], shared = told >> 16 ? min(max(shared_parts[pair], 0), a.slot0) : 0;
-  const int n = shared + min(told & 0xffff, a.slots - a.slot0);
-  auto slot = [&](int i) { return at + (i < shared ? i : a.slot0 + i - shared); };
+  const size_t pair = (size_t)row * a.q_heads + h, at = pair * (shared_splits + a.own.splits);
+  const int first = a.r.start[0], last = a.r.start[a.r.seqs];
+  const int told = part.n[pair + a.pairs];
+  const int shared_told = shared_splits ? part.n[pair] : 0;
+  if (row < first || row >= last) return;  // nobody's row
+  const int shared = told >> 16 ? min(max(shared_told, 0), shared_splits) : 0;
+  const int n = shared + min(told & 0xffff, a.own.splits);
+  auto slot = [&](int i) { return at + (i < shared ? i : shared_splits + i - shared); };
+  const int g = tid / L4, l4 = tid - g * L4;
+  floatx4 x[AHEAD];
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) x[u] = reinterpret_cast<const floatx4*>(part.o + slot(max(min(g + u * G, n - 1), 0)) * D)[l4];
   float mm = -INFINITY;
-  for (int i = tid; i < n; i += 64) mm = fmaxf(mm, part.ml[slot(i)].x);
+  for (int i = tid; i < n; i += WAVES * 64) mm = fmaxf(mm, part.ml[slot(i)].x);
 #pragma unroll
   for (int off = 32; off; off >>= 1) mm = fmaxf(mm, __shfl_xor(mm, off, kWave));
+  if (WAVES > 1) {
+    if ((tid & 63) == 0) sM[tid >> 6] = mm;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, sM[w]);
+  }
   const float base = mm == -INFINITY ? 0.f : mm;
   float L = 0.f;
-  for (int i = tid; i < n; i += 64) {
+  for (int i = tid; i < n; i += WAVES * 64) {
     const float2 ml = part.ml[slot(i)];
     const float f = exp2f(ml.x - base);
     sF[i] = f;
     L += f * ml.y;
   }
   L = warp_sum(L);
+  if ((tid & 63) == 0) sL[tid >> 6] = L;
   __syncthreads();
-  const int g = tid / L4, l4 = tid - g * L4;
+  L = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) L += sL[w];
   if (g < G) {
     floatx4 O = {0.f, 0.f, 0.f, 0.f};
-    for (int i = g; i < n; i += G) O += sF[i] * reinterpret_cast<const floatx4*>(part.o + slot(i) * D)[l4];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (g + u * G < n) O += sF[g + u * G] * x[u];
+    for (int i = g + AHEAD * G; i < n; i += G) O += sF[i] * reinterpret_cast<const floatx4*>(part.o + slot(i) * D)[l4];
     sO[g][l4] = O;
   }
   __syncthreads();
@@ -83,24 +83,22 @@ __global__ __launch_bounds__(64) void join_kernel(PrefixArgs a, Parts part, cons
 
 template <typename T, int D>
 void launch_prefix(PrefixArgs a, const PrefixPlan& plan, void* workspace, float* lse, hipStream_t s) {
-  a.slots = plan.slots();
-  const size_t pairs = (size_t)a.r.rows * a.q_heads, n = pairs * a.slots;
+  a.own = plan.own;
+  a.step = shared_step(D, sizeof(T) == 4);
+  a.shared_blocks = plan.shared_blocks;
+  a.blocks = plan.blocks;
+  a.pairs = (size_t)a.r.rows * a.q_heads;
+  const size_t n = a.pairs * plan.slots();
   Parts part;
   part.o = static_cast<float*>(workspace);
   part.ml = reinterpret_cast<float2*>(part.o + n * D);
   part.n = reinterpret_cast<int32_t*>(part.ml + n);
-  int32_t* const own_parts = part.n + pairs;
-  if (plan.shares) {
-    a.own = 0;
-    a.slot0 = 0;
-    launch_tiles<T, D>(a, plan.shared, part, s);
-  }
-  const int32_t* shared_parts = part.n;
-  part.n = own_parts;
-  a.own = 1;
-  a.slot0 = a.slots - plan.own.splits;
-  launch_tiles<T, D>(a, plan.own, part, s);
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3(a.r.rows, a.q_heads), dim3(64), 0, s, a, part, shared_parts, lse);
+  launch_tiles<T, D>(a, plan.shared, part, attend_grid(plan.blocks), s);
+  const dim3 grid(a.r.rows, a.q_heads);
+  if (plan.slots() <= kJoinFew)
+    hipLaunchKernelGGL((join_kernel<T, D, 1>), grid, dim3(64), 0, s, a, plan.shared.splits, part, lse);
+  else
+    hipLaunchKernelGGL((join_kernel<T, D, 4>), grid, dim3(256), 0, s, a, plan.shared.splits, part, lse);
   attend_launched(hipGetLastError());
 }
 

@@ -6,6 +6,12 @@
 
 namespace mit2hip {
 
+namespace {
+uint64_t workspace_of(const PrefixPlan& plan, const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads) {
+  return (uint64_t)r.rows * q_heads * ((uint64_t)plan.slots() * (c.head_dim + 2) + 2) * sizeof(float);
+}
+}  // namespace
+
 uint64_t kv_prefix_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, uint32_t q_heads,
                                        const mit2cfm_kv_prefix& x) {
   try {
@@ -15,8 +21,7 @@ uint64_t kv_prefix_attention_workspace(const mit2cfm_kv_cache& c, const mit2cfm_
     return 0;
   }
   if (r.seqs == 0 || r.rows == 0 || !query_rows_in_range(c, r, q_heads) || x.groups > 65535) return 0;
-  const uint64_t slots = prefix_plan(c, r, q_heads, x).slots();
-  return (uint64_t)r.rows * q_heads * (slots * (c.head_dim + 2) + 2) * sizeof(float);
+  return workspace_of(prefix_plan(c, r, q_heads, x), c, r, q_heads);
 }
 
 void kv_prefix_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm_kv_attention& p,
@@ -33,12 +38,12 @@ void kv_prefix_attention(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, co
              !meet(pieces(p.out, p.out_row, p.out_head, r.rows, p.q_heads, c.head_dim, e), lse),
          "lse overlaps q or out");
   }
-  need(p.workspace && p.workspace_bytes >= kv_prefix_attention_workspace(c, r, p.q_heads, x), "workspace is NULL or too small");
+  const PrefixPlan plan = prefix_plan(c, r, p.q_heads, x);
+  need(p.workspace && p.workspace_bytes >= workspace_of(plan, c, r, p.q_heads), "workspace is NULL or too small");
   a.bounds = x.group;
   a.shared = x.shared;
   a.groups = (int)x.groups;
   const int D = (int)c.head_dim;
-  const PrefixPlan plan = prefix_plan(c, r, p.q_heads, x);
   if (c.dtype == MIT2CFM_DTYPE_F32)
     launch_prefix_f32(a, plan, D, p.workspace, x.lse, s);
   else if (c.dtype == MIT2CFM_DTYPE_F16)
