@@ -820,6 +820,12 @@ __device__ __forceinline__ void load_to_lds(const void* src, lds_ptr_t* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, lds, 16, 0, 0);
 #endif
 }
+// Each lane's 4 bytes to lds + 4 * lane.
+__device__ __forceinline__ void load4_to_lds(const void* src, lds_ptr_t* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, lds, 4, 0, 0);
+#endif
+}
 
 // Many query rows: the block's waves have 16 WMT of them each and go over the
 // split's keys together, 16 KB of keys and values at a time.  Those are read

@@ -48,7 +48,7 @@ void kv_weigh(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm
   a.mask_words = p.mask ? (int)p.mask_words : 0;
   a.q_heads = (int)p.q_heads;
   a.group = (int)(p.q_heads / c.kv_heads);
-  set_scale(a, p.scale);
+  w.c2 = p.scale * 1.4426950408889634f;
   a.q_wide = aligned(p.q, 16) && p.q_row % 8 == 0 && p.q_head % 8 == 0;
   w.lse = p.lse;
   w.weights = p.weights;
@@ -64,7 +64,11 @@ void kv_weigh(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm
   plan.by_query = each * a.group / r.seqs > 16;  // more than a query tile on average
   const uint64_t keys = 16 * weigh_tiles(D, (int)e) * (plan.by_query ? 1 : kAttendWaves);
   const uint64_t len = std::min<uint64_t>({r.max_length, (uint64_t)c.table_stride * c.page_rows, p.weight_stride});
-  plan.chunks = (uint32_t)std::clamp<uint64_t>((len + keys - 1) / keys, 1, 1u << 20);
+  const uint64_t lines = (uint64_t)r.seqs * c.kv_heads;
+  // few queries: no more blocks than fill the chip four times over, each then has several chunks
+  const uint64_t most = plan.by_query ? 1u << 20 : std::max<uint64_t>(1, 4096 / lines);
+  plan.blocks = (uint32_t)std::clamp<uint64_t>((len + keys - 1) / keys, 1, most);
+  plan.by_xcd = plan.by_query && (lines % 8 == 0 || lines >= 32) && (lines + 7) * plan.blocks < (1u << 23);
   if (c.dtype == MIT2CFM_DTYPE_F32)
     launch_weigh_f32(w, plan, D, s);
   else if (c.dtype == MIT2CFM_DTYPE_F16)
