@@ -68,7 +68,9 @@ struct Ranks {
   }
   // The keys of a wave's places j0 .. j1 - 1 (at most kWaveKeys) to LDS, one after
   // the other, 0 past the end.  Read through resources that end where the places do.
-  __device__ __forceinline__ void load(int j0, int j1, uint32_t* to) const {
+  // then(place, weight, birth) of each place.
+  template <typename F>
+  __device__ __forceinline__ void load(int j0, int j1, uint32_t* to, F&& then) const {
     constexpr int B = 8;  // of a lane at once
     const int lane = threadIdx.x & 63, size = max(j1 - j0, 0);
     const int e0 = j0 >> page_shift, entries = size ? ((j1 - 1) >> page_shift) - e0 + 1 : 0;
@@ -89,11 +91,34 @@ struct Ranks {
       for (int u = 0; u < B; ++u) {
         const int i = i0 + 64 * u + lane;
         to[i] = i < size ? key_of(j0 + i, w[u], birth[u], page[u]) : 0u;
+        if (i < size) then(j0 + i, w[u], birth[u]);
       }
     }
   }
 };
 
+// count += key >= least, in two instructions (compiled, it was a select and a sum besides the comparison).
+__device__ __forceinline__ void add_if_from(uint32_t& count, uint32_t key, uint32_t least) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __asm__("v_cmp_le_u32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, 0, %0, vcc" : "+v"(count) : "s"(least), "v"(key) : "vcc");
+#else
+  count += key >= least;
+#endif
+}
+// The sum over a wave, in all lanes.
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1 .. 8: a row's sum in its last lane
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15, to the rows after the first and third
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return __builtin_amdgcn_readlane(v, 63);
+#else
+  return v;
+#endif
+}
 // base + #(voting lanes before this one)
 __device__ __forceinline__ uint32_t lanes_below(uint64_t vote, uint32_t base) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(vote >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote, base));
@@ -130,8 +155,15 @@ struct Line {
     weights_out = a.weights_out + at * a.stride;
     born_out = a.born_out ? a.born_out + at * a.stride : nullptr;
   }
-  // Weights and births to where they are wanted, of the places j0 .. j1 - 1 below m, by
-  // `by` threads.  (Those of places that rows left are written again by the moves.)
+  // A wave's keys to LDS (Ranks::load), the weights and births below m to where they are
+  // wanted.  (Those of places that rows left are written again by the moves.)
+  __device__ __forceinline__ void load(int j0, int j1, uint32_t* to) const {
+    r.load(j0, j1, to, [&](int j, float weight, int birth) {
+      if (apart && j < m) near(weights_out, j) = weight;
+      if (apart_born && j < m) near(born_out, j) = birth;
+    });
+  }
+  // Those of the places j0 .. j1 - 1 below m, by `by` threads.
   __device__ __forceinline__ void copy(int j0, int j1, int mine, int by) const {
     if (!apart && !apart_born) return;
     constexpr int B = 8;  // of a thread in flight
@@ -164,7 +196,7 @@ __device__ __forceinline__ void sweep(const Ranks& r, int j0, int j1, bool held,
 #pragma unroll 1
   for (int base = j0; base < j1; base += kWaveKeys) {
     const int size = min(j1 - base, kWaveKeys);
-    if (!held) r.load(base, base + size, keys);
+    if (!held) r.load(base, base + size, keys, [](int, float, int) {});
 #pragma unroll 1
     for (int i = 0; i < size; i += 64) f(base + i + lane, keys[i + lane], i + lane < size);
   }
@@ -196,13 +228,14 @@ __device__ __forceinline__ void list_moves(const EvictArgs& a, const Line& x, in
 
 // A block of W waves ranks a line whose keys lie in registers (longer lines than were
 // said are read again each time).  The key of the last row that stays, the m-th
-// largest, is found bit by bit from the top: votes count the keys from a candidate on,
-// and end the search once these are m.  No histogram, so no addition waits for another,
-// and of one wave no barrier.
+// largest, is found two bits at a time from the top: the lanes count the keys from each
+// of three candidates on, and the search ends once these are m.  No histogram, so
+// no addition waits for another, and of one wave no barrier.
 template <int W>
 __global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
   __shared__ uint32_t s_keys[W][kWaveKeys];
-  __shared__ uint32_t s_count[2][W], s_gt[W], s_eq[W], s_gt_below[W], s_eq_below[W];
+  __shared__ uint2 s_count[2][W];
+  __shared__ uint32_t s_gt[W], s_eq[W], s_gt_below[W], s_eq_below[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Line x(a, blockIdx.x);
   const int n = x.r.n, m = x.m;
@@ -218,55 +251,112 @@ __global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
   uint32_t* const keys = s_keys[wave];
   uint32_t key[kKeys];
   if (held) {
-    x.r.load(j0, j1, keys);
+    x.load(j0, j1, keys);
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) key[i] = keys[64 * i + lane];
   }
 
   int turn = 0;
-  auto whole = [&](uint32_t count) {  // over the block
-    if (W == 1) return count;
-    if (lane == 0) s_count[turn][wave] = count;
+  // Three counts of a lane, over the block.
+  auto whole = [&](uint32_t(&count)[3]) {
+    const uint32_t two = wave_sum(count[0] | count[1] << 16), third = wave_sum(count[2]);  // (at most 1024, or a wave alone)
+    count[0] = two & 0xffffu;
+    count[1] = two >> 16;
+    count[2] = third;
+    if (W == 1) return;
+    if (lane == 0) s_count[turn][wave] = make_uint2(two, third);
     __syncthreads();
-    uint32_t sum = 0;
+    count[0] = count[1] = count[2] = 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum += s_count[turn][w];
+    for (int w = 0; w < W; ++w) {
+      const uint2 o = s_count[turn][w];
+      count[0] += o.x & 0xffffu;
+      count[1] += o.x >> 16;
+      count[2] += o.y;
+    }
     turn ^= 1;
-    return (uint32_t)__builtin_amdgcn_readfirstlane(sum);
+#pragma unroll
+    for (int u = 0; u < 3; ++u) count[u] = __builtin_amdgcn_readfirstlane(count[u]);
   };
-  auto from_on = [&](uint32_t c) {  // keys >= c; c > 0, so none past the end
-    uint32_t count = 0;
+  // Keys >= c[u]; c > 0, so none past the end.
+  auto from_on = [&](const uint32_t(&c)[3], uint32_t(&count)[3]) {
+    count[0] = count[1] = count[2] = 0;
     if (held) {
 #pragma unroll
-      for (int i = 0; i < kKeys; ++i) count += __popcll(__ballot(key[i] >= c));
-    } else {
-      sweep(x.r, j0, j1, false, keys, [&](int, uint32_t k, bool) { count += __popcll(__ballot(k >= c)); });
+      for (int i = 0; i < kKeys; ++i)
+#pragma unroll
+        for (int u = 0; u < 3; ++u) add_if_from(count[u], key[i], c[u]);
+      whole(count);
+      return;
     }
-    return whole(count);
+    uint32_t total[3] = {0, 0, 0};
+    sweep(x.r, j0, j1, false, keys, [&](int, uint32_t k, bool) {
+#pragma unroll
+      for (int u = 0; u < 3; ++u) total[u] += __popcll(__ballot(k >= c[u]));
+    });
+    if (W == 1) {
+#pragma unroll
+      for (int u = 0; u < 3; ++u) count[u] = total[u];
+      return;
+    }
+    for (int u = 0; u < 3; ++u) {  // (counts past 16 bits)
+      __syncthreads();
+      if (lane == 0) s_gt[wave] = total[u];
+      __syncthreads();
+      for (int w = 0; w < W; ++w) count[u] += s_gt[w];
+      count[u] = __builtin_amdgcn_readfirstlane(count[u]);
+    }
+    __syncthreads();
   };
-  uint32_t least = 0, ties = 0;
+  uint32_t least = 0, ties = 0, count[3];
   bool exact = false;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = least | 1u << bit, count = from_on(c);
-    if (count >= (uint32_t)m) least = c;
-    if (count == (uint32_t)m) {
-      exact = true;
-      break;
+  for (int bit = 30; bit >= 0 && !exact; bit -= 2) {
+    const uint32_t c[3] = {least | 1u << bit, least | 2u << bit, least | 3u << bit};
+    from_on(c, count);
+#pragma unroll
+    for (int u = 0; u < 3; ++u) {
+      if (count[u] >= (uint32_t)m) least = c[u];
+      if (count[u] == (uint32_t)m) {
+        exact = true;
+        break;
+      }
     }
   }
-  if (exact)
+  if (exact) {
     least -= 1;  // all from the candidate on stay
-  else
-    ties = m - (least == 0xffffffffu ? 0u : from_on(least + 1));
+  } else if (least == 0xffffffffu) {
+    ties = m;
+  } else {
+    const uint32_t c[3] = {least + 1, least + 1, least + 1};
+    from_on(c, count);
+    ties = m - count[0];
+  }
 
   uint32_t gt = 0, eq = 0, gt_below = 0, eq_below = 0;
-  sweep(x.r, j0, j1, held, keys, [&](int j, uint32_t k, bool in) {
-    const uint64_t more = __ballot(in && k > least), equal = __ballot(in && k == least), low = __ballot(j < m);
-    gt += __popcll(more);
-    eq += __popcll(equal);
-    gt_below += __popcll(more & low);
-    eq_below += __popcll(equal & low);
-  });
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      const int j = j0 + 64 * i + lane;
+      const uint32_t more = key[i] > least ? 1u : 0u, equal = j < j1 && key[i] == least ? 1u : 0u;
+      gt += more;
+      eq += equal;
+      gt_below += j < m ? more : 0u;
+      eq_below += j < m ? equal : 0u;
+    }
+    const uint32_t all = wave_sum(gt | eq << 16), low = wave_sum(gt_below | eq_below << 16);
+    gt = all & 0xffffu;
+    eq = all >> 16;
+    gt_below = low & 0xffffu;
+    eq_below = low >> 16;
+  } else {
+    sweep(x.r, j0, j1, held, keys, [&](int j, uint32_t k, bool in) {
+      const uint64_t more = __ballot(in && k > least), equal = __ballot(in && k == least), low = __ballot(j < m);
+      gt += __popcll(more);
+      eq += __popcll(equal);
+      gt_below += __popcll(more & low);
+      eq_below += __popcll(equal & low);
+    });
+  }
   if (W > 1) {
     if (lane == 0) {
       s_gt[wave] = gt;
@@ -289,7 +379,7 @@ __global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
   const uint32_t stay_below = gt_below + min(eq_below, ties);  // of the places below m
   if (tid == 0) a.moves[x.at] = m - stay_below;
   list_moves(a, x, j0, j1, held, keys, least, ties, gt, eq, stay_below);
-  x.copy(j0, j1, lane, 64);
+  if (!held) x.copy(j0, j1, lane, 64);
 }
 
 // Long lines in segments, a block each: those of the first m places, then those of
@@ -299,7 +389,7 @@ struct Segment {
   int j0, j1;  // this one's places
   __device__ __forceinline__ Segment(const Line& x, int segments, int seg) {
     const int n = x.r.n, m = x.m;
-    lower = min(max((int)((int64_t)segments * m / n), 1), segments - 1);
+    lower = min(max((int)(((int64_t)segments * m + n / 2) / n), 1), segments - 1);
     const bool low = seg < lower;
     const int base = low ? 0 : m, size = low ? m : n - m, parts = low ? lower : segments - lower, i = low ? seg : seg - lower;
     const int each = ((size + parts - 1) / parts + 63) / 64 * 64;
@@ -323,10 +413,16 @@ __device__ __forceinline__ uint2 find_bin(const EvictArgs& a, const Line& x) {
   static_assert(PER == 4, "a thread's bins are a vector");
   const int mine = kSplitThreads - 1 - tid;  // from the top
   uint4 n = make_uint4(0, 0, 0, 0);
-#pragma unroll 8
-  for (int s = 0; s < a.segments; ++s) {
-    const uint4 o = hist[s * (kBins / 4) + mine];
-    n.x += o.x; n.y += o.y; n.z += o.z; n.w += o.w;
+#pragma unroll 1
+  for (int s0 = 0; s0 < a.segments; s0 += 16) {
+    uint4 o[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) o[u] = hist[min(s0 + u, a.segments - 1) * (kBins / 4) + mine];
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+      if (s0 + u < a.segments) {
+        n.x += o[u].x; n.y += o[u].y; n.z += o[u].z; n.w += o[u].w;
+      }
   }
   const uint32_t sum = n.x + n.y + n.z + n.w;
   uint32_t incl = sum;
@@ -374,6 +470,7 @@ __global__ __launch_bounds__(kSplitThreads) void split_count_kernel(EvictArgs a)
   sweep(x.r, j0, j1, false, s_keys[wave], [&](int, uint32_t k, bool there) {
     constexpr int above = ROUND == 0 ? 0 : bits_from(ROUND - 1);
     if (ROUND == 2) larger += __popcll(__ballot(there && k >> above > known >> above));
+    if (ROUND > 0 && !__any(there && k >> above == known >> above)) return;
     if (there && (ROUND == 0 || k >> above == known >> above)) {
       const uint32_t bin = k >> bits_from(ROUND) & bits_mask(ROUND);
       // lanes with the first one's bin add at once
@@ -454,7 +551,7 @@ __global__ __launch_bounds__(kSplitThreads) void split_list_kernel(EvictArgs a) 
   const int j0 = min(g.j0 + wave * share, g.j1), j1 = min(j0 + share, g.j1);
   const bool held = share <= kWaveKeys;
   uint32_t* const keys = s_keys[wave];
-  if (held) x.r.load(j0, j1, keys);
+  if (held) x.load(j0, j1, keys);
   uint32_t wgt = 0, weq = 0;
   sweep(x.r, j0, j1, held, keys, [&](int, uint32_t k, bool in) {
     wgt += __popcll(__ballot(in && k > least));
@@ -470,7 +567,7 @@ __global__ __launch_bounds__(kSplitThreads) void split_list_kernel(EvictArgs a) 
     eq += s_weq[w];
   }
   list_moves(a, x, j0, j1, held, keys, least, ties, gt, eq, stay_below);
-  x.copy(j0, j1, lane, 64);
+  if (!held) x.copy(j0, j1, lane, 64);
 }
 
 // Moves the rows of a line's list, 16 bytes of a key and of a value a lane at a time.
@@ -511,7 +608,8 @@ int segments_of(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p) {
   const uint64_t len = std::min<uint64_t>({p.max_length, p.weight_stride, (uint64_t)c.table_stride * c.page_rows});
   const uint64_t lines = (uint64_t)p.layers * p.seqs * c.kv_heads;
   if (len <= 16 * kWaveKeys) return 1;
-  return (int)std::min<uint64_t>({(len + kSplitKeys - 1) / kSplitKeys, (uint64_t)kMaxSegments, std::max<uint64_t>(2, 4096 / lines)});
+  // (with room: what lies below the budget is divided by itself)
+  return (int)std::min<uint64_t>({len / (kSplitKeys * 7 / 8) + 1, (uint64_t)kMaxSegments, std::max<uint64_t>(2, 4096 / lines)});
 }
 bool evict_in_range(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p) {
   return p.seqs <= 65535 && p.layers >= 1 && p.layers <= 16384 && (uint64_t)p.layers * p.seqs * c.kv_heads <= (1u << 24) &&
