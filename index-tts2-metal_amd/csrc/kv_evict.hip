@@ -711,6 +711,8 @@ void kv_evict(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p, hipStream_t 
     hipLaunchKernelGGL((choose_kernel<1>), grid, dim3(64), 0, s, a);
   } else if (len <= 4 * kWaveKeys) {
     hipLaunchKernelGGL((choose_kernel<4>), grid, dim3(256), 0, s, a);
+  } else if (len <= 8 * kWaveKeys) {
+    hipLaunchKernelGGL((choose_kernel<8>), grid, dim3(512), 0, s, a);
   } else {
     hipLaunchKernelGGL((choose_kernel<16>), grid, dim3(1024), 0, s, a);
   }

@@ -112,7 +112,7 @@ def test_types_heads_and_pages(mit2, ctx, dtype, dim, heads, page):
     Cut(mit2, [90, 40, 3], [50, 39, 3], heads=heads, dim=dim, page=page, dtype=dtype, born=True, seed=dim).check(ctx)
 
 
-@pytest.mark.parametrize("length,keep", [(700, 699), (700, 636), (2100, 700), (3000, 2999), (5000, 1250), (20000, 9999)])
+@pytest.mark.parametrize("length,keep", [(700, 699), (700, 636), (2100, 700), (3000, 2999), (5000, 1250), (8192, 4000), (8193, 8000), (20000, 9999)])
 def test_long_sequences(mit2, ctx, length, keep):
     Cut(mit2, [length, length // 3], [keep, length // 4], layers=1, heads=2, page=64, first=4, last=100, born=length % 1000 == 700, seed=length).check(ctx)
 
