@@ -17,7 +17,7 @@ constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64;
 constexpr int kSplitKeys = kSplitWaves * kWaveKeys;  // a segment's, where the length is as said
 constexpr int kBins = 2048;
 constexpr int kMaxSegments = 64;
-constexpr int kMoveThreads = 256;
+constexpr int kMoveThreads = 256, kMoveBatch = 2;  // a thread's moves in flight
 
 struct EvictArgs {
   CacheView c;
@@ -583,17 +583,31 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int chu
   const int64_t head16 = head * a.c.head_stride(a.row16);
   const int per = kMoveThreads / a.row16, mine = tid / a.row16, l = tid - mine * a.row16;
   if (mine >= per) return;
-  for (int64_t i = (int64_t)chunk * per + mine; i < moves; i += (int64_t)chunks * per) {
-    const int dst = to[i], src = from[i];
-    const int dst_page = a.c.page_of(seq, dst), src_page = a.c.page_of(seq, src);
-    if (l == 0) {
-      a.weights_out[line * a.stride + dst] = a.weights[line * a.stride + src];
-      if (a.born) a.born_out[line * a.stride + dst] = a.born[line * a.stride + src];
+  const int64_t step = (int64_t)chunks * per;
+  for (int64_t i0 = (int64_t)chunk * per + mine; i0 < moves; i0 += kMoveBatch * step) {
+    u32x4 x[kMoveBatch], y[kMoveBatch];
+    int64_t at[kMoveBatch];
+#pragma unroll
+    for (int u = 0; u < kMoveBatch; ++u) {
+      const int64_t i = min(i0 + u * step, (int64_t)moves - 1);
+      const int dst = to[i], src = from[i];
+      const int dst_page = a.c.page_of(seq, dst), src_page = a.c.page_of(seq, src);
+      const bool there = dst_page >= 0 && src_page >= 0 && i0 + u * step < moves;
+      at[u] = there ? a.c.row_in(dst_page, dst, a.row16) + head16 + l : -1;
+      const int64_t s = a.c.row_in(max(src_page, 0), src, a.row16) + head16 + l;
+      x[u] = k[s];
+      y[u] = v[s];
+      if (l == 0 && i0 + u * step < moves) {
+        a.weights_out[line * a.stride + dst] = a.weights[line * a.stride + src];
+        if (a.born) a.born_out[line * a.stride + dst] = a.born[line * a.stride + src];
+      }
     }
-    if (dst_page < 0 || src_page < 0) continue;
-    const int64_t d = a.c.row_in(dst_page, dst, a.row16) + head16 + l, s = a.c.row_in(src_page, src, a.row16) + head16 + l;
-    k[d] = k[s];
-    v[d] = v[s];
+#pragma unroll
+    for (int u = 0; u < kMoveBatch; ++u)
+      if (at[u] >= 0) {
+        __builtin_nontemporal_store(x[u], k + at[u]);
+        __builtin_nontemporal_store(y[u], v + at[u]);
+      }
   }
 }
 
@@ -718,7 +732,7 @@ void kv_evict(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p, hipStream_t 
   }
   kv_launched(hipGetLastError());
   const uint64_t per = kMoveThreads / a.row16;
-  const uint64_t wanted = std::max<uint64_t>(1, 8192 / lines);  // blocks of a line, for as many moves as half its places at most
+  const uint64_t wanted = std::max<uint64_t>(1, 4096 / lines);  // blocks of a line, for as many moves as half its places at most
   const int chunks = (int)std::min(wanted, (len / 2 + per - 1) / per + 1);
   hipLaunchKernelGGL(move_kernel, dim3(c.kv_heads * chunks, p.seqs, p.layers), dim3(kMoveThreads), 0, s, a, chunks);
   kv_launched(hipGetLastError());
