@@ -656,7 +656,9 @@ mit2cfm_status mit2cfm_kv_norm_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_
  * their first shared[g] rows: those have the same contents for each of them, the same
  * pages or copies, and which of them are read is not said.  New rows are never taken as
  * shared, whatever shared[g] says: no more are than every sequence of the group that has
- * new rows has before them.  group does not decrease; sequences in no group share nothing. */
+ * new rows has before them.  group does not decrease; sequences in no group share nothing.
+ * With 16-bit types the probabilities are rounded to the type where a group has more than
+ * 16 rows x query heads of a key head on average. */
 typedef struct mit2cfm_kv_prefix {
   const int32_t* group;  /* [groups + 1] */
   const int32_t* shared; /* [groups] */

@@ -848,9 +848,8 @@ __device__ __forceinline__ void load4_to_lds(const void* src, lds_ptr_t* lds) {
 //
 // The ring's buffers are objects of their own, named by constants in the usual
 // path: a read that might alias any of them would wait for every load.
-template <typename T, int D, int WMT, typename A>
-__device__ __forceinline__ void attend_wide(const A& a, const AttendPlan& plan, const Parts& part, Part p, u32x4* sK0, u32x4* sK1,
-                                            u32x4* sK2, u32x4* sV0, u32x4* sV1, u32x4* sV2) {
+template <typename T, int D, typename A>
+__global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_kernel(A a, AttendPlan plan, Parts part) {
   typedef Dims<T, D> S;
   typedef typename Mat<T>::op Op;
   constexpr int KT = S::KT, NT = S::NT, DP = S::DP, DC = S::DC, NV = S::NV;
@@ -859,10 +858,15 @@ __device__ __forceinline__ void attend_wide(const A& a, const AttendPlan& plan, 
   constexpr int KEYS = 512 / CPR;                 // keys of a buffer: 8 KB each of keys and values
   constexpr int STEP = kAttendThreads / CPR;      // rows a pass of the block loads
   constexpr int PASSES = KEYS / STEP;             // 2
+  constexpr int WMT = (std::is_same<A, PrefixArgs>::value ? kPrefixRows : wide_rows(sizeof(T) == 4)) / (16 * kAttendWaves);
   constexpr int XM = CPR < 16 ? CPR - 1 : 15;
+  __shared__ __attribute__((aligned(1024))) u32x4 sK0[KEYS * CPR], sK1[KEYS * CPR], sK2[KEYS * CPR];
+  __shared__ __attribute__((aligned(1024))) u32x4 sV0[KEYS * CPR], sV1[KEYS * CPR], sV2[KEYS * CPR];
   auto bufK = [&](int b) -> u32x4* { return b == 0 ? sK0 : b == 1 ? sK1 : sK2; };
   auto bufV = [&](int b) -> u32x4* { return b == 0 ? sV0 : b == 1 ? sV1 : sV2; };
 
+  Part p;
+  if (!find_part(a, plan, 16 * WMT * kAttendWaves, p)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lq = lane & 15, grp = lane >> 4;
   const int wm0 = p.m0 + 16 * WMT * wave;
@@ -1120,17 +1124,6 @@ __device__ __forceinline__ void attend_wide(const A& a, const AttendPlan& plan, 
     }
     if (grp == 0) tell_parts(a, plan, p, part, (size_t)x.row * a.q_heads + x.h);
   }
-}
-
-template <typename T, int D, typename A>
-__global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_kernel(A a, AttendPlan plan, Parts part) {
-  constexpr int PLACES = 512;  // of 16 bytes
-  constexpr int WMT = (std::is_same<A, PrefixArgs>::value ? kPrefixRows : wide_rows(sizeof(T) == 4)) / (16 * kAttendWaves);
-  __shared__ __attribute__((aligned(1024))) u32x4 sK0[PLACES], sK1[PLACES], sK2[PLACES];
-  __shared__ __attribute__((aligned(1024))) u32x4 sV0[PLACES], sV1[PLACES], sV2[PLACES];
-  Part p;
-  if (!find_part(a, plan, 16 * WMT * kAttendWaves, p)) return;
-  attend_wide<T, D, WMT>(a, plan, part, p, sK0, sK1, sK2, sV0, sV1, sV2);
 }
 
 // Joins a row and query head's splits, WAVES waves for each: lane groups of D/4
