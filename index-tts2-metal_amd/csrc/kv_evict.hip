@@ -71,7 +71,7 @@ struct Ranks {
   // then(place, weight, birth) of each place.
   template <typename F>
   __device__ __forceinline__ void load(int j0, int j1, uint32_t* to, F&& then) const {
-    constexpr int B = 8;  // of a lane at once
+    constexpr int B = kKeys;  // of a lane at once
     const int lane = threadIdx.x & 63, size = max(j1 - j0, 0);
     const int e0 = j0 >> page_shift, entries = size ? ((j1 - 1) >> page_shift) - e0 + 1 : 0;
     const buffer_rsrc_t rw = make_buffer_rsrc(weights + j0, 4 * size), rt = make_buffer_rsrc(table + e0, 4 * entries);
@@ -198,7 +198,13 @@ __device__ __forceinline__ void sweep(const Ranks& r, int j0, int j1, bool held,
     const int size = min(j1 - base, kWaveKeys);
     if (!held) r.load(base, base + size, keys, [](int, float, int) {});
 #pragma unroll 1
-    for (int i = 0; i < size; i += 64) f(base + i + lane, keys[i + lane], i + lane < size);
+    for (int i = lane; i - lane < size; i += 256) {  // (four at once wait once; past the end they count for nothing)
+      uint32_t k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) k[u] = keys[i + 64 * u];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) f(base + i + 64 * u, k[u], i + 64 * u < size);
+    }
   }
 }
 
@@ -228,12 +234,14 @@ __device__ __forceinline__ void list_moves(const EvictArgs& a, const Line& x, in
 
 // A block of W waves ranks a line whose keys lie in registers (longer lines than were
 // said are read again each time).  The key of the last row that stays, the m-th
-// largest, is found two bits at a time from the top: the lanes count the keys from each
-// of three candidates on, and the search ends once these are m.  No histogram, so
-// no addition waits for another, and of one wave no barrier.
+// largest, is found from the top, by one wave a bit at a time, by more, which wait for
+// each other at every step, two: the lanes count the keys from one candidate, or each of
+// three, on, and the search ends once these are m.  No histogram, so no addition waits
+// for another, and of one wave no barrier.
 template <int W>
 __global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
   __shared__ uint32_t s_keys[W][kWaveKeys];
+  constexpr int BITS = W == 1 ? 1 : 2, N = (1 << BITS) - 1;  // of a step, and its candidates
   __shared__ uint2 s_count[2][W];
   __shared__ uint32_t s_gt[W], s_eq[W], s_gt_below[W], s_eq_below[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -257,69 +265,65 @@ __global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
   }
 
   int turn = 0;
-  // Three counts of a lane, over the block.
-  auto whole = [&](uint32_t(&count)[3]) {
-    const uint32_t two = wave_sum(count[0] | count[1] << 16), third = wave_sum(count[2]);  // (at most 1024, or a wave alone)
-    count[0] = two & 0xffffu;
-    count[1] = two >> 16;
-    count[2] = third;
-    if (W == 1) return;
-    if (lane == 0) s_count[turn][wave] = make_uint2(two, third);
-    __syncthreads();
-    count[0] = count[1] = count[2] = 0;
+  // A lane's counts, over the block.
+  auto whole = [&](uint32_t(&count)[N]) {
+    if constexpr (N == 1) {
+      count[0] = wave_sum(count[0]);
+    } else {
+      const uint32_t two = wave_sum(count[0] | count[1] << 16), third = wave_sum(count[2]);  // (at most 1024 of a wave)
+      if (lane == 0) s_count[turn][wave] = make_uint2(two, third);
+      __syncthreads();
+      count[0] = count[1] = count[2] = 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const uint2 o = s_count[turn][w];
-      count[0] += o.x & 0xffffu;
-      count[1] += o.x >> 16;
-      count[2] += o.y;
+      for (int w = 0; w < W; ++w) {
+        const uint2 o = s_count[turn][w];
+        count[0] += o.x & 0xffffu;
+        count[1] += o.x >> 16;
+        count[2] += o.y;
+      }
+      turn ^= 1;
+#pragma unroll
+      for (int u = 0; u < 3; ++u) count[u] = __builtin_amdgcn_readfirstlane(count[u]);
     }
-    turn ^= 1;
-#pragma unroll
-    for (int u = 0; u < 3; ++u) count[u] = __builtin_amdgcn_readfirstlane(count[u]);
   };
   // Keys >= c[u]; c > 0, so none past the end.
-  auto from_on = [&](const uint32_t(&c)[3], uint32_t(&count)[3]) {
-    count[0] = count[1] = count[2] = 0;
+  auto from_on = [&](const uint32_t(&c)[N], uint32_t(&count)[N]) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) count[u] = 0;
     if (held) {
 #pragma unroll
       for (int i = 0; i < kKeys; ++i)
 #pragma unroll
-        for (int u = 0; u < 3; ++u) add_if_from(count[u], key[i], c[u]);
+        for (int u = 0; u < N; ++u) add_if_from(count[u], key[i], c[u]);
       whole(count);
       return;
     }
-    uint32_t total[3] = {0, 0, 0};
     sweep(x.r, j0, j1, false, keys, [&](int, uint32_t k, bool) {
 #pragma unroll
-      for (int u = 0; u < 3; ++u) total[u] += __popcll(__ballot(k >= c[u]));
+      for (int u = 0; u < N; ++u) count[u] += __popcll(__ballot(k >= c[u]));
     });
-    if (W == 1) {
-#pragma unroll
-      for (int u = 0; u < 3; ++u) count[u] = total[u];
-      return;
-    }
-    for (int u = 0; u < 3; ++u) {  // (counts past 16 bits)
+    if (W == 1) return;
+    for (int u = 0; u < N; ++u) {  // (counts past 16 bits)
       __syncthreads();
-      if (lane == 0) s_gt[wave] = total[u];
+      if (lane == 0) s_gt[wave] = count[u];
       __syncthreads();
+      count[u] = 0;
       for (int w = 0; w < W; ++w) count[u] += s_gt[w];
       count[u] = __builtin_amdgcn_readfirstlane(count[u]);
     }
     __syncthreads();
   };
-  uint32_t least = 0, ties = 0, count[3];
+  uint32_t least = 0, ties = 0, c[N], count[N];
   bool exact = false;
-  for (int bit = 30; bit >= 0 && !exact; bit -= 2) {
-    const uint32_t c[3] = {least | 1u << bit, least | 2u << bit, least | 3u << bit};
+  for (int bit = 32 - BITS; bit >= 0 && !exact; bit -= BITS) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) c[u] = least | (u + 1u) << bit;
     from_on(c, count);
 #pragma unroll
-    for (int u = 0; u < 3; ++u) {
+    for (int u = 0; u < N; ++u) {
+      if (exact) continue;
       if (count[u] >= (uint32_t)m) least = c[u];
-      if (count[u] == (uint32_t)m) {
-        exact = true;
-        break;
-      }
+      exact = count[u] == (uint32_t)m;
     }
   }
   if (exact) {
@@ -327,7 +331,8 @@ __global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
   } else if (least == 0xffffffffu) {
     ties = m;
   } else {
-    const uint32_t c[3] = {least + 1, least + 1, least + 1};
+#pragma unroll
+    for (int u = 0; u < N; ++u) c[u] = least + 1;
     from_on(c, count);
     ties = m - count[0];
   }
