@@ -72,8 +72,12 @@ __device__ __forceinline__ void load_row(const T* q, bool wide, int grp, typenam
 // queries, two exchanges for each 16 keys.  BYQ: the block's four waves have the
 // same keys and every fourth query tile each, and join in LDS, in order; else
 // each wave goes over keys of its own.  No place is added to by two waves.
+//
+// The third block of a CU is worth the few registers that 16-bit rows of 256 bytes spill
+// for it: 4 ragged prompts of 1029 rows 63 us for 76, even ones 103 for 110 (of 512 rows 66
+// for 63); f32 rows, bound by their products, lose.
 template <typename T, int D, bool BYQ>
-__global__ __launch_bounds__(kAttendThreads, 2) void weigh_kernel(WeighArgs w, WeighPlan plan) {
+__global__ __launch_bounds__(kAttendThreads, (BYQ && sizeof(T) == 2 && D <= 128) ? 3 : 2) void weigh_kernel(WeighArgs w, WeighPlan plan) {
   typedef Dims<T, D> S;
   typedef typename Mat<T>::op Op;
   constexpr int DC = S::DC, NT = weigh_tiles(D, sizeof(T)), KEYS = 16 * NT;
