@@ -119,6 +119,23 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
   return v;
 #endif
 }
+// The least (the largest) over a wave, in all lanes.
+template <bool LEAST>
+__device__ __forceinline__ uint32_t wave_end(uint32_t v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr uint32_t none = LEAST ? 0xffffffffu : 0u;
+  auto join = [&](uint32_t o) { v = LEAST ? min(v, o) : max(v, o); };
+  join(__builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));
+  join(__builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
+#else
+  return v;
+#endif
+}
 // base + #(voting lanes before this one)
 __device__ __forceinline__ uint32_t lanes_below(uint64_t vote, uint32_t base) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(vote >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote, base));
@@ -262,6 +279,36 @@ __global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
     x.load(j0, j1, keys);
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) key[i] = keys[64 * i + lane];
+  }
+
+  if (held && n - m == 1) {  // the last of the least leaves, and the row behind the budget takes its place
+    uint32_t low = 0xffffffffu, place = 0;
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+      if (j0 + 64 * i + lane < j1 && key[i] <= low) {
+        low = key[i];
+        place = j0 + 64 * i + lane;
+      }
+    const uint32_t least = wave_end<true>(low);
+    place = wave_end<false>(low == least ? place : 0u);
+    if (W > 1) {
+      if (lane == 0) s_count[0][wave] = make_uint2(least, place);
+      __syncthreads();
+    }
+    if (tid == 0) {
+      uint2 out = make_uint2(least, place);
+      for (int w = 1; w < W; ++w) {  // (a wave without places tells of the largest key at the first)
+        const uint2 o = s_count[0][w];
+        if (o.x < out.x || (o.x == out.x && o.y > out.y)) out = o;
+      }
+      const bool moves = out.y < (uint32_t)m;
+      a.moves[x.at] = moves;
+      if (moves) {
+        a.to[x.at * a.list_stride] = out.y;
+        a.from[x.at * a.list_stride] = m;
+      }
+    }
+    return;
   }
 
   int turn = 0;

@@ -165,6 +165,20 @@ def test_any_length_hint(mit2, ctx, hint):
     Cut(mit2, [700, 30], [300, 29], hint=hint, seed=9).check(ctx)
 
 
+@pytest.mark.parametrize("kind", ["any", "equal", "few", "wild"])
+@pytest.mark.parametrize("length", [2, 64, 700, 1024, 1025, 4096, 8190, 16384, 17000])
+def test_one_row_leaves(mit2, ctx, length, kind):
+    """The last of the least, which may be the row behind the budget; of a hint of one wave's length too."""
+    rng = np.random.default_rng(length)
+    shape = (2, 3, 2, length)
+    w = {"any": rng.exponential(1.0, shape), "equal": np.full(shape, 0.25), "few": rng.integers(0, 3, shape) * 0.5,
+         "wild": rng.choice([np.nan, np.inf, -np.inf, 0.0, -0.0, 1.0], shape)}[kind].astype(np.float32)
+    w[0, 0, 0, length - 1] = -3e38
+    lengths = [length, max(2, length // 2), max(2, length - 3)]
+    for first, last, hint in ((0, 0, None), (1, 5, None), (2 ** 32 - 1, 0, None), (4, 0, 0)):
+        Cut(mit2, lengths, [n - 1 for n in lengths], heads=2, page=64, weights=w, stride=length, first=first, last=last, hint=hint, seed=length).check(ctx)
+
+
 def test_many_sequences_and_layers(mit2, ctx):
     length = [(7 * s) % 40 for s in range(150)]
     Cut(mit2, length, [n // 2 for n in length], layers=5, heads=3, seed=10).check(ctx)
