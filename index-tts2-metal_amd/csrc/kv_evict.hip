@@ -783,8 +783,11 @@ void kv_evict(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p, hipStream_t 
     hipLaunchKernelGGL((choose_kernel<16>), grid, dim3(1024), 0, s, a);
   }
   kv_launched(hipGetLastError());
-  const uint64_t per = kMoveThreads / a.row16;
-  const uint64_t wanted = std::max<uint64_t>(1, 4096 / lines);  // blocks of a line, for as many moves as half its places at most
+  // 16 blocks a CU, of a line no more than its moves want, half its places at most: 256
+  // lines of 2048 moves 75 us (4 a CU 80); but lines that are 4 a CU themselves have one
+  // block each: 1440 of them with a move each 10.8 us (two blocks each 11.9, eleven 17.2).
+  const uint64_t per = kMoveThreads / a.row16 * kMoveBatch;
+  const uint64_t wanted = lines >= 1024 ? 1 : 4096 / lines;
   const int chunks = (int)std::min(wanted, (len / 2 + per - 1) / per + 1);
   hipLaunchKernelGGL(move_kernel, dim3(c.kv_heads * chunks, p.seqs, p.layers), dim3(kMoveThreads), 0, s, a, chunks);
   kv_launched(hipGetLastError());

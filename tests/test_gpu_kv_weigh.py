@@ -84,6 +84,25 @@ def test_chains_and_trees(mit2, ctx, dtype, dim, heads, new, tree):
     Weigh(mit2, b, mask=ops_ref.trees(b, dim)[0] if tree else None, decay=0.75).check(ctx)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,heads", [(32, (6, 2)), (64, (3, 3)), (96, (8, 1)), (128, (5, 1)), (192, (2, 1)), (256, (14, 2))])
+@pytest.mark.parametrize("tree", [False, True])
+def test_prompts(mit2, ctx, dtype, dim, heads, tree):
+    """Queries of many tiles; a page is missing, of one sequence the rows are more than its length."""
+    new = [131, 0, 200, 97]
+    b = Batch(new, [131 + 300, 50, 200, 97 + 65], page=16, q_heads=heads[0], kv_heads=heads[1], dim=dim, dtype=dtype, seed=dim, tail_rows=1, lead_rows=2)
+    b.table[0, 2] = -1
+    b.length[2] = 190
+    Weigh(mit2, b, mask=ops_ref.trees(b, dim)[0] if tree else None, decay=0.75).check(ctx)
+
+
+@pytest.mark.parametrize("dtype,dim,last", [("f32", 64, 0), ("f16", 128, 0), ("bf16", 96, 0), ("f16", 64, 7)])
+def test_many_sequences_of_some_rows(mit2, ctx, dtype, dim, last):
+    new = [(37 * s) % 41 for s in range(50)]
+    b = Batch(new, [n + (29 * s) % 300 for s, n in enumerate(new)], page=8, q_heads=12, kv_heads=4, dim=dim, dtype=dtype, seed=dim)
+    Weigh(mit2, b, decay=0.5, last=last).check(ctx)
+
+
 @pytest.mark.parametrize("last", [1, 5, 16, 40, 1000])
 @pytest.mark.parametrize("tree", [False, True])
 def test_last_rows_alone(mit2, ctx, last, tree):
