@@ -35,6 +35,9 @@ __device__ __forceinline__ float group_sum(float v) {
 //
 // The first heads are asked for before the row's sequence is known, and the angles'
 // frequencies formed meanwhile (fp64, as the positions times them).
+//
+// 9 prompts of up to 2047 rows, 32 + 8 + 8 bf16 heads of 128: 67 us, 4.9 TB/s, as fast as
+// a copy (5.0).  3 rows of 20 fp32 heads of 64: 4.4 us, the launch and the way to the row's page.
 template <typename T, int VEC, int G, int NI>
 __global__ __launch_bounds__(kNormThreads) void norm_append_kernel(NormArgs n, int D) {
   constexpr int HEADS = kNormThreads / G;  // heads of a pass
@@ -255,7 +258,8 @@ template <typename T, int VEC, int G, int NI>
 void launch_by(const NormArgs& n, int D, hipStream_t s) {
   constexpr int HEADS = kNormThreads / G;
   const int heads = n.a.q_heads + 2 * n.a.c.kv_heads;
-  // few rows: their heads over more blocks, down to one a group of lanes
+  // few rows: their heads over more blocks, down to one a group of lanes (64 rows of 48
+  // heads 4.6 us, with a block a row 5.9; 512 to 8192 blocks are alike)
   const int by = std::max(1, std::min((heads + HEADS - 1) / HEADS, 2048 / n.a.r.rows));
   hipLaunchKernelGGL((norm_append_kernel<T, VEC, G, NI>), dim3(n.a.r.rows, by), dim3(kNormThreads), 0, s, n, D);
   kv_launched(hipGetLastError());

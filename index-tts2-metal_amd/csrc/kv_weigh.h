@@ -73,6 +73,10 @@ __device__ __forceinline__ void load_row(const T* q, bool wide, int grp, typenam
 // same keys and every fourth query tile each, and join in LDS, in order; else
 // each wave goes over keys of its own.  No place is added to by two waves.
 //
+// Waves of their own keys: the cache's bytes bound it, 64 tokens over up to 8191 bf16 keys of
+// 128 in 8 heads 164 us, 4.75 TB/s.  Shared keys: the products and exponentials, 16 prompts of
+// 1029 rows, 32 heads, over 2047 f16 keys 317 us, 650 TFLOP/s.
+//
 // The third block of a CU is worth the few registers that 16-bit rows of 256 bytes spill
 // for it: 4 ragged prompts of 1029 rows 63 us for 76, even ones 103 for 110 (of 512 rows 66
 // for 63); f32 rows, bound by their products, lose.
@@ -250,7 +254,7 @@ __global__ __launch_bounds__(kAttendThreads, (BYQ && sizeof(T) == 2 && D <= 128)
         // Through LDS, a ring of the wave's own: 16 lanes read a row's neighbouring 16 bytes
         // each.  (Straight into operands each lane is in a row of its own, and the loads'
         // 64 addresses a third of the time: 16 prompts of 1029 rows over 2047 f16 keys 480 us
-        // so, now 374, 552 TFLOP/s.)  Three tiles, objects of their own so that a read waits
+        // so, 374 through LDS, both at two blocks a CU.)  Three tiles, objects of their own so that a read waits
         // for its own alone, two ahead; tiles past the end are the last one again, so that
         // the loads in flight are always as many.
         const int o0 = lane / CPR, place16 = lane % CPR;
