@@ -17,6 +17,10 @@ constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / 64;
 constexpr int kSplitKeys = kSplitWaves * kWaveKeys;  // a segment's, where the length is as said
 constexpr int kBins = 2048;
 constexpr int kMaxSegments = 64;
+// Rows that leave a line of one wave are found one after the other up to this many: 1440
+// lines of 704 places, with the moves, 10.8, 11.5, 12.8, 16.0, 18.5 us for 1, 2, 4, 8, 12 rows,
+// by the search 16.2 to 18.6 (one row 18.9).
+constexpr int kFewLeave = 8;
 constexpr int kMoveThreads = 256, kMoveBatch = 2;  // a thread's moves in flight
 
 struct EvictArgs {
@@ -257,7 +261,7 @@ __device__ __forceinline__ void list_moves(const EvictArgs& a, const Line& x, in
 // for another, and of one wave no barrier.
 //
 // Instructions and waits bound it, not its few bytes.  1440 lines of 703 of 704 places, one
-// wave each: 7.0 us (13.5 without the shortcut for one row); 256 lines of 8191, eight waves:
+// wave each: 7 us (13.5 by the search); 256 lines of 8191, eight waves:
 // 22 us.  More waves for a line wait longer for each other than they count less: lines of
 // 1000 (32 of them, with the moves) 15.7, 18.4, 20.4 us by 1, 4, 8 waves, of 4000 22.8, 24.5,
 // 40.2 by 4, 8, 16, of 8000 29.2 and 48.4 by 8 and 16.
@@ -287,31 +291,53 @@ __global__ __launch_bounds__(64 * W) void choose_kernel(EvictArgs a) {
     for (int i = 0; i < kKeys; ++i) key[i] = keys[64 * i + lane];
   }
 
-  if (held && n - m == 1) {  // the last of the least leaves, and the row behind the budget takes its place
-    uint32_t low = 0xffffffffu, place = 0;
+  // Few rows leave: the last of the least, as often as that, and the rows behind the budget
+  // that are not of them take their places.
+  if (held && n - m <= (W == 1 ? kFewLeave : 1)) {
+    uint32_t taken = 0;  // of this lane's keys, a bit each
+    auto last_of_least = [&]() {
+      uint32_t low = 0xffffffffu, place = 0;
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i)
-      if (j0 + 64 * i + lane < j1 && key[i] <= low) {
-        low = key[i];
-        place = j0 + 64 * i + lane;
+      for (int i = 0; i < kKeys; ++i)
+        if (j0 + 64 * i + lane < j1 && key[i] <= low && !(taken >> i & 1u)) {
+          low = key[i];
+          place = j0 + 64 * i + lane;
+        }
+      const uint32_t least = wave_end<true>(low);
+      return make_uint2(least, wave_end<false>(low == least ? place : 0u));
+    };
+    int32_t *const to = a.to + x.at * a.list_stride, *const from = a.from + x.at * a.list_stride;
+    if constexpr (W == 1) {
+      const int leave = n - m;
+      uint32_t gone = 0, mine = 0xffffffffu;  // of the rows from m on, a bit each; of the leaving ones, lane by lane
+#pragma unroll 1
+      for (int t = 0; t < leave; ++t) {
+        const uint32_t place = last_of_least().y;
+        if ((place & 63) == lane) taken |= 1u << (place >> 6);
+        if (lane == t) mine = place;
+        if (place >= (uint32_t)m) gone |= 1u << (place - m);
       }
-    const uint32_t least = wave_end<true>(low);
-    place = wave_end<false>(low == least ? place : 0u);
-    if (W > 1) {
-      if (lane == 0) s_count[0][wave] = make_uint2(least, place);
+      uint32_t before = 0;  // freed places before this lane's
+#pragma unroll 1
+      for (int t = 0; t < leave && leave > 1; ++t) before += __builtin_amdgcn_readlane(mine, t) < mine;
+      if (mine < (uint32_t)m) to[before] = mine;
+      if (lane < leave && !(gone >> lane & 1u)) from[__popc(~gone & ((1u << lane) - 1u))] = m + lane;
+      if (lane == 0) a.moves[x.at] = leave - __popc(gone);
+    } else {
+      uint2 out = last_of_least();
+      if (lane == 0) s_count[0][wave] = out;
       __syncthreads();
-    }
-    if (tid == 0) {
-      uint2 out = make_uint2(least, place);
-      for (int w = 1; w < W; ++w) {  // (a wave without places tells of the largest key at the first)
-        const uint2 o = s_count[0][w];
-        if (o.x < out.x || (o.x == out.x && o.y > out.y)) out = o;
-      }
-      const bool moves = out.y < (uint32_t)m;
-      a.moves[x.at] = moves;
-      if (moves) {
-        a.to[x.at * a.list_stride] = out.y;
-        a.from[x.at * a.list_stride] = m;
+      if (tid == 0) {
+        for (int w = 1; w < W; ++w) {  // (a wave without places tells of the largest key at the first)
+          const uint2 o = s_count[0][w];
+          if (o.x < out.x || (o.x == out.x && o.y > out.y)) out = o;
+        }
+        const bool moves = out.y < (uint32_t)m;
+        a.moves[x.at] = moves;
+        if (moves) {
+          to[0] = out.y;
+          from[0] = m;
+        }
       }
     }
     return;

@@ -179,6 +179,24 @@ def test_one_row_leaves(mit2, ctx, length, kind):
         Cut(mit2, lengths, [n - 1 for n in lengths], heads=2, page=64, weights=w, stride=length, first=first, last=last, hint=hint, seed=length).check(ctx)
 
 
+@pytest.mark.parametrize("kind", ["any", "equal", "few", "wild"])
+@pytest.mark.parametrize("length", [40, 64, 129, 700, 1024])
+def test_few_rows_leave(mit2, ctx, length, kind):
+    """2 to 33 of a line, those behind the budget among them; all protected, and some places without a page."""
+    rng = np.random.default_rng(length)
+    leave = [2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 32, 33]
+    shape = (1, len(leave), 2, length)
+    w = {"any": rng.exponential(1.0, shape), "equal": np.full(shape, 0.25), "few": rng.integers(0, 3, shape) * 0.5,
+         "wild": rng.choice([np.nan, np.inf, -np.inf, 0.0, -0.0, 1.0], shape)}[kind].astype(np.float32)
+    w[:, :, 0, length - 6:] = -1.0  # (those behind the budget leave, with others or alone)
+    for first, last, born in ((0, 0, False), (3, 4, False), (2 ** 32 - 1, 0, False), (1, 20, True)):
+        c = Cut(mit2, [length] * len(leave), [length - r for r in leave], layers=1, heads=2, page=8, weights=w, stride=length, first=first, last=last, born=born,
+                seed=length)
+        if kind == "few":
+            c.table[:, 2] = -1
+        c.check(ctx)
+
+
 def test_many_sequences_and_layers(mit2, ctx):
     length = [(7 * s) % 40 for s in range(150)]
     Cut(mit2, length, [n // 2 for n in length], layers=5, heads=3, seed=10).check(ctx)
