@@ -657,8 +657,7 @@ mit2cfm_status mit2cfm_kv_norm_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_
  * pages or copies, and which of them are read is not said.  New rows are never taken as
  * shared, whatever shared[g] says: no more are than every sequence of the group that has
  * new rows has before them.  group does not decrease; sequences in no group share nothing.
- * With 16-bit types the probabilities are rounded to the type where a group has more than
- * 16 rows x query heads of a key head on average. */
+ * With 16-bit types the probabilities are a pair of that type, however many rows there are. */
 typedef struct mit2cfm_kv_prefix {
   const int32_t* group;  /* [groups + 1] */
   const int32_t* shared; /* [groups] */

@@ -47,7 +47,9 @@ struct PrefixArgs : AttendArgs {
 };
 
 template <typename A>
-constexpr int wide_blocks = std::is_same<A, PrefixArgs>::value ? 3 : 2;  // of a CU
+constexpr bool is_prefix = std::is_same<A, PrefixArgs>::value;
+template <typename A>
+constexpr int wide_blocks = is_prefix<A> ? 3 : 2;  // of a CU
 
 // What splits leave for their join: [row][query head][split] outputs, maxima and
 // weights' sums, [row][query head] the number of splits.
@@ -544,8 +546,13 @@ __device__ __forceinline__ void score_tile(const typename Mat<T>::op (&kv)[Dims<
 // it: 64 tokens over up to 8191 bf16 keys 297 us with it, 294 without, one over 131001
 // 103 and 102.  Two tiles do not (24 rows of 20 f16 heads of 64 over 3000 keys 39 us,
 // not 36), nor does the block form (trees of 63 rows over up to 4099 f16 keys 68, not
-// 59; a bf16 prompt of 2047 90, not 75).
-template <typename T, int D, int MT, bool WHOLE>
+// 59; a bf16 prompt of 2047 90, not 75).  Shared prefixes have it in all forms, so that a token's
+// precision does not hang on its group's size: 64 tokens on 8191 shared bf16 rows 48 us, not
+// 44, trees of up to 9 rows 60, not 55, prompts of 300 rows 395, not 346.
+//
+// INF: an infinite value's product stays as the first left it: what is left of its weight, 0
+// or less, is no part of it.  Without, the outputs' last step sees to it (infinities).
+template <typename T, int D, int MT, bool WHOLE, bool INF = true>
 __device__ __forceinline__ void add_values(const Piece<T, Dims<T, D>::DP> (&vv)[Dims<T, D>::NV],
                                            const float (&s)[MT][Dims<T, D>::NV], Running<T, D>* run) {
   typedef Dims<T, D> S;
@@ -566,10 +573,10 @@ __device__ __forceinline__ void add_values(const Piece<T, Dims<T, D>::DP> (&vv)[
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         run[mt].o[d] = Mat<T>::mul(v, p[mt], run[mt].o[d]);
-        if (WHOLE) {  // (what is left, 0 or less, of an infinite value's weight is no part of it)
+        if (WHOLE) {
           const floatx4 more = Mat<T>::mul(v, left[mt], run[mt].o[d]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) run[mt].o[d][r] = finite(more[r]) ? more[r] : run[mt].o[d][r];
+          for (int r = 0; r < 4; ++r) run[mt].o[d][r] = !INF || finite(more[r]) ? more[r] : run[mt].o[d][r];
         }
       }
     }
@@ -614,6 +621,34 @@ __device__ __forceinline__ void put_back(const AttendArgs& a, const Part& p, con
 template <typename T>
 __device__ __forceinline__ float taken_out(T v) {
   return finite(v) ? 0.f : (float)v;
+}
+// Outputs that infinite values made NaN: what is left of a weight, 0 or less, times them.
+// Where an output is not finite, the values that stayed in the products, of the split's rows
+// before `end`, are looked at again.
+template <typename T, int D>
+__device__ __forceinline__ void infinities(const AttendArgs& a, const Part& p, int end, int grp, floatx4 (&o)[Dims<T, D>::DP], float weights) {
+  constexpr int DP = Dims<T, D>::DP;
+  bool odd = false;
+#pragma unroll
+  for (int d = 0; d < DP; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) odd = odd | !finite(o[d][r]);
+  if (!odd || !finite(weights)) return;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float met[DP];
+#pragma unroll
+    for (int d = 0; d < DP; ++d) met[d] = 0.f;
+    for (int j = p.begin; j < end; ++j) {
+      const int page = a.c.page_of(p.seq, j);
+      if (page < 0) continue;
+      const T* v = reinterpret_cast<const T*>(a.c.v) + a.c.row_in(page, j, D) + p.kvh * a.c.head_stride(D) + D / 4 * grp + DP * r;
+#pragma unroll
+      for (int d = 0; d < DP; ++d) met[d] += taken_out(v[d]);
+    }
+#pragma unroll
+    for (int d = 0; d < DP; ++d) o[d][r] = met[d] == 0.f ? o[d][r] : met[d];
+  }
 }
 
 // Few query rows: 16 MT of them a block, whose waves take every fourth tile of
@@ -742,7 +777,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(A a, AttendPlan 
       score_tile<T, D>(kv, qv[mt], !all_there || fresh, seen, s[mt]);
       run[mt].weigh(s[mt], a.scale2);
     }
-    add_values<T, D, MT, MT == 1>(vv, s, run);
+    add_values<T, D, MT, MT == 1 || is_prefix<A>>(vv, s, run);
   }
 
   // the join: 16 rows at a time; thread -> row tid / 16, elements DP (tid % 16) ..
@@ -858,8 +893,9 @@ __global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_ke
   constexpr int KEYS = 512 / CPR;                 // keys of a buffer: 8 KB each of keys and values
   constexpr int STEP = kAttendThreads / CPR;      // rows a pass of the block loads
   constexpr int PASSES = KEYS / STEP;             // 2
-  constexpr int WMT = (std::is_same<A, PrefixArgs>::value ? kPrefixRows : wide_rows(sizeof(T) == 4)) / (16 * kAttendWaves);
+  constexpr int WMT = (is_prefix<A> ? kPrefixRows : wide_rows(sizeof(T) == 4)) / (16 * kAttendWaves);
   constexpr int XM = CPR < 16 ? CPR - 1 : 15;
+  constexpr bool WHOLE = is_prefix<A> && sizeof(T) == 2;
   __shared__ __attribute__((aligned(1024))) u32x4 sK0[KEYS * CPR], sK1[KEYS * CPR], sK2[KEYS * CPR];
   __shared__ __attribute__((aligned(1024))) u32x4 sV0[KEYS * CPR], sV1[KEYS * CPR], sV2[KEYS * CPR];
   auto bufK = [&](int b) -> u32x4* { return b == 0 ? sK0 : b == 1 ? sK1 : sK2; };
@@ -1028,7 +1064,7 @@ __global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_ke
           read_keys(bufK(B == 2 ? 0 : B + 1), kv);
         }
         __builtin_amdgcn_s_setprio(1);
-        add_values<T, D, WMT, false>(vv, s, run);
+        add_values<T, D, WMT, WHOLE, false>(vv, s, run);
       }
     };
     for (;;) {
@@ -1043,6 +1079,7 @@ __global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_ke
       one(std::integral_constant<int, 2>{});
     }
   }
+  const int all_see = b0;
   // The other buffers: keys may be missing or new, so that not all rows see them all
   // (query tiles one after the other, for fewer registers).
   bool dirty = false;
@@ -1073,7 +1110,7 @@ __global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_ke
         dirty = dirty || odd;
       }
       run[mt].weigh(s[0], a.scale2);
-      add_values<T, D, 1, false>(vv, s, run + mt);
+      add_values<T, D, 1, WHOLE, false>(vv, s, run + mt);
     }
   };
   for (; b0 < p.end; buf = buf == 2 ? 0 : buf + 1) {
@@ -1088,6 +1125,7 @@ __global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_ke
 #pragma unroll
   for (int mt = 0; mt < WMT; ++mt) {
     const float L = run[mt].sum();
+    if (WHOLE) infinities<T, D>(a, p, min(p.end, max(p.first, all_see)), grp, run[mt].o, L);
     if (wm0 + 16 * mt + lq >= p.mrows) continue;
     const Query x(a, p, qm[mt]);
     const int d0 = D / 4 * grp;
