@@ -653,10 +653,10 @@ mit2cfm_status mit2cfm_kv_norm_append_device(mit2cfm_ctx* ctx, const mit2cfm_kv_
 
 /* mit2cfm_kv_attention of sequences that share their first rows, which are then read
  * once for all of a group's new rows.  The sequences group[g] .. group[g + 1] - 1 share
- * their first shared[g] rows: those have the same contents for each of them, the same
- * pages or copies, and which of them are read is not said.  New rows are never taken as
- * shared, whatever shared[g] says: no more are than every sequence of the group that has
- * new rows has before them.  group does not decrease; sequences in no group share nothing.
+ * their first shared[g] rows: those have the same contents for each of them that has new
+ * rows, the same pages or copies, and which of these are read is not said; sequences without
+ * new rows may hold anything.  New rows are never taken as shared, whatever shared[g] says:
+ * no more are than every sequence of the group that has new rows has before them.  group does not decrease; sequences in no group share nothing.
  * With 16-bit types the probabilities are a pair of that type, however many rows there are. */
 typedef struct mit2cfm_kv_prefix {
   const int32_t* group;  /* [groups + 1] */

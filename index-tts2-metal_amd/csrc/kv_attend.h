@@ -271,22 +271,29 @@ struct Few {
 };
 
 // Rows that the sequences lo .. hi - 1 may share: as many as said, of those before any
-// of their new rows, in whole runs of `step`.  (The same for all lanes.)
-__device__ __forceinline__ int shared_rows(const PrefixArgs& a, const Few& few, int lo, int hi, int said) {
+// of their new rows, in whole runs of `step`; and the first of them that has new rows (-1:
+// none), whose pages are read: the others' may be anything.  (The same for all lanes.)
+struct Sharing {
+  int rows, reader;
+};
+__device__ __forceinline__ Sharing shared_rows(const PrefixArgs& a, const Few& few, int lo, int hi, int said) {
   const int lane = threadIdx.x & 63;
-  int least = min(said, a.c.capacity());
+  int least = min(said, a.c.capacity()), reader = -1;
+  auto look = [&](int base, bool in, int start, int stop, auto&& length) {
+    in = in && stop > start;
+    if (in) least = min(least, length() - (stop - start));
+    const uint64_t have = __ballot(in);
+    if (have && reader < 0) reader = base + __ffsll((unsigned long long)have) - 1;
+  };
   if (few.all) {
-    if (lane >= lo && lane < hi && few.stop > few.start) least = min(least, few.length - (few.stop - few.start));
+    look(0, lane >= lo && lane < hi, few.start, few.stop, [&] { return few.length; });
   } else {
     for (int base = lo; base < hi; base += 64) {
-      const int s = base + lane;
-      if (s < hi) {
-        const int s0 = a.r.start[s], s1 = a.r.start[s + 1];
-        if (s1 > s0) least = min(least, a.r.length[s] - (s1 - s0));
-      }
+      const int s = min(base + lane, hi - 1);
+      look(base, base + lane < hi, a.r.start[s], a.r.start[s + 1], [&] { return a.r.length[s]; });
     }
   }
-  return max(wave_min(least), 0) & -a.step;
+  return {max(wave_min(least), 0) & -a.step, reader};
 }
 // A sequence's own rows (see Part).
 __device__ __forceinline__ bool find_own(const PrefixArgs& a, const Few& few, int mtile, int tile, Part& p) {
@@ -326,7 +333,7 @@ __device__ __forceinline__ bool find_own(const PrefixArgs& a, const Few& few, in
     if (!mine) continue;
     const int l = __ffsll((unsigned long long)mine) - 1;
     from = shared_rows(a, few, max(__builtin_amdgcn_readlane(lo, l), 0), min(__builtin_amdgcn_readlane(hi, l), a.r.seqs),
-                       __builtin_amdgcn_readlane(said, l));
+                       __builtin_amdgcn_readlane(said, l)).rows;
     break;
   }
   const int chunk = chunk_of(p.len - from, a.own.chunk, a.own.splits);
@@ -362,12 +369,13 @@ __device__ __forceinline__ bool find_shared(const PrefixArgs& a, const AttendPla
     }
     const int l = run_of(some ? tiles_of(a, start, stop, mtile) : 0, tile, before);
     if (l < 0) continue;
-    p.seq = __builtin_amdgcn_readlane(lo, l);
     p.raw_start = __builtin_amdgcn_readlane(start, l);
     p.start = max(p.raw_start, 0);
     p.mrows = (min(__builtin_amdgcn_readlane(stop, l), a.r.rows) - p.start) * a.group;
     p.m0 = (tile - before) * mtile;
-    p.len = p.first = shared_rows(a, few, p.seq, __builtin_amdgcn_readlane(hi, l), __builtin_amdgcn_readlane(said, l));
+    const Sharing of = shared_rows(a, few, __builtin_amdgcn_readlane(lo, l), __builtin_amdgcn_readlane(hi, l), __builtin_amdgcn_readlane(said, l));
+    p.seq = max(of.reader, 0);
+    p.len = p.first = of.rows;
     const int chunk = chunk_of(p.len, plan.chunk, plan.splits);
     p.begin = p.split * chunk;
     p.end = min(p.begin + chunk, p.len);
