@@ -19,20 +19,9 @@ struct WeighArgs {
   int32_t* born;
 };
 
-struct WeighPlan {
-  int by_query;     // a block's waves share their keys and divide the queries
-  uint32_t blocks;  // of a sequence and key head
-  int by_xcd;       // those on one XCD, whose L2 then has their queries
-};
-
 void launch_weigh_f32(const WeighArgs& w, const WeighPlan& plan, int D, hipStream_t s);
 void launch_weigh_f16(const WeighArgs& w, const WeighPlan& plan, int D, hipStream_t s);
 void launch_weigh_bf16(const WeighArgs& w, const WeighPlan& plan, int D, hipStream_t s);
-
-// 16-key tiles of a wave: up to 64 keys, 16 KB of them.
-constexpr int weigh_tiles(int D, int bytes) {
-  return D * bytes <= 256 ? 4 : D * bytes <= 512 ? 2 : 1;
-}
 
 #if defined(KV_ATTEND_KERNELS)
 
@@ -412,7 +401,8 @@ __global__ __launch_bounds__(kAttendThreads, (BYQ && sizeof(T) == 2 && D <= 128)
 template <typename T, int D>
 void launch_weigh(const WeighArgs& w, const WeighPlan& plan, hipStream_t s) {
   const uint32_t lines = (uint32_t)w.a.c.kv_heads * w.a.r.seqs;
-  const dim3 grid = plan.by_xcd ? dim3(8 * ((lines + 7) / 8) * plan.blocks) : dim3(plan.blocks, w.a.c.kv_heads, w.a.r.seqs);
+  const uint32_t x = weigh_grid(plan, lines);
+  const dim3 grid = plan.by_xcd ? dim3(x) : dim3(x, w.a.c.kv_heads, w.a.r.seqs);
   const dim3 block(kAttendThreads);
   if (plan.by_query)
     hipLaunchKernelGGL((weigh_kernel<T, D, true>), grid, block, 0, s, w, plan);

@@ -1,5 +1,5 @@
 // kv_weigh.hip -- adding up the attention weight that cached rows get: its arguments
-// and how its launch is laid out (the kernels: kv_weigh.h).
+// (the kernels: kv_weigh.h; how their launch is laid out: kv_plan.h).
 #include "kv_weigh.h"
 
 #include <algorithm>
@@ -59,29 +59,7 @@ void kv_weigh(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r, const mit2cfm
   w.position = p.position;
   w.born = p.born;
   const int D = (int)c.head_dim;
-  WeighPlan plan;
-  const uint64_t len = std::min<uint64_t>({r.max_length, (uint64_t)c.table_stride * c.page_rows, p.weight_stride});
-  const uint64_t lines = (uint64_t)r.seqs * c.kv_heads;
-  const uint64_t wave_keys = 16 * weigh_tiles(D, (int)e), all_blocks = lines * ((len + 4 * wave_keys - 1) / (4 * wave_keys));
-  // Waves that divide the queries make four times the blocks, and each loads all of its
-  // block's keys: worth it while the blocks of waves with keys of their own do not fill
-  // the chip, or where the queries take longer than that.  2047 f16 keys of 128, 8 key
-  // heads, 4 query heads each, us with keys of their own / queries divided:
-  //              16 rows      64 rows      256 rows     1029 rows
-  //   1 prompt   10.0 / 8.7   24.8 / 13.0  54.1 / 20.5
-  //   4 prompts  10.3 / 19.6  25.5 / 26.8  66.1 / 44.8  238 / 111
-  //   16         26.0 / 56.9  59.4 / 74.0  138 / 134    496 / 339
-  const uint64_t each = p.last_rows ? std::min<uint64_t>(r.rows, (uint64_t)r.seqs * p.last_rows) : r.rows;
-  const uint64_t tiles = each * a.group / r.seqs / 16;  // of queries, on average
-  plan.by_query = tiles > std::clamp<uint64_t>(all_blocks / 16, 2, 64);
-  const uint64_t keys = wave_keys * (plan.by_query ? 1 : kAttendWaves);
-  // With keys of their own, no more blocks than 8 a CU, each then has several chunks: 64
-  // sequences of up to 8191 keys 164 us (4 a CU 172, 16 a CU 169, one for each chunk 213).
-  const uint64_t most = plan.by_query ? 1u << 20 : std::max<uint64_t>(1, 2048 / lines);
-  plan.blocks = (uint32_t)std::clamp<uint64_t>((len + keys - 1) / keys, 1, most);
-  // A line's blocks on one XCD, whose L2 has their queries: 4 ragged prompts of 1029 rows
-  // 65 us (in launch order 94), 16 of 64 rows 56 (66).
-  plan.by_xcd = plan.by_query && (lines % 8 == 0 || lines >= 32) && (lines + 7) * plan.blocks < (1u << 23);
+  const WeighPlan plan = weigh_plan(c, r, p.q_heads, p.last_rows, p.weight_stride);
   if (c.dtype == MIT2CFM_DTYPE_F32)
     launch_weigh_f32(w, plan, D, s);
   else if (c.dtype == MIT2CFM_DTYPE_F16)
