@@ -681,7 +681,8 @@ mit2cfm_status mit2cfm_kv_prefix_attention_device(mit2cfm_ctx* ctx, const mit2cf
  * is new itself, and had no weight, without the first term.  Who sees what: as for
  * mit2cfm_kv_attention.  lse is mit2cfm_kv_prefix_attention's; a row of -inf adds nothing.
  * Places without a page get the first term alone; places from a sequence's length on, and
- * sequences without new rows, are left alone.  Sums are fp32, in the same order each time. */
+ * sequences without new rows, are left alone.  Sums are fp32, in an order that is the same
+ * each time for equal sizes (rows, seqs, last_rows, weight_stride, the cache's) and max_length. */
 typedef struct mit2cfm_kv_weigh {
   const void* q; /* [rows][q_heads][head_dim] by q_row, q_head */
   uint64_t q_row, q_head;

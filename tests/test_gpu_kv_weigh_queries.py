@@ -156,6 +156,31 @@ def test_hints(mit2, ctx):  # noqa: F811
         assert torch.equal(w.run(ctx).nan_to_num(-1.0), first.nan_to_num(-1.0))
 
 
+@pytest.mark.parametrize("c", cases.HINTED, ids=_name)
+def test_hints_that_choose_the_form(mit2, ctx, c):  # noqa: F811
+    """Any hint is right; where hints choose another form its sums go in another order, and bits are each form's own, the same each time."""
+    b = _batch(c)
+    ref, tol = None, None
+    for hints in (cases.FEW, cases.MANY):
+        first = None
+        for hint in hints:
+            w = Weigh(mit2, b)
+            w.on.rows.max_length = hint
+            raw = w.run(ctx)
+            if ref is None:
+                ref, tol = weigh64(b, w.lse, w.weights, w.scale)
+                for s, n in enumerate(b.length):
+                    ref[s, :, n:] = 0.0
+            if first is None:
+                first = raw
+            assert torch.equal(raw.nan_to_num(-1.0), first.nan_to_num(-1.0)) and torch.equal(w.run(ctx).nan_to_num(-1.0), first.nan_to_num(-1.0))
+        got = first.clone()
+        for s, n in enumerate(b.length):
+            assert bool(torch.isnan(got[s, :, n:]).all())
+            got[s, :, n:] = 0.0
+        check(got, ref, tol, f"hints {hints}")
+
+
 def test_offsets_past_32_bits(mit2, ctx):  # noqa: F811
     """Keys in the last pages of a cache of over 2^32 elements, queries and weights over 2^31 elements in."""
     pages, heads, page, dim, new = 70000, 8, 64, 128, 130

@@ -45,3 +45,10 @@ def test_sizes_reach_the_waves_that_divide_the_queries(mit2, exe):
         assert by_query and bool(by_xcd) == c["by_xcd"], (c, stride, by_query, blocks, by_xcd)
     for hint in (0, 1, 100, 1 << 20, 2 ** 32 - 1):
         assert plans(mit2, exe, [(Batch(**cases.LONG["args"]), 0, None, hint)])[0][0], hint
+
+
+def test_the_said_length_chooses_the_form(mit2, exe):
+    for c in cases.HINTED:
+        b = Batch(**c["args"])
+        assert all(by_query for by_query, _, _ in plans(mit2, exe, [(b, 0, None, hint) for hint in cases.FEW])), c
+        assert not any(by_query for by_query, _, _ in plans(mit2, exe, [(b, 0, None, hint) for hint in cases.MANY])), c

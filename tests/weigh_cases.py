@@ -29,3 +29,6 @@ OTHERS = dict(in_place=case([100, 0, 90], [100, 7, 90], dim=64, heads=(2, 1), dt
 LAST = 70  # rows that are counted of `last`
 FINITE = [case([130, 90], [90, 40], dim=dim, heads=(2, 1), dtype=dtype) for dim, dtype in ((64, "f32"), (128, "bf16"), (96, "f16"))]
 QUERIES = [case([100, 130], [60, 200], dim=dim, heads=(4, 2), dtype=dtype) for dim, dtype in ((32, "f16"), (64, "f16"), (64, "f32"), (128, "bf16"), (128, "f32"), (192, "f16"))]
+# The form follows the length that the rows are said to have: up to FEW the queries are divided, from MANY on the keys.
+HINTED = [case([40] * 16, [(1990 if s == 5 else 60 + 7 * s) for s in range(16)], dim=dim, heads=(16, 4), dtype=dtype) for dim, dtype in ((64, "bf16"), (128, "f32"))]
+FEW, MANY = (0, 1, 256), (1990, 1 << 20, 2 ** 32 - 1)
