@@ -18,8 +18,8 @@ constexpr int kSplitKeys = kSplitWaves * kWaveKeys;  // a segment's, where the l
 constexpr int kBins = 2048;
 constexpr int kMaxSegments = 64;
 // Rows that leave a line of one wave are found one after the other up to this many: 1440
-// lines of 704 places, with the moves, 10.8, 11.5, 12.8, 16.0, 18.5 us for 1, 2, 4, 8, 12 rows,
-// by the search 16.2 to 18.6 (one row 18.9).
+// lines of 704 places, with the moves, on the same data again and again, 10.7, 11.5, 12.8, 16.0,
+// 18.5 us for 1, 2, 4, 8, 12 rows, by the search 16.2 to 18.6 (one row 18.9).
 constexpr int kFewLeave = 8;
 constexpr int kMoveThreads = 256, kMoveBatch = 2;  // a thread's moves in flight
 
@@ -823,7 +823,7 @@ void kv_evict(const mit2cfm_kv_cache& c, const mit2cfm_kv_evict& p, hipStream_t 
   kv_launched(hipGetLastError());
   // 16 blocks a CU, of a line no more than its moves want, half its places at most: 256
   // lines of 2048 moves 75 us (4 a CU 80); but lines that are 4 a CU themselves have one
-  // block each: 1440 of them with a move each 10.8 us (two blocks each 11.9, eleven 17.2).
+  // block each: 1440 of them with a move each 10.7 us (two blocks each 11.9, eleven 17.2).
   const uint64_t per = kMoveThreads / a.row16 * kMoveBatch;
   const uint64_t wanted = lines >= 1024 ? 1 : 4096 / lines;
   const int chunks = (int)std::min(wanted, (len / 2 + per - 1) / per + 1);

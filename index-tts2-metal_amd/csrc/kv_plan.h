@@ -28,7 +28,7 @@ constexpr int wide_rows(bool f32) { return f32 ? 64 : 128; }
 constexpr bool wide_dim(int D) { return D == 64 || D == 128; }
 
 // The same where prefixes are shared: three blocks fit on a CU (64 tokens on one prefix of
-// 8191 bf16 rows 42 us, with 128 rows and two blocks 54, and parts of twice the bytes).
+// 8191 bf16 rows 48 us, with 128 rows and two blocks 70, and parts of twice the bytes).
 constexpr int kPrefixRows = 64;
 constexpr int kBlocksWanted = 1024;   // four blocks of the small tiles a CU
 // Blocks of the wide form that run at once on 256 CUs: two a CU at 128 elements of
@@ -214,11 +214,12 @@ inline WeighPlan weigh_plan(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& r,
   // Waves that divide the queries make four times the blocks, and each loads all of its
   // block's keys: worth it while the blocks of waves with keys of their own do not fill
   // the chip, or where the queries take longer than that.  2047 f16 keys of 128, 8 key
-  // heads, 4 query heads each, us with keys of their own / queries divided:
+  // heads, 4 query heads each, prompts of as many rows, us with keys of their own / queries
+  // divided:
   //              16 rows      64 rows      256 rows     1029 rows
-  //   1 prompt   10.0 / 8.7   24.8 / 13.0  54.1 / 20.5
-  //   4 prompts  10.3 / 19.6  25.5 / 26.8  66.1 / 44.8  238 / 111
-  //   16         26.0 / 56.9  59.4 / 74.0  138 / 134    496 / 339
+  //   1 prompt   10.0 / 9.0   24.9 / 13.1  54.2 / 21.0  225 / 52
+  //   4 prompts  10.2 / 19.7  25.7 / 27.2  66.2 / 44.6  236 / 107
+  //   16         25.7 / 56.5  60.4 / 74.1  139 / 129    496 / 319
   const uint64_t each = last_rows ? std::min<uint64_t>(r.rows, (uint64_t)r.seqs * last_rows) : r.rows;
   const uint64_t tiles = each * group / r.seqs / 16;  // of queries, on average
   WeighPlan plan;

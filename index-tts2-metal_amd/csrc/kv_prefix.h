@@ -17,7 +17,7 @@ void launch_prefix_bf16(const PrefixArgs& a, const PrefixPlan& plan, int D, void
 // Joins the parts of a row and query head: those of the shared rows, then its
 // sequence's own.  Lane groups of D/4 take every so manyth part, four elements a lane,
 // AHEAD of them at once; WAVES of them for more parts than those.  Its parts' way through
-// the cache bounds it: 48 trees of up to 9 rows, 32 heads of 128, 8 us beside the parts' 47.
+// the cache bounds it: 48 trees of up to 9 rows, 32 heads of 128, 8 us beside the parts' 52.
 constexpr int kJoinFew = 16;
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void join_kernel(PrefixArgs a, int shared_splits, Parts part, float* lse) {

@@ -64,11 +64,11 @@ __device__ __forceinline__ void load_row(const T* q, bool wide, int grp, typenam
 //
 // Waves of their own keys: the cache's bytes bound it, 64 tokens over up to 8191 bf16 keys of
 // 128 in 8 heads 164 us, 4.75 TB/s.  Shared keys: the products and exponentials, 16 prompts of
-// 1029 rows, 32 heads, over 2047 f16 keys 317 us, 650 TFLOP/s.
+// 1029 rows, 32 heads, over 2047 f16 keys 319 us, 650 TFLOP/s.
 //
 // The third block of a CU is worth the few registers that 16-bit rows of 256 bytes spill
-// for it: 4 ragged prompts of 1029 rows 63 us for 76, even ones 103 for 110 (of 512 rows 66
-// for 63); f32 rows, bound by their products, lose.
+// for it: 4 ragged prompts of 1029 rows 70 us for 80, even ones 107 for 110 (of 512 rows 67
+// for 63), 16 even ones 319 for 369; f32 rows, bound by their products, lose.
 template <typename T, int D, bool BYQ>
 __global__ __launch_bounds__(kAttendThreads, (BYQ && sizeof(T) == 2 && D <= 128) ? 3 : 2) void weigh_kernel(WeighArgs w, WeighPlan plan) {
   typedef Dims<T, D> S;
