@@ -632,30 +632,39 @@ __device__ __forceinline__ float taken_out(T v) {
 }
 // Outputs that infinite values made NaN: what is left of a weight, 0 or less, times them.
 // Where an output is not finite, the values that stayed in the products, of the split's rows
-// before `end`, are looked at again.
+// before `end` (all of them seen by all of the wave's queries), are looked at again, every
+// 16th row by a lane: with one infinite value 64 tokens on 8191 shared bf16 rows take 142 us,
+// without 50.
 template <typename T, int D>
-__device__ __forceinline__ void infinities(const AttendArgs& a, const Part& p, int end, int grp, floatx4 (&o)[Dims<T, D>::DP], float weights) {
+__device__ __forceinline__ void infinities(const AttendArgs& a, const Part& p, int end, floatx4 (&o)[Dims<T, D>::DP], float weights) {
   constexpr int DP = Dims<T, D>::DP;
+  const int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), lq = lane & 15, grp = lane >> 4;  // (not held until here)
   bool odd = false;
 #pragma unroll
   for (int d = 0; d < DP; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r) odd = odd | !finite(o[d][r]);
-  if (!odd || !finite(weights)) return;
+  odd = odd && finite(weights);
+  if (!__any(odd)) return;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+  for (int r = 0; r < 4; ++r) {  // (one after the other, for fewer registers)
     float met[DP];
 #pragma unroll
     for (int d = 0; d < DP; ++d) met[d] = 0.f;
-    for (int j = p.begin; j < end; ++j) {
+    for (int j = p.begin + lq; j < end; j += 16) {
       const int page = a.c.page_of(p.seq, j);
       if (page < 0) continue;
       const T* v = reinterpret_cast<const T*>(a.c.v) + a.c.row_in(page, j, D) + p.kvh * a.c.head_stride(D) + D / 4 * grp + DP * r;
+      const Piece<T, DP> x = *reinterpret_cast<const Piece<T, DP>*>(v);
 #pragma unroll
-      for (int d = 0; d < DP; ++d) met[d] += taken_out(v[d]);
+      for (int d = 0; d < DP; ++d) met[d] += taken_out(x.v[d]);
     }
 #pragma unroll
-    for (int d = 0; d < DP; ++d) o[d][r] = met[d] == 0.f ? o[d][r] : met[d];
+    for (int d = 0; d < DP; ++d) {
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) met[d] += __shfl_xor(met[d], off, kWave);
+      o[d][r] = odd && met[d] != 0.f ? met[d] : o[d][r];
+    }
   }
 }
 
@@ -1133,7 +1142,7 @@ __global__ __launch_bounds__(kAttendThreads, wide_blocks<A>) void attend_wide_ke
 #pragma unroll
   for (int mt = 0; mt < WMT; ++mt) {
     const float L = run[mt].sum();
-    if (WHOLE) infinities<T, D>(a, p, min(p.end, max(p.first, all_see)), grp, run[mt].o, L);
+    if (WHOLE) infinities<T, D>(a, p, min(p.end, max(p.first, all_see)), run[mt].o, L);
     if (wm0 + 16 * mt + lq >= p.mrows) continue;
     const Query x(a, p, qm[mt]);
     const int d0 = D / 4 * grp;
