@@ -710,11 +710,12 @@ mit2cfm_status mit2cfm_kv_weigh_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache*
  * ones the lowest place first (a NaN counts as less than all, and so does a place without a
  * page; a row that moves to one is lost).  Protected rows are equal: where keep[s] is less than
  * there are of them, those in the lowest places stay (without births the newest leave), so give
- * a budget of first_rows + last_rows at least.  The rows that stay from place keep[s] on move down: the i-th
- * of them in order goes to the i-th place below keep[s] that a row left.  Everything else stays where it is, so places
- * tell ages no more: give born where a cache is cut again and again.  Keys keep the
- * rotation they were appended with; new rows are appended at positions of the caller's.
- * Pages that sequences share must lie below first_rows (others are written to). */
+ * a budget of first_rows + last_rows at least.  The rows that stay from place keep[s] on move
+ * down: the i-th of them in order goes to the i-th place below keep[s] that a row left.
+ * Everything else stays where it is, so places tell ages no more: give born where a cache is
+ * cut again and again.  Keys keep the rotation they were appended with; new rows are appended
+ * at positions of the caller's.  Pages that sequences share must lie below first_rows (others
+ * are written to). */
 typedef struct mit2cfm_kv_evict {
   uint32_t seqs;           /* 0 .. 65535 */
   uint32_t layers;         /* >= 1; the cache's k and v are the first's; layers * seqs * kv_heads <= 2^24 */
