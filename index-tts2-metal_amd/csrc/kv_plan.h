@@ -143,7 +143,8 @@ inline PrefixPlan prefix_plan(const mit2cfm_kv_cache& c, const mit2cfm_kv_rows& 
   p.shared.tiles = shares ? attend_tiles(c, some, q_heads, mtile) : 0;
   p.own.tiles = attend_tiles(c, r, q_heads, mtile);
   const uint64_t shared_len = shares ? attend_length(c, x.max_shared) : 0;
-  const uint64_t own_len = attend_length(c, !shares ? r.max_length : r.max_length > x.max_shared ? r.max_length - x.max_shared + shared_step(D, f32) - 1 : 1);
+  const uint64_t past = r.max_length > x.max_shared ? (uint64_t)r.max_length - x.max_shared + shared_step(D, f32) - 1 : 1;
+  const uint64_t own_len = attend_length(c, shares ? past : r.max_length);
   const uint64_t step = p.own.form == kWide ? wide_keys(D, f32) : chunk_step(f32), longest = std::max(shared_len, own_len);
   auto splits = [](uint64_t len, uint64_t chunk) { return (len + chunk - 1) / chunk; };
   // What a chunk costs, in a block's steps on a CU (0.5 us each where its places are
