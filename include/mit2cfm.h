@@ -718,7 +718,7 @@ mit2cfm_status mit2cfm_kv_weigh_device(mit2cfm_ctx* ctx, const mit2cfm_kv_cache*
  * are written to). */
 typedef struct mit2cfm_kv_evict {
   uint32_t seqs;           /* 0 .. 65535 */
-  uint32_t layers;         /* >= 1; the cache's k and v are the first's; layers * seqs * kv_heads <= 2^24 */
+  uint32_t layers;         /* 1 .. 16384; the cache's k and v are the first's; layers * seqs * kv_heads <= 2^24 */
   uint64_t layer_stride;   /* elements from a layer's k (v) to the next's: a multiple of 8, a layer's at least */
   const int32_t* length;   /* [seqs] */
   const int32_t* keep;     /* [seqs]; negative counts as 0 */
@@ -792,7 +792,7 @@ mit2cfm_status mit2cfm_beam_select_device(mit2cfm_ctx* ctx, const mit2cfm_beam_s
 typedef struct mit2cfm_beam_reorder {
   uint32_t groups;        /* groups * beams <= 2^20 */
   uint32_t beams;         /* 1 .. 64 */
-  uint32_t layers;        /* >= 1; the cache's k and v are the first's */
+  uint32_t layers;        /* 1 .. 16384; the cache's k and v are the first's */
   uint64_t layer_stride;  /* elements from a layer's k (v) to the next's: a multiple of 8, a layer's at least */
   const int32_t* parent;  /* [groups][beams], rows parent_stride apart */
   uint32_t parent_stride; /* >= beams */
